@@ -14,9 +14,11 @@ from ._lib import get_keep_samples, get_math_mode, set_keep_samples, set_math_mo
 from . import dconv_native, fast_depthwise_conv3d
 from .dconv_native import (DConv3d, DeformConv3d, MDConv3d, deform_conv3d, dyn_dilated_conv3d)
 from .fast_depthwise_conv3d import DepthwiseConv3d
+from .tokens import CrossAttention3d, LayerNorm3d, cross_attention, layer_norm, rotary_embedding_3d
 
 __all__ = ["dconv_native", "fast_depthwise_conv3d", "deform_conv3d", "dyn_dilated_conv3d", "DeformConv3d",
-           "DConv3d", "MDConv3d", "DepthwiseConv3d", "set_math_mode", "get_math_mode", "set_keep_samples", "get_keep_samples",
+           "DConv3d", "MDConv3d", "DepthwiseConv3d", "layer_norm", "rotary_embedding_3d", "cross_attention", "LayerNorm3d",
+           "CrossAttention3d", "set_math_mode", "get_math_mode", "set_keep_samples", "get_keep_samples",
            "install_as_dropin"]
 
 

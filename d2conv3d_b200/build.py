@@ -16,13 +16,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libd2conv3d.so")
-TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_tokens.cpp")]
+TORCH_DEPS = TORCH_SRCS + [os.path.join(CSRC, "torch_common.h"), os.path.join(INCLUDE, "d2conv3d.h")]
 TORCH_LIB = os.path.join(HERE, "_C.so")
 OBJ_DIR = os.path.join(HERE, "build")
 TORCH_STAMP = os.path.join(OBJ_DIR, "torch_ops.stamp")
 
 SOURCES = ["d2c_api.cu", "depthwise.cu", "deform_sm100_fwd.cu", "deform_sm100_bwd.cu", "deform_sm100_dw.cu",
-           "deform_exact_f32.cu", "deform_exact_f64.cu", "act_norm.cu"]
+           "deform_exact_f32.cu", "deform_exact_f64.cu", "act_norm.cu", "layer_norm.cu", "rotary.cu", "attention_exact.cu",
+           "attention_api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE,
@@ -36,7 +38,7 @@ def _nvcc():
 def _deps():
     out = [os.path.join(INCLUDE, "d2conv3d.h")]
     for f in os.listdir(CSRC):
-        if not f.endswith(".cpp"):
+        if not f.endswith(".cpp") and not f.startswith("torch_"):
             out.append(os.path.join(CSRC, f))
     return out
 
@@ -61,11 +63,11 @@ def _torch_needs_build():
         if f.read() != _torch_stamp():
             return True
     t = os.path.getmtime(TORCH_LIB)
-    return any(os.path.getmtime(d) > t for d in (TORCH_SRC, os.path.join(INCLUDE, "d2conv3d.h")))
+    return any(os.path.getmtime(d) > t for d in TORCH_DEPS)
 
 
 def build_torch(force=False):
-    """The PyTorch front-end _C.so: csrc/torch_ops.cpp against the installed torch, linked to libd2conv3d.so (which it
+    """The PyTorch front-end _C.so: csrc/torch_*.cpp against the installed torch, linked to libd2conv3d.so (which it
     finds beside itself)."""
     if not force and not _torch_needs_build():
         return TORCH_LIB
@@ -79,7 +81,7 @@ def build_torch(force=False):
     cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
            + [a for i in inc for a in ("-isystem", i)]
-           + [TORCH_SRC, "-o", TORCH_LIB, "-L", lib_dir, "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda",
+           + TORCH_SRCS + ["-o", TORCH_LIB, "-L", lib_dir, "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda",
               "-ltorch_python", "-L", HERE, "-l:libd2conv3d.so", "-L", "/usr/local/cuda/lib64", "-lcudart",
               "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib_dir}"])
     p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)

@@ -1,0 +1,52 @@
+// Cross attention: what its kernels share (attention_exact.cu: CUDA cores, any type and head width; attention_sm100.cu: tensor
+// cores, 16-bit types) and the host side that chooses between them (attention_api.cu).
+#pragma once
+
+#include "token_common.cuh"
+
+namespace d2c {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  const void *q, *k, *v, *g, *o_in;      // g, o_in: gradient of the output and the output (backward)
+  void *o, *gq, *gk, *gv;
+  float* lse;                            // [B, Hq, Lq]: log2 of the sum of exp2(scores in log2 units); -inf without keys
+  float* delta;                          // [B, Hq, Lq]: sum_d grad_o * o
+  const void* lengths;
+  int lengths_i64;
+  int B, Lq, Lk, Hq, Hkv, D;
+  float scale;
+  long long qs[3], ks[3], vs[3], gs[3];  // batch, token, head
+  int splits;                            // shares of the inner loop; > 1: partial results
+  float* part;                           // forward [splits][B, Lq, Hq][D]; grad_q the same; grad_k, then grad_v [splits][B, Lk, Hkv][D]
+  float* part_lse;                       // forward [splits][B, Lq, Hq]
+};
+
+// Valid keys of clip b.
+__device__ __forceinline__ int key_length(const Args& a, int b) {
+  if (!a.lengths) return a.Lk;
+  const long long n = a.lengths_i64 ? reinterpret_cast<const long long*>(a.lengths)[b]
+                                    : (long long)reinterpret_cast<const int*>(a.lengths)[b];
+  return (int)(n < 0 ? 0 : (n > a.Lk ? a.Lk : n));
+}
+
+// Share [begin, end) of n items, of `splits`.
+__device__ __forceinline__ void share(int n, int splits, int s, int& begin, int& end) {
+  begin = (int)((long long)n * s / splits);
+  end = (int)((long long)n * (s + 1) / splits);
+}
+
+// ---- attention_exact.cu
+enum { kTile = 64, kFewRows = 4 };
+int exact_fwd(int dtype, const Args& a, cudaStream_t st);
+int few_fwd(int dtype, const Args& a, cudaStream_t st);          // needs 16-byte rows: see few_fits
+int exact_bwd_q(int dtype, const Args& a, cudaStream_t st);
+int exact_bwd_kv(int dtype, const Args& a, cudaStream_t st);
+int combine(int dtype, const Args& a, cudaStream_t st);          // partial outputs -> o, lse
+int delta_rows(int dtype, const Args& a, cudaStream_t st);
+int sum_parts(int dtype, const float* part, int splits, long long n, void* out, cudaStream_t st);
+
+}  // namespace attn
+}  // namespace d2c

@@ -80,6 +80,7 @@ static int status_take() {
   *w = 0;
   return D2C_ERR_DEVICE_TIMEOUT;
 }
+int take_device_status() { return status_take(); }
 #define D2C_TAKE_STATUS()                      \
   do {                                         \
     const int _st = ::d2c::status_take();      \
@@ -289,6 +290,7 @@ const char* d2c_status_string(int status) {
     case D2C_ERR_WEIGHT_SHAPE: return "weight shape does not match the channel counts";
     case D2C_ERR_SCRATCH_LIMIT:
       return "out_channels * kernel taps exceeds the 32768 accumulator slots of the built-in scratch buffer";
+    case D2C_ERR_ALIGN: return "a pointer or stride is not aligned as the op asks";
     case D2C_ERR_CUDA: return "CUDA runtime error";
     case D2C_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait gave up";
     default: return "unknown status";

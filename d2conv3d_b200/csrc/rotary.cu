@@ -1,0 +1,195 @@
+// Rotary positions with three axes (time, height, width): the channels of a head are cut into one section per axis and a
+// rest; pair i of section a turns by the angle p_a * base^(-2 i / n_a), n_a the section's channels, p_a the token's
+// position on that axis; the rest stays.  The gradient is the same with the angle's sign changed.
+//
+// HBM-bound: 2 * sizeof(T) bytes per element.  A thread holds the same pairs of every token it meets, so that their
+// frequencies are formed once; the angle is formed once per token and used for all heads.  Angles: position times
+// frequency in turns, in 64 bits, its whole turns taken off, then sin and cos in 32 bits: at position 100 000 a 32-bit
+// product would be off by thousandths of a turn.
+#include <algorithm>
+
+#include "token_common.cuh"
+
+namespace d2c {
+namespace {
+
+struct RotaryArgs {
+  const void *x, *positions;
+  void* y;
+  long long tokens;                  // batch * length
+  long long sb, sl, sh;              // strides of x; y is contiguous
+  long long pos_batch;               // positions' elements between two batch entries (0: shared)
+  int length, heads, dim;
+  int n[3];                          // channels of the sections
+  int pos_kind;
+  int grid_h, grid_w;
+  double step[3], first[3];          // grid positions: index * step + first
+  double log2_base;
+  float sign;
+};
+
+// V pairs of a thread: channels u0 .. and v0 .. (halves of a section), or 2 V neighbouring channels.
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
+  const int j = threadIdx.x * V;                                 // first pair of this thread
+  // section of the pair: the three axes, then the rest
+  int axis = 0, start = 0, i = j;
+  while (axis < 3 && i >= a.n[axis] / 2) {
+    i -= a.n[axis] / 2;
+    start += a.n[axis];
+    ++axis;
+  }
+  const bool turns = axis < 3;
+  const int half = (turns ? a.n[axis] : a.dim - start) / 2;
+  if (!turns && i >= half) return;                               // block rounded up to whole warps
+  const int u0 = kInterleaved ? start + 2 * i : start + i, v0 = start + i + half;
+  double freq[V];                                                // turns per position
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    freq[e] = turns ? exp2(-2.0 * (i + e) / a.n[axis] * a.log2_base) * 0.15915494309189533577 : 0.0;
+  for (long long tok = (long long)blockIdx.x * blockDim.y + threadIdx.y; tok < a.tokens; tok += (long long)gridDim.x * blockDim.y) {
+    const long long b = tok / a.length;
+    const int l = (int)(tok - b * a.length);
+    float c[V], s[V];
+    if (turns) {
+      double pos;
+      if (a.pos_kind == D2C_POS_GRID) {
+        const int row = l / a.grid_w, idx = axis == 2 ? l - row * a.grid_w : (axis == 1 ? row % a.grid_h : row / a.grid_h);
+        pos = idx * a.step[axis] + a.first[axis];
+      } else {
+        const long long at = b * a.pos_batch + (long long)l * 3 + axis;
+        pos = a.pos_kind == D2C_POS_I32   ? (double)reinterpret_cast<const int*>(a.positions)[at]
+              : a.pos_kind == D2C_POS_I64 ? (double)reinterpret_cast<const long long*>(a.positions)[at]
+                                          : (double)reinterpret_cast<const float*>(a.positions)[at];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double t = pos * freq[e];
+        sincospif(2.f * (float)(t - rint(t)), &s[e], &c[e]);
+        s[e] *= a.sign;
+      }
+    }
+    const T* x = reinterpret_cast<const T*>(a.x) + b * a.sb + (long long)l * a.sl;
+    T* y = reinterpret_cast<T*>(a.y) + tok * a.heads * a.dim;
+#pragma unroll 4
+    for (int h = 0; h < a.heads; ++h, x += a.sh, y += a.dim) {
+      if constexpr (kInterleaved) {
+        Vec<T, 2 * V> p = load_vec<T, 2 * V>(x + u0);
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float u = to_f32(p.v[2 * e]), v = to_f32(p.v[2 * e + 1]);
+            p.v[2 * e] = from_f32<T>(u * c[e] - v * s[e]);
+            p.v[2 * e + 1] = from_f32<T>(u * s[e] + v * c[e]);
+          }
+        }
+        store_vec<T, 2 * V>(y + u0, p);
+      } else {
+        Vec<T, V> p = load_vec<T, V>(x + u0), q = load_vec<T, V>(x + v0);
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float u = to_f32(p.v[e]), v = to_f32(q.v[e]);
+            p.v[e] = from_f32<T>(u * c[e] - v * s[e]);
+            q.v[e] = from_f32<T>(u * s[e] + v * c[e]);
+          }
+        }
+        store_vec<T, V>(y + u0, p);
+        store_vec<T, V>(y + v0, q);
+      }
+    }
+  }
+}
+
+template <typename T, int V, bool kInterleaved>
+int launch(const RotaryArgs& a, cudaStream_t st) {
+  int sms = 0;
+  if (const int rc = device_sm_count(&sms)) return rc;
+  const int px = a.dim / 2 / V, py = std::max(1, 256 / px);
+  const long long blocks = std::min<long long>((a.tokens + py - 1) / py, (long long)sms * 16);
+  rotary_kernel<T, V, kInterleaved><<<(unsigned)blocks, dim3(px, py), 0, st>>>(a);
+  D2C_LAUNCH_CHECK();
+  return D2C_OK;
+}
+
+template <typename T>
+int run(const d2c_rotary_desc& d, const RotaryArgs& a, cudaStream_t st) {
+  // pairs a thread: as many as every section, the strides and the pointers allow, 16 bytes an access at most
+  auto fits = [&](int v) {
+    const int run = d.interleaved ? 2 * v : v;                   // contiguous channels of one access
+    for (int k = 0; k < 3; ++k)
+      if ((a.n[k] / 2) % v) return false;
+    return (a.dim / 2) % v == 0 && a.sb % run == 0 && a.sl % run == 0 && a.sh % run == 0 &&
+           run * (int)sizeof(T) <= 16 && aligned_to(a.x, run * sizeof(T)) && aligned_to(a.y, run * sizeof(T));
+  };
+  if (d.interleaved) {
+    if (fits(4)) return launch<T, 4, true>(a, st);
+    if (fits(2)) return launch<T, 2, true>(a, st);
+    if (fits(1)) return launch<T, 1, true>(a, st);
+    return D2C_ERR_ALIGN;
+  }
+  if (fits(4)) return launch<T, 4, false>(a, st);
+  if (fits(2)) return launch<T, 2, false>(a, st);
+  return launch<T, 1, false>(a, st);
+}
+
+int checked(const d2c_rotary_desc* d) {
+  if (!d) return D2C_ERR_NULL;
+  if (!token_dtype_ok(d->dtype)) return D2C_ERR_DTYPE;
+  if (d->batch < 1 || d->length < 1 || d->heads < 1 || d->dim < 2 || d->dim % 2 || d->dim > 512) return D2C_ERR_SHAPE;
+  int sum = 0;
+  for (int k = 0; k < 3; ++k) {
+    if (d->axis_dims[k] < 0 || d->axis_dims[k] % 2 || d->axis_dims[k] > d->dim) return D2C_ERR_SHAPE;
+    sum += d->axis_dims[k];
+  }
+  if (sum > d->dim || !(d->base > 0)) return D2C_ERR_SHAPE;
+  if (d->pos_kind < D2C_POS_GRID || d->pos_kind > D2C_POS_F32) return D2C_ERR_MODE;
+  if (d->pos_kind == D2C_POS_GRID) {
+    long long n = 1;
+    for (int k = 0; k < 3; ++k) {
+      if (d->grid[k] < 1) return D2C_ERR_SHAPE;
+      n *= d->grid[k];
+      if (n > d->length) return D2C_ERR_SHAPE;
+    }
+    if (n != d->length) return D2C_ERR_SHAPE;
+  }
+  return D2C_OK;
+}
+
+}  // namespace
+}  // namespace d2c
+
+extern "C" int d2c_rotary_check(const d2c_rotary_desc* desc) { return d2c::checked(desc); }
+
+extern "C" int d2c_rotary(const d2c_rotary_desc* desc, const void* x, const void* positions, void* y, d2c_stream_t stream) {
+  using namespace d2c;
+  if (const int rc = take_device_status()) return rc;
+  if (const int rc = checked(desc)) return rc;
+  if (!x || !y || (desc->pos_kind != D2C_POS_GRID && !positions)) return D2C_ERR_NULL;
+  RotaryArgs a{};
+  a.x = x; a.positions = positions; a.y = y;
+  a.tokens = (long long)desc->batch * desc->length;
+  a.sb = desc->stride_batch; a.sl = desc->stride_token; a.sh = desc->stride_head;
+  a.pos_batch = desc->pos_batch_stride;
+  a.length = desc->length; a.heads = desc->heads; a.dim = desc->dim;
+  a.pos_kind = desc->pos_kind;
+  a.grid_h = desc->grid[1]; a.grid_w = desc->grid[2];
+  for (int k = 0; k < 3; ++k) {
+    a.n[k] = desc->axis_dims[k];
+    // centres of cells: (index + 1/2) * step - 1/2
+    a.step[k] = desc->grid_step[k];
+    a.first[k] = 0.5 * desc->grid_step[k] - 0.5;
+  }
+  a.log2_base = log2(desc->base);
+  a.sign = desc->inverse ? -1.f : 1.f;
+  cudaStream_t st = (cudaStream_t)stream;
+  prof_mark(st, "rotary");
+  int rc;
+  switch (desc->dtype) {
+    case D2C_F32: rc = run<float>(*desc, a, st); break;
+    case D2C_F16: rc = run<__half>(*desc, a, st); break;
+    default: rc = run<__nv_bfloat16>(*desc, a, st); break;
+  }
+  prof_mark(st, nullptr);
+  return rc;
+}

@@ -8,50 +8,23 @@
 //
 // Interfaces it stands in for: csrc/ops/dconv3d.h:70-226 (DeformConv3dFunction, deform_conv3d), csrc/ops/dconv1d.h:69-186,
 // fast-depthwise-conv3d/csrc/grouped_conv3d.h:29-106, and the half-precision up-cast of deform_conv.py:54-59.
-#include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/cuda/Event.h>
-#include <torch/extension.h>
 
 #include <array>
 #include <atomic>
 #include <mutex>
-#include <optional>
 #include <vector>
 
-#include "d2conv3d.h"
+#include "torch_common.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
+using namespace d2c_torch;
 using Triple = std::array<int64_t, 3>;
-using OptTensor = std::optional<Tensor>;
 
 // ---- helpers --------------------------------------------------------------------------------------------
-
-// TORCH_CHECK(expr) of the reference reads "Expected <expr> to be true ..."
-#define D2C_REQUIRE(cond, text) TORCH_CHECK(cond, "Expected " text " to be true, but got false.")
-
-void check(int status, const char* what) {
-  TORCH_CHECK(status == 0, what, ": ", d2c_status_string(status), status > 0 ? ": " : "",
-              status > 0 ? d2c_last_cuda_error() : "", " (status ", status, ")");
-}
-
-Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-Tensor like(const Tensor& t) { return t.defined() ? at::empty_like(t, at::MemoryFormat::Contiguous) : t; }
-Tensor bytes_on(size_t n, const Tensor& t) {
-  return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)) : Tensor();
-}
-void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // deform_conv.py:15-16,54-59: if any tensor is fp16, every tensor is converted to fp32 and the result stays fp32
 void upcast_if_any_half(std::initializer_list<Tensor*> tensors) {
@@ -121,17 +94,6 @@ struct ReadyEvents {
 ReadyEvents& ready_events() {
   static auto* const events = new ReadyEvents();     // outlives the CUDA context
   return *events;
-}
-
-// Results of a backward node: gradients are computed outside the graph, so a second derivative has to fail loudly.
-variable_list once_differentiable(variable_list&& grads) {
-  if (!at::GradMode::is_enabled()) return std::move(grads);
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)grads.size());
-  error->set_next_edges(torch::autograd::edge_list(1));
-  for (Tensor& t : grads)
-    if (t.defined()) t.set_requires_grad(true);
-  return (*error)(std::move(grads));
 }
 
 // ---- deformable / dynamic-dilated / fused-head / 1-D op ---------------------------------------------------
@@ -549,4 +511,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_keep_samples", set_keep_samples);
   m.def("get_keep_samples", get_keep_samples);
   m.def("take_params_ready_event", take_params_ready_event);
+  d2c_torch::bind_token_ops(m);
 }

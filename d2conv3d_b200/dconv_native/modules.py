@@ -25,6 +25,7 @@ from torch.nn.modules.utils import _triple
 from torch.utils.checkpoint import checkpoint
 
 from . import _ops
+from ..tokens import LayerNorm3d
 from .deform_conv import DeformConv3d
 from .grid import offsets_from_size_map
 
@@ -61,7 +62,8 @@ class _DConvBase(nn.Module):
     `deform_param_op`), all of them also accepted as keywords:
 
       init             "zero" (default) | "random" (modulated layers only: network/layers.py:122-132)
-      norm_type        "none" | "GroupNorm" | "BatchNorm": a norm on the predictor's input (layers.py:37-44)
+      norm_type        "none" | "GroupNorm" | "BatchNorm": a norm on the predictor's input (layers.py:37-44), or "LayerNorm3d",
+                       which the reference does not have: over the channels of every voxel (tokens.py)
       norm_groups      groups of that GroupNorm
       size_activation  "elu" | "relu" | "relu_plus_one" | "linear" (layers.py:171-181)
       deform_param_op  class of the predictor, or a ready nn.Module instance (then used as is, not initialised)
@@ -109,12 +111,14 @@ class _DConvBase(nn.Module):
         self.fused_field = fused_field
         self.fused_head = fused_head
         self._mask_act_name = activation if isinstance(activation, str) else None
-        if norm_type not in ("BatchNorm", "GroupNorm", "none"):
+        if norm_type not in ("BatchNorm", "GroupNorm", "LayerNorm3d", "none"):
             raise ValueError(f"Unexpected norm_type: '{norm_type}'")
         if norm is None and norm_type == "GroupNorm":
             norm = nn.GroupNorm(norm_groups, in_channels)
         elif norm is None and norm_type == "BatchNorm":
             norm = nn.BatchNorm3d(in_channels)
+        elif norm is None and norm_type == "LayerNorm3d":
+            norm = LayerNorm3d(in_channels)
         self.norm = norm
         self.alpha_channels = offset_groups * self.num_kernel_points if self.modulated else 0
         if self.field_mode is None:

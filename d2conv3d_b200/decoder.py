@@ -22,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .dconv_native.util import add_deformable_conv
+from .tokens import CrossAttention3d
 
 
 class GlobalConv3d(nn.Module):
@@ -37,6 +38,19 @@ class GlobalConv3d(nn.Module):
 
     def forward(self, x):
         return self.conv_l2(self.conv_l1(x)) + self.conv_r2(self.conv_r1(x))
+
+
+class CrossAttentionBridge3d(nn.Module):
+    """Bridge without a counterpart in the reference: the coarsest level, projected to the decoder's channels, looks at every
+    voxel of the level above it (layer norm, rotary positions in time, height and width, cross attention: tokens.py)."""
+
+    def __init__(self, in_channels, context_channels, out_channels, heads=4):
+        super().__init__()
+        self.proj = nn.Conv3d(in_channels, out_channels, 1)
+        self.attention = CrossAttention3d(out_channels, context_channels, heads=heads, head_dim=out_channels // heads)
+
+    def forward(self, x, context):
+        return self.attention(self.proj(x), context)
 
 
 class ConvActNorm(nn.Sequential):
@@ -79,12 +93,19 @@ class Refine3d(nn.Module):
 
 class Decoder(nn.Module):
     """widths: channels of the four pyramid levels, fine to coarse.  conv: None for plain convolutions, or a
-    version name understood by add_deformable_conv for the refine blocks' 3x3x3 convolutions."""
+    version name understood by add_deformable_conv for the refine blocks' 3x3x3 convolutions.  bridge: "global_conv" (the
+    reference's) or "cross_attention" (the coarsest level looks at all of the one above it)."""
 
     def __init__(self, widths=(256, 512, 1024, 2048), channels=256, num_classes=2,
-                 conv="XYZSizeConditionedDCNv2", offset_groups=8):
+                 conv="XYZSizeConditionedDCNv2", offset_groups=8, bridge="global_conv"):
         super().__init__()
-        self.gc = GlobalConv3d(widths[3], channels, mid_channels=channels)
+        if bridge == "global_conv":
+            self.gc = GlobalConv3d(widths[3], channels, mid_channels=channels)
+        elif bridge == "cross_attention":
+            self.gc = CrossAttentionBridge3d(widths[3], widths[2], channels)
+        else:
+            raise ValueError(f"Unexpected bridge: '{bridge}'")
+        self.bridge = bridge
         self.convG1 = nn.Conv3d(channels, channels, 3, padding=1)
         self.convG2 = nn.Conv3d(channels, channels, 3, padding=1)
         self.rf3 = Refine3d(widths[2], channels)
@@ -99,7 +120,7 @@ class Decoder(nn.Module):
                 self.converted += n
 
     def forward(self, e1, e2, e3, e4):
-        x = self.gc(e4)
+        x = self.gc(e4) if self.bridge == "global_conv" else self.gc(e4, e3)
         m4 = x + self.convG2(F.relu(self.convG1(F.relu(x))))
         m3 = self.rf3(e3, m4)
         m2 = self.rf2(e2, m3)

@@ -32,7 +32,7 @@ extern "C" {
 typedef void* d2c_stream_t; /* a cudaStream_t */
 typedef void* d2c_event_t;  /* a cudaEvent_t */
 
-enum d2c_dtype { D2C_F32 = 0, D2C_F64 = 1, D2C_F16 = 2 /* depthwise only */ };
+enum d2c_dtype { D2C_F32 = 0, D2C_F64 = 1, D2C_F16 = 2 /* depthwise and token operators */, D2C_BF16 = 3 /* token operators */ };
 
 /* How the Cin*K x Cout contraction of the deformable ops is evaluated.
  *   D2C_MATH_FP32   fp32 (or fp64) FMA pipeline; matches a cuBLAS S/Dgemm up to
@@ -76,6 +76,7 @@ enum d2c_status {
   D2C_ERR_MODE = -10,         /* unknown math / field mode */
   D2C_ERR_WEIGHT_SHAPE = -11, /* weight.size(1)*groups != Cin, or depthwise weight rule */
   D2C_ERR_SCRATCH_LIMIT = -12,/* problem needs more scratch than the library's built-in buffer holds */
+  D2C_ERR_ALIGN = -13,        /* a pointer or stride is not aligned as the op asks */
   D2C_ERR_CUDA = 1,           /* a CUDA runtime call failed (see d2c_last_cuda_error) */
   D2C_ERR_DEVICE_TIMEOUT = 2  /* a bounded device-side wait gave up */
 };
@@ -385,6 +386,77 @@ int d2c_act_group_norm_fwd(const float* x, const float* gamma, const float* beta
 int d2c_depthwise_conv3d_bwd_noalloc(const d2c_conv_desc* desc, const void* grad_y, const void* x,
                                      const void* w, void* grad_x, void* grad_w, void* grad_bias,
                                      d2c_stream_t stream);
+
+/* ---- token operators --------------------------------------------------------
+ * What one level of a feature pyramid needs to look at all of another: layer norm over the channels of a position, rotary
+ * positions on the (time, height, width) grid, and cross attention.  No counterpart in the reference.  dtype: F32, F16 or
+ * BF16; arithmetic, statistics and sums are fp32.  Results are the same bits in every call (no atomics). */
+
+enum d2c_norm_layout {
+  D2C_NORM_ROWS = 0,           /* x, y [batch, positions, channels] */
+  D2C_NORM_VOLUME = 1,         /* x, y [batch, channels, positions] */
+  D2C_NORM_VOLUME_TO_ROWS = 2  /* x [batch, channels, positions], y [batch, positions, channels] */
+};
+typedef struct d2c_layer_norm_desc {
+  int32_t dtype;
+  int32_t param_dtype;         /* of w, b and their gradients: dtype or D2C_F32 */
+  int32_t layout;              /* d2c_norm_layout */
+  int32_t batch, channels;
+  int64_t positions;
+  float eps;
+} d2c_layer_norm_desc;
+
+int d2c_layer_norm_check(const d2c_layer_norm_desc* desc);
+/* y = (x - mean) / sqrt(var + eps) * w + b over the channels of every position; w, b [channels] may be NULL (1 / 0).
+ * stats: NULL, or batch * positions pairs of floats that the backward reads.  x, y contiguous, not overlapping. */
+int d2c_layer_norm_fwd(const d2c_layer_norm_desc* desc, const void* x, const void* w, const void* b, void* y, void* stats,
+                       d2c_stream_t stream);
+/* Any of grad_x, grad_w, grad_b may be NULL.  grad_y is laid out like y.  The workspace is for grad_w / grad_b. */
+size_t d2c_layer_norm_bwd_workspace_bytes(const d2c_layer_norm_desc* desc);
+int d2c_layer_norm_bwd(const d2c_layer_norm_desc* desc, const void* grad_y, const void* x, const void* w, const void* stats,
+                       void* grad_x, void* grad_w, void* grad_b, void* workspace, size_t workspace_bytes, d2c_stream_t stream);
+
+enum d2c_position_kind { D2C_POS_GRID = 0, D2C_POS_I32 = 1, D2C_POS_I64 = 2, D2C_POS_F32 = 3 };
+typedef struct d2c_rotary_desc {
+  int32_t dtype;
+  int32_t batch, length, heads, dim;                 /* x [batch, length, heads, dim]; dim even, <= 512 */
+  int64_t stride_batch, stride_token, stride_head;   /* of x, in elements; its last dimension and y are contiguous */
+  int32_t axis_dims[3];                              /* channels that time, height, width turn; even, sum <= dim */
+  int32_t interleaved;                               /* pairs are neighbours (2i, 2i+1); else (i, i + n/2) of a section */
+  int32_t inverse;                                   /* turn back: the gradient */
+  int32_t pos_kind;
+  int32_t grid[3];                                   /* D2C_POS_GRID: tokens are this volume's voxels, row-major */
+  double grid_step[3];                               /* position = (index + 1/2) * step - 1/2 */
+  int64_t pos_batch_stride;                          /* elements between two clips' positions [length, 3]; 0: shared */
+  double base;
+} d2c_rotary_desc;
+
+int d2c_rotary_check(const d2c_rotary_desc* desc);
+/* Interleaved pairs ask for x and y aligned to a pair and even strides (D2C_ERR_ALIGN). */
+int d2c_rotary(const d2c_rotary_desc* desc, const void* x, const void* positions, void* y, d2c_stream_t stream);
+
+typedef struct d2c_attention_desc {
+  int32_t dtype;
+  int32_t batch, queries, keys;
+  int32_t q_heads, kv_heads, dim;                    /* q_heads a multiple of kv_heads; head h reads h / (q_heads / kv_heads) */
+  int32_t lengths_i64;                               /* key_lengths are int64 (else int32) */
+  float scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3];     /* batch, token, head, in elements; the last dimension is contiguous */
+  int64_t g_stride[3];                               /* of grad_o */
+} d2c_attention_desc;
+
+int d2c_attention_check(const d2c_attention_desc* desc);
+/* o [batch, queries, q_heads, dim] = softmax(scale q k^T) v over the first key_lengths[b] keys of clip b (NULL: all; values
+ * outside 0 .. keys are taken as the nearer of the two).  No keys: o = 0.  lse: NULL, or [batch, q_heads, queries] floats for
+ * the backward.  Keys and values behind a clip's length are not used, whatever they hold.  dim <= 128. */
+size_t d2c_attention_fwd_workspace_bytes(const d2c_attention_desc* desc);
+int d2c_attention_fwd(const d2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* key_lengths,
+                      void* o, void* lse, void* workspace, size_t workspace_bytes, d2c_stream_t stream);
+/* grad_q, grad_k, grad_v contiguous [batch, tokens, heads, dim], written whole (zero behind a clip's length). */
+size_t d2c_attention_bwd_workspace_bytes(const d2c_attention_desc* desc);
+int d2c_attention_bwd(const d2c_attention_desc* desc, const void* grad_o, const void* q, const void* k, const void* v,
+                      const void* key_lengths, const void* o, const void* lse, void* grad_q, void* grad_k, void* grad_v,
+                      void* workspace, size_t workspace_bytes, d2c_stream_t stream);
 
 #ifdef __cplusplus
 }
