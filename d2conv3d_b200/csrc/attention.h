@@ -48,5 +48,8 @@ int combine(int dtype, const Args& a, cudaStream_t st);          // partial outp
 int delta_rows(int dtype, const Args& a, cudaStream_t st);
 int sum_parts(int dtype, const float* part, int splits, long long n, void* out, cudaStream_t st);
 
+// ---- attention_sm100.cu: 16-bit types, 16-byte rows, positive strides, scale >= 0
+int tc_fwd(int dtype, const Args& a, cudaStream_t st);
+
 }  // namespace attn
 }  // namespace d2c

@@ -7,7 +7,7 @@ namespace d2c {
 namespace attn {
 namespace {
 
-enum class Path { few, exact };
+enum class Path { few, exact, tensor };
 struct Plan {
   Path path;
   int splits;
@@ -31,6 +31,19 @@ bool few_fits(const d2c_attention_desc& d) {
   return d.dim % v == 0 && rows_fit(d, d.q_stride) && rows_fit(d, d.k_stride) && rows_fit(d, d.v_stride);
 }
 
+// What the tensor-core kernels' tensor maps take: 16-bit types, 16-byte rows, no dimension that repeats its elements, strides under
+// 2^40 bytes; and, for the running maximum to be that of the raw scores, a scale above zero.
+bool tensor_fits(const d2c_attention_desc& d) {
+  if (d.dtype == D2C_F32 || d.dim % 8 || !(d.scale > 1e-30f)) return false;
+  auto fits = [&](const int64_t (&s)[3], int tokens, int heads) {
+    const int n[3] = {d.batch, tokens, heads};
+    for (int i = 0; i < 3; ++i)
+      if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= 1LL << 39)) return false;
+    return true;
+  };
+  return fits(d.q_stride, d.queries, d.q_heads) && fits(d.k_stride, d.keys, d.kv_heads) && fits(d.v_stride, d.keys, d.kv_heads);
+}
+
 // few: up to 16 query rows on a head's keys; every four rows read the keys once, from L2 after the first.
 Plan plan_fwd(const d2c_attention_desc& d, bool aligned, int sms) {
   Plan p{Path::exact, 1};
@@ -39,6 +52,9 @@ Plan plan_fwd(const d2c_attention_desc& d, bool aligned, int sms) {
     p.path = Path::few;
     const long long blocks = (long long)ceil_div(rows, kFewRows) * d.kv_heads * d.batch;
     p.splits = std::max(1, std::min({ceil_div(4LL * sms, blocks), ceil_div(d.keys, 128), 128}));
+  } else if (aligned && tensor_fits(d)) {
+    p.path = Path::tensor;
+    p.splits = shares((long long)ceil_div(d.queries, 256) * d.q_heads * d.batch, ceil_div(d.keys, 128), 2, sms);
   } else {
     p.splits = shares((long long)ceil_div(d.queries, kTile) * d.q_heads * d.batch, ceil_div(d.keys, kTile), 2, sms);
   }
@@ -100,7 +116,9 @@ int run_fwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaS
     a.part_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) +
                                           align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256));
   }
-  const int rc = p.path == Path::few ? few_fwd(d.dtype, a, st) : exact_fwd(d.dtype, a, st);
+  const int rc = p.path == Path::few      ? few_fwd(d.dtype, a, st)
+                 : p.path == Path::tensor ? tc_fwd(d.dtype, a, st)
+                                          : exact_fwd(d.dtype, a, st);
   if (rc || p.splits == 1) return rc;
   return combine(d.dtype, a, st);
 }

@@ -1,0 +1,136 @@
+// Pieces that the tensor-core attention kernels share: TMA tile loads, tensor-memory stores, MMAs whose A operand lies in tensor
+// memory, and the shared-memory operand tile.
+//
+// Operand tile: 128 rows (queries or keys) of one head, as 64-channel halves of [128][128 bytes] with the 128-byte swizzle: what one
+// tensor-map box delivers.  Read with the channels as the reduction (K-major) it is an operand of q k^T; read with the rows as the
+// reduction (MN-major) the same bytes are the B operand of p v.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "attention.h"
+#include "sm100_ptx.cuh"
+
+namespace d2c {
+namespace attn {
+
+constexpr int kRows = 128;                       // rows of a tile
+constexpr int kHalfBytes = kRows * 128;          // 64 channels of it
+template <int DP>
+constexpr int kTileBytes = kHalfBytes * (DP / 64);
+
+// One box of 64 channels x 1 head x 128 tokens x 1 clip; what lies outside the tensor arrives as zeros.  x is 0 or 64.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, int clip, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(token), "r"(clip), "r"(bar)
+               : "memory");
+}
+template <int DP>
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int head, int token, int clip, uint32_t bar) {
+#pragma unroll
+  for (int h = 0; h < DP / 64; ++h) tma_box(dst + h * kHalfBytes, map, h * 64, head, token, clip, bar);
+}
+
+// Zeroes rows [from, 128) of a tile (one warp).
+template <int DP>
+__device__ __forceinline__ void clear_rows(uint32_t tile, int from) {
+  const int lane = threadIdx.x & 31;
+  for (int i = from * 8 + lane; i < kRows * 8; i += 32) {        // 16-byte pieces: the swizzle stays inside a row
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h) ptx::sts_v4(tile + h * kHalfBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
+  }
+}
+
+// 32 lanes x 32 consecutive 32-bit columns of tensor memory.
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem], A 128 rows (lanes) x 16 of the reduction (8 columns of pairs).  Issued by one thread.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: A and B fp16 or bf16 alike, fp32 accumulator, 128 x N.  b_mn: B's rows are the reduction (MN-major).
+template <typename T>
+__device__ __forceinline__ uint32_t idesc_of(int N, bool b_mn) {
+  const uint32_t fmt = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// D (128 x 128) = X Y^T over the channels, both K-major; ksteps = channels / 16 rounded up (zero-filled above D).
+__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ksteps) {
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t at = (uint32_t)((k >> 2) * kHalfBytes + (k & 3) * 32);
+    ptx::umma_bf16(d_tmem, ptx::umma_desc_kmajor_sw128(x + at), ptx::umma_desc_kmajor_sw128(y + at), idesc, k > 0);
+  }
+}
+// D (128 x N) (+)= A Y, A 128 x 128 in tensor memory, Y's 128 rows the reduction.
+__device__ __forceinline__ void mma_weigh(uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int k = 0; k < kRows / 16; ++k)
+    umma_ts(d_tmem, a_tmem + 8 * k, ptx::umma_desc_mnmajor_sw128(y + 2048 * k, kHalfBytes, 1024), idesc, accumulate | (k > 0));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    return ptx::pack_bf16x2(lo, hi);
+  } else {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Register split of a block of 12 warps launched with 168 registers a thread: 8 working warps take 208, the 4 others keep 80
+// (8 * 208 + 4 * 80 <= 12 * 168).  Executed by every warp of a group of four.
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+
+// Called by all threads at a kernel's end: reports a wait that gave up to the host.
+__device__ __forceinline__ void report(int* status, volatile int* abort_flag) {
+  if (threadIdx.x == 0 && *abort_flag && status) {
+    *reinterpret_cast<volatile int*>(status) = 1;
+    __threadfence_system();
+  }
+}
+
+// A wait of a whole warp: all lanes go on, or none (the warp's next step needs them all).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag));
+}
+
+// Bounded wait of a thread that may not leave with copies or MMAs in flight, whatever else happened.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (clock64() - t0 > ptx::kWaitBudgetCycles) break;
+}
+
+// attention_sm100.cu: host helpers
+int status_pointer(int** out);
+
+}  // namespace attn
+}  // namespace d2c
