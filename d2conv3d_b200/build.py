@@ -24,7 +24,7 @@ TORCH_STAMP = os.path.join(OBJ_DIR, "torch_ops.stamp")
 
 SOURCES = ["d2c_api.cu", "depthwise.cu", "deform_sm100_fwd.cu", "deform_sm100_bwd.cu", "deform_sm100_dw.cu",
            "deform_exact_f32.cu", "deform_exact_f64.cu", "act_norm.cu", "layer_norm.cu", "rotary.cu", "attention_exact.cu",
-           "attention_sm100.cu", "attention_api.cu"]
+           "attention_sm100.cu", "attention_sm100_bwd.cu", "attention_api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE,

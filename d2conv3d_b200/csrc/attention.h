@@ -50,6 +50,9 @@ int sum_parts(int dtype, const float* part, int splits, long long n, void* out, 
 
 // ---- attention_sm100.cu: 16-bit types, 16-byte rows, positive strides, scale >= 0
 int tc_fwd(int dtype, const Args& a, cudaStream_t st);
+// ---- attention_sm100_bwd.cu: the same, and grad_o's rows
+int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st);              // fp16: [B, Hkv][2], for tc_bwd
+int tc_bwd(int dtype, const Args& a, bool keys, const uint32_t* bounds, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace d2c

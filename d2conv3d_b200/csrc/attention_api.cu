@@ -33,15 +33,16 @@ bool few_fits(const d2c_attention_desc& d) {
 
 // What the tensor-core kernels' tensor maps take: 16-bit types, 16-byte rows, no dimension that repeats its elements, strides under
 // 2^40 bytes; and, for the running maximum to be that of the raw scores, a scale above zero.
+bool tensor_rows(const d2c_attention_desc& d, const int64_t (&s)[3], int tokens, int heads) {
+  const int n[3] = {d.batch, tokens, heads};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= 1LL << 39)) return false;
+  return true;
+}
 bool tensor_fits(const d2c_attention_desc& d) {
   if (d.dtype == D2C_F32 || d.dim % 8 || !(d.scale > 1e-30f)) return false;
-  auto fits = [&](const int64_t (&s)[3], int tokens, int heads) {
-    const int n[3] = {d.batch, tokens, heads};
-    for (int i = 0; i < 3; ++i)
-      if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= 1LL << 39)) return false;
-    return true;
-  };
-  return fits(d.q_stride, d.queries, d.q_heads) && fits(d.k_stride, d.keys, d.kv_heads) && fits(d.v_stride, d.keys, d.kv_heads);
+  return tensor_rows(d, d.q_stride, d.queries, d.q_heads) && tensor_rows(d, d.k_stride, d.keys, d.kv_heads) &&
+         tensor_rows(d, d.v_stride, d.keys, d.kv_heads);
 }
 
 // few: up to 16 query rows on a head's keys; every four rows read the keys once, from L2 after the first.
@@ -60,12 +61,18 @@ Plan plan_fwd(const d2c_attention_desc& d, bool aligned, int sms) {
   }
   return p;
 }
-Plan plan_bwd_q(const d2c_attention_desc& d, int sms) {
-  return {Path::exact, shares((long long)ceil_div(d.queries, kTile) * d.q_heads * d.batch, ceil_div(d.keys, kTile), 2, sms)};
-}
-Plan plan_bwd_kv(const d2c_attention_desc& d, int sms) {
-  return {Path::exact, shares((long long)ceil_div(d.keys, kTile) * d.kv_heads * d.batch,
-                              ceil_div(d.queries, kTile) * (d.q_heads / d.kv_heads), 2, sms)};
+// A gradient kernel's block has a tile of one side and runs over the other.
+Plan plan_bwd(const d2c_attention_desc& d, bool keys, bool aligned, int sms) {
+  Plan p{Path::exact, 1};
+  int tile = kTile;
+  if (aligned && tensor_fits(d) && tensor_rows(d, d.g_stride, d.queries, d.q_heads)) {
+    p.path = Path::tensor;
+    tile = 128;
+  }
+  const int q = ceil_div(d.queries, tile), k = ceil_div(d.keys, tile);
+  p.splits = keys ? shares((long long)k * d.kv_heads * d.batch, q * (d.q_heads / d.kv_heads), 2, sms)
+                  : shares((long long)q * d.q_heads * d.batch, k, 2, sms);
+  return p;
 }
 
 long long q_rows(const d2c_attention_desc& d) { return (long long)d.batch * d.queries * d.q_heads; }
@@ -76,11 +83,16 @@ size_t fwd_bytes(const d2c_attention_desc& d, const Plan& p) {
   return align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256) + align_up(sizeof(float) * p.splits * q_rows(d), 256);
 }
 size_t bwd_part_bytes(const d2c_attention_desc& d, int sms) {
-  const int sq = plan_bwd_q(d, sms).splits, skv = plan_bwd_kv(d, sms).splits;
-  const size_t q = sq > 1 ? sizeof(float) * sq * q_rows(d) * d.dim : 0;
-  const size_t kv = skv > 1 ? sizeof(float) * 2 * skv * kv_rows(d) * d.dim : 0;
-  return align_up(std::max(q, kv), 256);
+  size_t most = 0;                    // whatever the pointers' alignment, and so the plan, turns out to be
+  for (int al = 0; al < 2; ++al) {
+    const int sq = plan_bwd(d, false, al, sms).splits, skv = plan_bwd(d, true, al, sms).splits;
+    if (sq > 1) most = std::max<size_t>(most, sizeof(float) * sq * q_rows(d) * d.dim);
+    if (skv > 1) most = std::max<size_t>(most, sizeof(float) * 2 * skv * kv_rows(d) * d.dim);
+  }
+  return align_up(most, 256);
 }
+size_t delta_bytes(const d2c_attention_desc& d) { return align_up(sizeof(float) * q_rows(d), 256); }
+size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 2 * d.batch * d.kv_heads, 256); }
 
 int checked(const d2c_attention_desc* d) {
   if (!d) return D2C_ERR_NULL;
@@ -89,7 +101,7 @@ int checked(const d2c_attention_desc* d) {
     return D2C_ERR_SHAPE;
   if (d->q_heads % d->kv_heads) return D2C_ERR_GROUPS;
   // grids and row indexes of the kernels
-  if (q_rows(*d) > 0x7fffffffLL || kv_rows(*d) > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
+  if (q_rows(*d) > 0x7fffffffLL || kv_rows(*d) > 0x7fffffffLL || (long long)d->batch * d->q_heads > 65535) return D2C_ERR_TOO_LARGE;
   return D2C_OK;
 }
 
@@ -109,7 +121,7 @@ Args make_args(const d2c_attention_desc& d, const void* q, const void* k, const 
 bool ws_ok(const void* ws, size_t have, size_t need) { return need == 0 || (ws && aligned_to(ws, 256) && have >= need); }
 
 int run_fwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaStream_t st) {
-  const Plan p = plan_fwd(d, aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16), sms);
+  const Plan p = plan_fwd(d, aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.o, 16), sms);
   a.splits = p.splits;
   if (p.splits > 1) {
     a.part = reinterpret_cast<float*>(workspace);
@@ -124,19 +136,26 @@ int run_fwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaS
 }
 
 int run_bwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaStream_t st) {
-  a.part = reinterpret_cast<float*>(workspace);
-  a.delta = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + bwd_part_bytes(d, sms));
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.delta = reinterpret_cast<float*>(ws);
+  uint32_t* bounds = reinterpret_cast<uint32_t*>(ws + delta_bytes(d));
+  a.part = reinterpret_cast<float*>(ws + delta_bytes(d) + bound_bytes(d));
+  const bool aligned = aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.g, 16) &&
+                       aligned_to(a.gq, 16) && aligned_to(a.gk, 16) && aligned_to(a.gv, 16);
   int rc = delta_rows(d.dtype, a, st);
   if (rc) return rc;
-  a.splits = plan_bwd_kv(d, sms).splits;
-  if ((rc = exact_bwd_kv(d.dtype, a, st))) return rc;
+  const Plan pk = plan_bwd(d, true, aligned, sms), pq = plan_bwd(d, false, aligned, sms);
+  const bool tensor = pk.path == Path::tensor;
+  if (tensor && d.dtype == D2C_F16 && (rc = tc_bounds(a, bounds, st))) return rc;
+  a.splits = pk.splits;
+  if ((rc = tensor ? tc_bwd(d.dtype, a, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
   if (a.splits > 1) {
     const long long n = kv_rows(d) * d.dim;
     if ((rc = sum_parts(d.dtype, a.part, a.splits, n, a.gk, st))) return rc;
     if ((rc = sum_parts(d.dtype, a.part + a.splits * n, a.splits, n, a.gv, st))) return rc;
   }
-  a.splits = plan_bwd_q(d, sms).splits;
-  if ((rc = exact_bwd_q(d.dtype, a, st))) return rc;
+  a.splits = pq.splits;
+  if ((rc = tensor ? tc_bwd(d.dtype, a, false, bounds, st) : exact_bwd_q(d.dtype, a, st))) return rc;
   if (a.splits > 1) return sum_parts(d.dtype, a.part, a.splits, q_rows(d) * d.dim, a.gq, st);
   return D2C_OK;
 }
@@ -179,7 +198,7 @@ size_t d2c_attention_bwd_workspace_bytes(const d2c_attention_desc* desc) {
   using namespace d2c;
   int sms = 0;
   if (attn::checked(desc) || device_sm_count(&sms)) return 0;
-  return attn::bwd_part_bytes(*desc, sms) + align_up(sizeof(float) * attn::q_rows(*desc), 256);
+  return attn::delta_bytes(*desc) + attn::bound_bytes(*desc) + attn::bwd_part_bytes(*desc, sms);
 }
 
 int d2c_attention_bwd(const d2c_attention_desc* desc, const void* grad_o, const void* q, const void* k, const void* v,

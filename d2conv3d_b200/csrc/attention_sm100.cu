@@ -288,20 +288,6 @@ int encoder(EncodeTiled* out) {
   return D2C_OK;
 }
 
-// [clips, tokens, heads, D] with element strides s (clip, token, head); a dimension of one element has no stride.
-int tile_map(CUtensorMap* map, int dtype, const void* p, int D, int heads, int tokens, int clips, const long long (&s)[3]) {
-  EncodeTiled f;
-  if (const int rc = encoder(&f)) return rc;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)clips};
-  auto bytes = [&](long long st, int n) { return (cuuint64_t)(n == 1 ? 256 : 2 * st); };
-  const cuuint64_t strides[3] = {bytes(s[2], heads), bytes(s[1], tokens), bytes(s[0], clips)};
-  const cuuint32_t box[4] = {64, 1, kRows, 1}, ones[4] = {1, 1, 1, 1};
-  const CUresult rc = f(map, dtype == D2C_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                        const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return rc == CUDA_SUCCESS ? D2C_OK : check_cuda(cudaErrorInvalidValue);
-}
-
 template <typename T, int DP>
 int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, unsigned grid, cudaStream_t st) {
   if (const int rc = allow_dynamic_smem<fwd_tc_kernel<T, DP>>(kFwdSmem<DP>)) return rc;
@@ -319,6 +305,20 @@ int status_pointer(int** out) {
   const int rc = status_word_device_ptr(out);
   const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
   return rc ? rc : check_cuda(back);
+}
+
+// [clips, tokens, heads, D] with element strides s (clip, token, head); a dimension of one element has no stride.
+int tile_map(CUtensorMap* map, int dtype, const void* p, int D, int heads, int tokens, int clips, const long long (&s)[3]) {
+  EncodeTiled f;
+  if (const int rc = encoder(&f)) return rc;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)clips};
+  auto bytes = [&](long long st, int n) { return (cuuint64_t)(n == 1 ? 256 : 2 * st); };
+  const cuuint64_t strides[3] = {bytes(s[2], heads), bytes(s[1], tokens), bytes(s[0], clips)};
+  const cuuint32_t box[4] = {64, 1, kRows, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult rc = f(map, dtype == D2C_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? D2C_OK : check_cuda(cudaErrorInvalidValue);
 }
 
 int tc_fwd(int dtype, const Args& a, cudaStream_t st) {

@@ -1,0 +1,415 @@
+// Gradients of cross attention on tensor cores (fp16 and bf16 tensors, head widths that are multiples of 8 up to 128).
+//
+// One kernel, two uses.  A block keeps a tile of 128 rows X (X1, X2) and runs over tiles of 128 rows Y (Y1, Y2):
+//   S = X1 Y1^T,  dP = X2 Y2^T,  P = 2^(S scale log2 e - lse),  dS = P (dP - delta)
+//   queries:  X = (q, grad_o), Y = (k, v):        grad_q += dS Y1
+//   keys:     X = (k, v),      Y = (q, grad_o):   grad_v += P Y2, grad_k += dS Y1      (S, P, dS are transposed; over all heads
+//                                                                                       that share the keys)
+// so that every gradient has one writer: no atomics, the same bits in every call, for 7 products a score instead of 5.  S, dP and
+// the accumulators fill tensor memory (4 x 128 columns); P and dS go back over S and dP as 16-bit A operands.  8 warps, a thread a
+// row and half of the columns.  The order of the issued products lets the tensor cores work on the next S while the warps form dS,
+// and on the next dP while they form P.
+//
+// fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
+// they are rounded (P by 2^14; dS so that 2 max|grad_o_i| max|v_j|, which bounds it, becomes 2^15) and the sums scaled back.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_tc.cuh"
+
+namespace d2c {
+namespace attn {
+namespace {
+
+struct BwdParams {
+  int B, Lq, Lk, Hq, Hkv, D;
+  float c, scale;
+  int splits, blocks_x;          // tiles of X per head
+  const float *lse, *delta;
+  const uint32_t* bounds;        // fp16: [B, Hkv] pairs: largest |grad_o_i|^2, |v_j|^2 (bits of a float)
+  void *g1, *g2;                 // keys: grad_v, grad_k; queries: g2 = grad_q
+  float* part;                   // queries [splits][B, Lq, Hq][D]; keys [grad_k, grad_v][splits][B, Lk, Hkv][D]
+  Args a;                        // lengths
+  int* status;
+};
+
+constexpr int kThreads = 384;                     // 8 working warps; MMA issuer, loader, two idle (see registers_up)
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+template <int DP>
+constexpr int kStages = DP == 64 ? 8 : 4;
+template <int DP>
+constexpr int kSmem = kTileBytes<DP> * (2 + kStages<DP>) + 1024;
+
+template <typename T, int DP, bool kKeys>
+__global__ void __launch_bounds__(kThreads, 1)
+bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2, const __grid_constant__ CUtensorMap my1,
+              const __grid_constant__ CUtensorMap my2, const __grid_constant__ BwdParams p) {
+  constexpr int kSt = kStages<DP>, kTB = kTileBytes<DP>;
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bars[2 * kSt + 8];
+  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][2][kRows];     // lse - kUp, delta of the queries of a Y tile
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t sx = base, ring = base + 2 * kTB, bar0 = ptx::smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8 * s; };
+  auto empty = [&](int s) { return bar0 + 8 * (kSt + s); };
+  const uint32_t x_full = bar0 + 16 * kSt, tail = x_full + 8, done = x_full + 16, s_full = x_full + 24, dp_full = x_full + 32,
+                 p_ready = x_full + 40, ds_ready = x_full + 48;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  long long id = blockIdx.x;
+  const int xb = (int)(id % p.blocks_x); id /= p.blocks_x;
+  const int split = (int)(id % p.splits); id /= p.splits;
+  const int heads = kKeys ? p.Hkv : p.Hq, head = (int)(id % heads), b = (int)(id / heads);
+  const int group = p.Hq / p.Hkv, hk = kKeys ? head : head / group;
+  const int x0 = xb * kRows;
+  const int len = key_length(p.a, b);
+  const int qtiles = (p.Lq + kRows - 1) / kRows;
+  int i0, i1;
+  share(kKeys ? qtiles * group : (len + kRows - 1) / kRows, p.splits, split, i0, i1);
+  if (kKeys && x0 >= len) i1 = i0;                // keys that are not there
+  const int n = i1 - i0;
+  // tile i of Y: head, first row
+  auto y_head = [&](int i) { return kKeys ? head * group + i / qtiles : hk; };
+  auto y_row = [&](int i) { return (kKeys ? i % qtiles : i) * kRows; };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSt; ++i) { ptx::mbar_init(full(i), 1); ptx::mbar_init(empty(i), 1); }
+    ptx::mbar_init(x_full, 1);
+    ptx::mbar_init(tail, 1);
+    ptx::mbar_init(done, 1);
+    ptx::mbar_init(s_full, 1);
+    ptx::mbar_init(dp_full, 1);
+    ptx::mbar_init(p_ready, 8);
+    ptx::mbar_init(ds_ready, 8);
+    abort_word = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = tmem_slot, tS = tmem, tD = tmem + 128, tA1 = tmem + 256, tA2 = tmem + 384;
+
+  if (warp >= 8) {
+    registers_down();
+    if (warp == kLoadWarp) {
+      int i = 0;                                  // Y tiles asked for: Y1 Y2 Y1 Y2 ...
+      if (n > 0) {
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(x_full, 2 * kTB);
+          tma_tile<DP>(sx, &mx1, head, x0, b, x_full);
+          tma_tile<DP>(sx + kTB, &mx2, head, x0, b, x_full);
+        }
+        for (; i < 2 * n; ++i) {
+          const int s = i % kSt, y = i0 + (i >> 1), h = y_head(y), r0 = y_row(y);
+          const bool second = i & 1;
+          if (!warp_wait(empty(s), ((i / kSt) & 1) ^ 1, abort_flag)) break;
+          if constexpr (kKeys) {
+            if (!second) {
+              const long long at = ((long long)b * p.Hq + h) * p.Lq + r0;
+#pragma unroll
+              for (int e = 0; e < kRows / 32; ++e) {
+                const int r = lane + 32 * e;
+                const bool live = r0 + r < p.Lq;  // queries that are not there: P = 0
+                rows_of_y[s >> 1][0][r] = live ? p.lse[at + r] - kUp : INFINITY;
+                rows_of_y[s >> 1][1][r] = live ? p.delta[at + r] : 0.f;
+              }
+              __syncwarp();
+            }
+          }
+          // keys behind the clip's length may hold anything: dS is 0 there, and 0 * NaN is NaN
+          const bool patch = !kKeys && !second && len - r0 < kRows && len < p.Lk;
+          const uint32_t bar = patch ? tail : full(s), dst = ring + s * kTB;
+          if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(bar, kTB);
+            tma_tile<DP>(dst, second ? &my2 : &my1, h, r0, b, bar);
+          }
+          if (patch) {                            // the last tile: once per block
+            drain(tail, 0);
+            clear_rows<DP>(dst, len - r0);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(full(s));
+          }
+        }
+        if (lane == 0) {
+          drain(x_full, 0);
+          for (int w = i > kSt ? i - kSt : 0; w < i; ++w) drain(full(w % kSt), (w / kSt) & 1);
+        }
+      }
+    } else if (warp == kMmaWarp && lane == 0 && n > 0) {
+      const uint32_t id_s = idesc_of<T>(kRows, false), id_a = idesc_of<T>((p.D + 15) & ~15, true);
+      const int ksteps = (p.D + 15) >> 4;
+      auto slot = [&](int i) { return ring + (i % kSt) * kTB; };
+      auto there = [&](int i) { return ptx::mbar_wait(full(i % kSt), (i / kSt) & 1, abort_flag); };
+      auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {
+#pragma unroll
+        for (int k = 0; k < kRows / 16; ++k)      // each half of the columns has its 16-bit values at its own start
+          umma_ts(acc, w + 8 * k + (k >= 4 ? 32 : 0), ptx::umma_desc_mnmajor_sw128(y + 2048 * k, kHalfBytes, 1024), id_a, more || k > 0);
+      };
+      auto run = [&]() {
+        if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
+        ptx::tc_fence_after();
+        mma_scores(tS, sx, slot(0), id_s, ksteps);
+        ptx::umma_commit(s_full);
+        if (!there(1)) return;
+        mma_scores(tD, sx + kTB, slot(1), id_s, ksteps);
+        ptx::umma_commit(dp_full);
+        if (!kKeys) ptx::umma_commit(empty(1));
+        for (int i = 0; i < n; ++i) {
+          const int y1 = 2 * i, y2 = y1 + 1;
+          const bool more = i + 1 < n;
+          if (!ptx::mbar_wait(p_ready, i & 1, abort_flag)) return;
+          ptx::tc_fence_after();
+          if constexpr (kKeys) {
+            weigh(tA1, tS, slot(y2), i > 0);
+            ptx::umma_commit(empty(y2 % kSt));
+          }
+          if (more) {
+            if (!there(y1 + 2)) return;
+            mma_scores(tS, sx, slot(y1 + 2), id_s, ksteps);
+            ptx::umma_commit(s_full);
+          }
+          if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
+          ptx::tc_fence_after();
+          weigh(tA2, tD, slot(y1), i > 0);
+          ptx::umma_commit(empty(y1 % kSt));
+          if (more) {
+            if (!there(y2 + 2)) return;
+            mma_scores(tD, sx + kTB, slot(y2 + 2), id_s, ksteps);
+            ptx::umma_commit(dp_full);
+            if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
+          }
+        }
+      };
+      run();
+      ptx::umma_commit(done);
+      drain(done, 0);
+    }
+  } else {
+    registers_up();
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, xi = x0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tS + 64 * half + lanes, d_at = tD + 64 * half + lanes;
+    float lse = INFINITY, delta = 0.f;            // queries: this row's
+    if (!kKeys && xi < p.Lq) {
+      const long long at = ((long long)b * p.Hq + head) * p.Lq + xi;
+      lse = p.lse[at] - kUp;
+      delta = p.delta[at];
+    }
+    const bool row_in = kKeys ? xi < len : true;
+    // fp16: dS leaves scaled by 2^down * 2^kUp ...
+    float ds_mul = 1.f, ds_back = 1.f;
+    if constexpr (kHalf) {
+      const uint32_t* q = p.bounds + 2 * ((long long)b * p.Hkv + hk);
+      const float bound = 2.f * sqrtf(__uint_as_float(q[0])) * sqrtf(__uint_as_float(q[1]));
+      int e = 0;                                  // 2^e * bound <= 2^15
+      if (bound > 0.f && bound < INFINITY) e = max(-100, min(100, 14 - ilogbf(bound)));
+      ds_mul = exp2f((float)e - kUp);
+      ds_back = exp2f((float)-e);
+    }
+    bool ok = true;
+    for (int i = 0; ok && i < n; ++i) {
+      if (!warp_wait(s_full, i & 1, abort_flag)) { ok = false; break; }
+      ptx::tc_fence_after();
+      uint32_t s[2][32];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) ptx::tmem_ld_32x32(s_at + 32 * k, s[k]);
+      ptx::tmem_ld_wait();
+      if constexpr (!kKeys) {                     // S has been read
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready);
+      }
+      const int valid = kKeys ? kRows : len - y_row(i0 + i);   // columns from there on are masked
+      const float* ly = kKeys ? &rows_of_y[(2 * i % kSt) >> 1][0][64 * half] : nullptr;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float4 l4 = make_float4(lse, lse, lse, lse);
+          if constexpr (kKeys) l4 = *reinterpret_cast<const float4*>(ly + 32 * k + e);
+          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float pr = exp2_fast(fmaf(__uint_as_float(s[k][e + u]), p.c, -lv[u]));
+            if (kKeys && !row_in) pr = 0.f;
+            s[k][e + u] = __float_as_uint(pr);
+          }
+        }
+      if constexpr (kKeys) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          w[e] = pack2<T>(__uint_as_float(s[e >> 4][2 * e & 31]), __uint_as_float(s[e >> 4][(2 * e & 31) + 1]));
+        tmem_st_32x32(s_at, w);
+        tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready);
+      }
+      if (!warp_wait(dp_full, i & 1, abort_flag)) { ok = false; break; }
+      ptx::tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t d[32];
+        ptx::tmem_ld_32x32(d_at + 32 * k, d);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float4 d4 = make_float4(delta, delta, delta, delta);
+          if constexpr (kKeys) d4 = *reinterpret_cast<const float4*>(ly + kRows + 32 * k + e);
+          const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+          float v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            v[u] = __uint_as_float(s[k][e + u]) * (__uint_as_float(d[e + u]) - dv[u]);
+            if constexpr (kHalf) v[u] *= ds_mul;
+            if (kKeys ? !row_in : 64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
+          }
+          w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
+          w[16 * k + e / 2 + 1] = pack2<T>(v[2], v[3]);
+        }
+      }
+      tmem_st_32x32(d_at, w);
+      tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) {
+      ok = warp_wait(done, 0, abort_flag);
+      ptx::tc_fence_after();
+    }
+    if (ok) {
+      // keys: the first four warps write grad_v, the others grad_k; queries: a half of the channels each
+      const int there = kKeys ? p.Lk : p.Lq;
+      const long long rows = (long long)p.B * there * heads, out = ((long long)b * there + xi) * heads + head;
+      const bool first = kKeys && half == 0;
+      const float mul = first ? exp2f(-kUp) : p.scale * ds_back;
+      const uint32_t acc = (first ? tA1 : tA2) + lanes;
+      T* dst = reinterpret_cast<T*>(first ? p.g1 : p.g2) + out * p.D;
+      float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
+      const int c_end = kKeys ? p.D : min(p.D, (half + 1) * (DP / 2));
+      for (int c0 = kKeys ? 0 : half * (DP / 2); c0 < c_end; c0 += 32) {
+        uint32_t r[32];
+        if (n > 0) {
+          ptx::tmem_ld_32x32(acc + c0, r);
+          ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+        }
+        if (xi >= there) continue;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (c0 + e >= c_end) break;
+          float f[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(r[e + u]) * mul;
+          if (part) {
+            *reinterpret_cast<float4*>(part + c0 + e) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(part + c0 + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          } else {
+            *reinterpret_cast<uint4*>(dst + c0 + e) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+          }
+        }
+      }
+    }
+    ptx::tc_fence_before();
+  }
+  __syncthreads();
+  report(p.status, abort_flag);
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Largest squared norm of a row of x [B, L, H, D] among the valid ones, per (clip, key head): bits of a float that is not negative
+// order like the float, so that the maximum does not depend on the order of the atomics (a NaN is above all).  A warp a row.
+__global__ void __launch_bounds__(256) row_bound_kernel(Args a, const __half* x, long long sb, long long sl, long long sh, int L, int H,
+                                                        int keys, uint32_t* out) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = blockIdx.y % H, b = blockIdx.y / H, hk = h / (H / a.Hkv);
+  const int len = keys ? key_length(a, b) : L;
+  float most = 0.f;
+  bool bad = false;
+  for (int r = blockIdx.x * 8 + warp; r < len; r += gridDim.x * 8) {
+    const __half* p = x + b * sb + (long long)r * sl + h * sh;
+    float s = 0.f;
+    for (int c = lane; c < a.D; c += 32) {
+      const float v = __half2float(p[c]);
+      s = fmaf(v, v, s);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    bad |= s != s;
+    most = fmaxf(most, s);
+  }
+  if (lane == 0 && len > 0) atomicMax(out + 2 * ((long long)b * a.Hkv + hk), bad ? 0x7fffffffu : __float_as_uint(most));
+}
+
+template <typename T, int DP, bool kKeys>
+int launch(const CUtensorMap (&m)[4], const BwdParams& p, cudaStream_t st) {
+  const long long blocks = (long long)p.blocks_x * p.splits * (kKeys ? p.Hkv : p.Hq) * p.B;
+  if (blocks > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
+  if (const int rc = allow_dynamic_smem<bwd_tc_kernel<T, DP, kKeys>>(kSmem<DP>)) return rc;
+  bwd_tc_kernel<T, DP, kKeys><<<(unsigned)blocks, kThreads, kSmem<DP>, st>>>(m[0], m[1], m[2], m[3], p);
+  D2C_LAUNCH_CHECK();
+  return D2C_OK;
+}
+template <typename T>
+int by_width(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStream_t st) {
+  if (keys) return p.D <= 64 ? launch<T, 64, true>(m, p, st) : launch<T, 128, true>(m, p, st);
+  return p.D <= 64 ? launch<T, 64, false>(m, p, st) : launch<T, 128, false>(m, p, st);
+}
+
+}  // namespace
+
+int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st) {
+  D2C_CUDA_TRY(cudaMemsetAsync(bounds, 0, sizeof(uint32_t) * 2 * a.B * a.Hkv, st));
+  const long long hq = (long long)a.B * a.Hq, hk = (long long)a.B * a.Hkv;
+  if (hq > 65535) return D2C_ERR_TOO_LARGE;
+  auto blocks = [](int L, long long heads) {
+    return (unsigned)std::max<long long>(1, std::min<long long>((L + 7) / 8, (148 * 8 + heads - 1) / heads));
+  };
+  row_bound_kernel<<<dim3(blocks(a.Lq, hq), (unsigned)hq), 256, 0, st>>>(a, (const __half*)a.g, a.gs[0], a.gs[1], a.gs[2], a.Lq, a.Hq, 0, bounds);
+  D2C_LAUNCH_CHECK();
+  row_bound_kernel<<<dim3(blocks(a.Lk, hk), (unsigned)hk), 256, 0, st>>>(a, (const __half*)a.v, a.vs[0], a.vs[1], a.vs[2], a.Lk, a.Hkv, 1, bounds + 1);
+  D2C_LAUNCH_CHECK();
+  return D2C_OK;
+}
+
+int tc_bwd(int dtype, const Args& a, bool keys, const uint32_t* bounds, cudaStream_t st) {
+  CUtensorMap q, k, v, g;
+  int rc;
+  if ((rc = tile_map(&q, dtype, a.q, a.D, a.Hq, a.Lq, a.B, a.qs))) return rc;
+  if ((rc = tile_map(&k, dtype, a.k, a.D, a.Hkv, a.Lk, a.B, a.ks))) return rc;
+  if ((rc = tile_map(&v, dtype, a.v, a.D, a.Hkv, a.Lk, a.B, a.vs))) return rc;
+  if ((rc = tile_map(&g, dtype, a.g, a.D, a.Hq, a.Lq, a.B, a.gs))) return rc;
+  const CUtensorMap maps[4] = {keys ? k : q, keys ? v : g, keys ? q : k, keys ? g : v};
+  BwdParams p{};
+  p.B = a.B; p.Lq = a.Lq; p.Lk = a.Lk; p.Hq = a.Hq; p.Hkv = a.Hkv; p.D = a.D;
+  p.c = a.scale * kLog2e; p.scale = a.scale;
+  p.splits = a.splits;
+  p.blocks_x = ((keys ? a.Lk : a.Lq) + kRows - 1) / kRows;
+  p.lse = a.lse; p.delta = a.delta; p.bounds = bounds;
+  p.g1 = a.gv; p.g2 = keys ? a.gk : a.gq;
+  p.part = a.part;
+  p.a = a;
+  if ((rc = status_pointer(&p.status))) return rc;
+  return dtype == D2C_BF16 ? by_width<__nv_bfloat16>(maps, p, keys, st) : by_width<__half>(maps, p, keys, st);
+}
+
+}  // namespace attn
+}  // namespace d2c

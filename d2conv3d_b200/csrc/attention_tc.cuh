@@ -131,6 +131,7 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
 
 // attention_sm100.cu: host helpers
 int status_pointer(int** out);
+int tile_map(CUtensorMap* map, int dtype, const void* p, int D, int heads, int tokens, int clips, const long long (&s)[3]);
 
 }  // namespace attn
 }  // namespace d2c

@@ -255,8 +255,16 @@ Tensor rotary(const Tensor& x, const OptTensor& positions_, const std::array<int
 
 // ---- cross attention --------------------------------------------------------------------------------------------
 
-// [B, L, H, D] with contiguous channels; any strides otherwise.
-Tensor rows_contiguous(const Tensor& t) { return t.size(3) > 1 && t.stride(3) != 1 ? t.contiguous() : t; }
+// [B, L, H, D] with contiguous channels; any strides otherwise, but where the fast kernels could read a head's rows 16 bytes at a
+// time if they were laid out so (or if a repeated dimension were written out), they are: a copy costs less than the slow kernels.
+Tensor attention_rows(const Tensor& t) {
+  if (t.size(3) > 1 && t.stride(3) != 1) return t.contiguous();
+  const int64_t piece = 16 / t.element_size();
+  if (t.size(3) % piece) return t;
+  bool fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d < 3; ++d) fits &= t.size(d) == 1 || (t.stride(d) > 0 && t.stride(d) % piece == 0);
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 void take_strides(int64_t (&out)[3], const Tensor& t) {
   for (int64_t d = 0; d < 3; ++d) out[d] = stride_or_zero(t, d);
 }
@@ -290,7 +298,7 @@ struct AttentionNode : public Node {
       if (empty) {
         gq.zero_(); gk.zero_(); gv.zero_();
       } else {
-        const Tensor g = rows_contiguous(grads[0]);
+        const Tensor g = attention_rows(grads[0]);
         d2c_attention_desc d = desc;
         take_strides(d.g_stride, g);
         const size_t n = d2c_attention_bwd_workspace_bytes(&d);
@@ -339,7 +347,7 @@ Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& val
   {
     at::AutoGradMode no_grad(false);
     c10::cuda::CUDAGuard guard(query.device());
-    q = rows_contiguous(query); k = rows_contiguous(key); v = rows_contiguous(value); n = contiguous(lengths);
+    q = attention_rows(query); k = attention_rows(key); v = attention_rows(value); n = contiguous(lengths);
     take_strides(d.q_stride, q); take_strides(d.k_stride, k); take_strides(d.v_stride, v);
     o = at::empty(query.sizes(), query.options().requires_grad(false));
     if (empty) {
