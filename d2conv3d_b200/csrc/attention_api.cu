@@ -15,11 +15,26 @@ struct Plan {
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Shares of an inner loop of `steps` steps, so that `blocks` blocks become about two per SM; no share under `least` steps.
-int shares(long long blocks, int steps, int least, int sms) {
-  if (blocks >= 2LL * sms) return 1;
-  return std::max(1, std::min({ceil_div(2LL * sms, blocks), steps / least, 128}));
+// Shares of an inner loop of `steps` steps: what costs least in steps, where `slots` blocks run at the same time, a block costs
+// `start` steps besides its loop, and joining costs `join` per share.  (A wave that is not full costs as much as a full one: 64
+// blocks of 102 steps on 148 SMs take 102 steps whole, 4 * 28.5 in 9 shares.)
+int shares(long long blocks, int steps, int slots, double start, double join) {
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= std::min(steps, 128); ++s) {
+    const long long waves = (blocks * s + slots - 1) / slots;
+    const double cost = waves * (ceil_div(steps, s) + start) + (s > 1 ? start + join * s : 0.0);
+    if (s == 1 || cost < least) { best = s; least = cost; }
+    if (s > 1 && waves > 16) break;
+  }
+  return best;
 }
+
+long long q_rows(const d2c_attention_desc& d) { return (long long)d.batch * d.queries * d.q_heads; }
+long long kv_rows(const d2c_attention_desc& d) { return (long long)d.batch * d.keys * d.kv_heads; }
+
+// What writing and reading one share's fp32 results takes, in steps of about 1.5 us, at 5 TB/s.
+double join_steps(long long rows, int dim) { return 8.0 * rows * dim / 5e6 / 1.5; }
 
 // 16-byte pieces of every row
 bool rows_fit(const d2c_attention_desc& d, const int64_t (&s)[3]) {
@@ -55,9 +70,9 @@ Plan plan_fwd(const d2c_attention_desc& d, bool aligned, int sms) {
     p.splits = std::max(1, std::min({ceil_div(4LL * sms, blocks), ceil_div(d.keys, 128), 128}));
   } else if (aligned && tensor_fits(d)) {
     p.path = Path::tensor;
-    p.splits = shares((long long)ceil_div(d.queries, 256) * d.q_heads * d.batch, ceil_div(d.keys, 128), 2, sms);
+    p.splits = shares((long long)ceil_div(d.queries, 256) * d.q_heads * d.batch, ceil_div(d.keys, 128), sms, 3.0, join_steps(q_rows(d), d.dim));
   } else {
-    p.splits = shares((long long)ceil_div(d.queries, kTile) * d.q_heads * d.batch, ceil_div(d.keys, kTile), 2, sms);
+    p.splits = shares((long long)ceil_div(d.queries, kTile) * d.q_heads * d.batch, ceil_div(d.keys, kTile), 2 * sms, 1.0, join_steps(q_rows(d), d.dim));
   }
   return p;
 }
@@ -70,13 +85,12 @@ Plan plan_bwd(const d2c_attention_desc& d, bool keys, bool aligned, int sms) {
     tile = 128;
   }
   const int q = ceil_div(d.queries, tile), k = ceil_div(d.keys, tile);
-  p.splits = keys ? shares((long long)k * d.kv_heads * d.batch, q * (d.q_heads / d.kv_heads), 2, sms)
-                  : shares((long long)q * d.q_heads * d.batch, k, 2, sms);
+  const int slots = p.path == Path::tensor ? sms : 2 * sms;
+  const double start = p.path == Path::tensor ? 3.0 : 1.0;
+  p.splits = keys ? shares((long long)k * d.kv_heads * d.batch, q * (d.q_heads / d.kv_heads), slots, start, join_steps(2 * kv_rows(d), d.dim))
+                  : shares((long long)q * d.q_heads * d.batch, k, slots, start, join_steps(q_rows(d), d.dim));
   return p;
 }
-
-long long q_rows(const d2c_attention_desc& d) { return (long long)d.batch * d.queries * d.q_heads; }
-long long kv_rows(const d2c_attention_desc& d) { return (long long)d.batch * d.keys * d.kv_heads; }
 
 size_t fwd_bytes(const d2c_attention_desc& d, const Plan& p) {
   if (p.splits == 1) return 0;

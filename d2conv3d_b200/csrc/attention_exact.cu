@@ -350,6 +350,7 @@ constexpr int kFewThreads = 128;
 template <typename T, int LPK, int R>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
   constexpr int V = 16 / (int)sizeof(T), kGroups = kFewThreads / LPK, kU = 4;
+  next_kernel_may_start();
   const int group = a.Hq / a.Hkv, all_rows = group * a.Lq, row_sets = (all_rows + R - 1) / R;
   long long id = blockIdx.x;
   const int set = (int)(id % row_sets); id /= row_sets;          // blocks that read the same keys run beside one another
@@ -418,36 +419,54 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
       }
     }
   }
-  // the groups' results, one row at a time
-  __shared__ float sm[kGroups], sl[kGroups], so[kGroups][LPK * V];
+  // the lane groups of a warp, then the warps
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    __syncthreads();
-    if (lane == 0) {
-      sm[grp] = m[r];
-      sl[grp] = l[r];
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int o = LPK; o < 32; o <<= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m[r], o), mx = fmaxf(m[r], om), shift = mx == -INFINITY ? 0.f : mx;
+      const float f = exp2f(m[r] - shift), of = exp2f(om - shift);
+      m[r] = mx;
+      l[r] = l[r] * f + __shfl_xor_sync(0xffffffffu, l[r], o) * of;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[r][e] = acc[r][e] * f + __shfl_xor_sync(0xffffffffu, acc[r][e], o) * of;
     }
+  constexpr int kWarps = kFewThreads / 32, kWidth = LPK * V;
+  __shared__ float sm[R][kWarps], sl[R][kWarps], so[R][kWarps][kWidth];
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) < LPK) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) so[grp][c + e] = acc[r][e];
-    __syncthreads();
-    const int row = set * R + r;
-    if (row >= all_rows) continue;                               // the same for the whole block
+    for (int r = 0; r < R; ++r) {
+      if (lane == 0) {
+        sm[r][warp] = m[r];
+        sl[r][warp] = l[r];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) so[r][warp][c + e] = acc[r][e];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * kWidth; i += kFewThreads) {
+    const int r = i / kWidth, d = i % kWidth, row = set * R + r;
+    if (row >= all_rows || d >= a.D) continue;
     float mx = -INFINITY;
-    for (int i = 0; i < kGroups; ++i) mx = fmaxf(mx, sm[i]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[r][w]);
     const float shift = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
-    for (int i = 0; i < kGroups; ++i) sum += sl[i] * exp2f(sm[i] - shift);
+    float sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(sm[r][w] - shift);
+      sum += sl[r][w] * f;
+      o = fmaf(so[r][w][d], f, o);
+    }
     const float inv = j1 == j0 || (a.splits > 1 && sum == 0.f) ? 0.f : 1.f / sum;
     const float lse = j1 > j0 ? mx + log2f(sum) : -INFINITY;
     const int qi = row / group, h = hk * group + row % group;
     const long long out = ((long long)b * a.Lq + qi) * a.Hq + h;
-    for (int d = threadIdx.x; d < a.D; d += kFewThreads) {
-      float o = 0.f;
-      for (int i = 0; i < kGroups; ++i) o = fmaf(so[i][d], exp2f(sm[i] - shift), o);
-      if (a.splits > 1) a.part[((long long)split * a.B * a.Lq * a.Hq + out) * a.D + d] = o * inv;
-      else reinterpret_cast<T*>(a.o)[out * a.D + d] = from_f32<T>(o * inv);
-    }
-    if (threadIdx.x == 0) {
+    if (a.splits > 1) a.part[((long long)split * a.B * a.Lq * a.Hq + out) * a.D + d] = o * inv;
+    else reinterpret_cast<T*>(a.o)[out * a.D + d] = from_f32<T>(o * inv);
+    if (d == 0) {
       if (a.splits > 1) a.part_lse[(long long)split * a.B * a.Lq * a.Hq + out] = lse;
       else if (a.lse) a.lse[((long long)b * a.Hq + h) * a.Lq + qi] = lse;
     }
@@ -456,29 +475,41 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
 
 // ---- joining shares -----------------------------------------------------------------------------------------
 
-// A warp per row: o = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m).
-template <typename T>
+// o = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m).  A block of 8 warps; W of them share a row's parts (1, or 8 where a few rows
+// have many parts: their loads then wait for memory at the same time).  Launched beside the kernel that writes the parts, which it
+// waits for: nothing here is read before that, and nothing through the read-only path.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) combine_kernel(Args a) {
-  const long long rows = (long long)a.B * a.Lq * a.Hq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  wait_for_kernels_before();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = warp % W;
+  const long long rows = (long long)a.B * a.Lq * a.Hq, row = (long long)blockIdx.x * (8 / W) + warp / W;
+  if (row >= rows) return;                                       // W = 8: the whole block
   float m = -INFINITY;
   for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_lse[s * rows + row]);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float shift = m == -INFINITY ? 0.f : m;
   float acc[4] = {}, sum = 0.f;
-  for (int s0 = 0; s0 < a.splits; s0 += 32) {
-    const float mine = s0 + lane < a.splits ? exp2f(a.part_lse[(s0 + lane) * rows + row] - shift) : 0.f;
-    const int n = min(32, a.splits - s0);
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float f = __shfl_sync(0xffffffffu, mine, s);
-      sum += f;
-      const float* p = a.part + ((long long)(s0 + s) * rows + row) * a.D;
+  for (int s = first; s < a.splits; s += W) {
+    const float f = exp2f(a.part_lse[s * rows + row] - shift);
+    const float* p = a.part + (s * rows + row) * a.D;
+    sum += f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < a.D) acc[e] = fmaf(f, p[lane + 32 * e], acc[e]);
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < a.D) acc[e] = fmaf(f, p[lane + 32 * e], acc[e]);
+  }
+  if constexpr (W > 1) {
+    __shared__ float sh[W][4][32], sums[W];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[warp][e][lane] = acc[e];
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (warp) return;
+    for (int w = 1; w < W; ++w) {
+      sum += sums[w];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += sh[w][e][lane];
     }
   }
   const int h = (int)(row % a.Hq);
@@ -602,16 +633,22 @@ int few_fwd(int dtype, const Args& a, cudaStream_t st) {
   }
 }
 
-int combine(int dtype, const Args& a, cudaStream_t st) {
+template <typename T>
+static int combine_typed(const Args& a, cudaStream_t st) {
+  const long long rows = (long long)a.B * a.Lq * a.Hq;
+  const bool wide = a.splits >= 16 && rows <= 148 * 16;          // 8 rows, 102 parts: 22.7 us with a warp a row
   unsigned grid = 0;
-  if (const int rc = grid_of(((long long)a.B * a.Lq * a.Hq + 7) / 8, &grid)) return rc;
-  switch (dtype) {
-    case D2C_F32: combine_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case D2C_F16: combine_kernel<__half><<<grid, 256, 0, st>>>(a); break;
-    default: combine_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a); break;
-  }
+  if (const int rc = grid_of(wide ? rows : (rows + 7) / 8, &grid)) return rc;
+  D2C_CUDA_TRY(launch_beside(wide ? combine_kernel<T, 8> : combine_kernel<T, 1>, dim3(grid), dim3(256), 0, st, a));
   D2C_LAUNCH_CHECK();
   return D2C_OK;
+}
+int combine(int dtype, const Args& a, cudaStream_t st) {
+  switch (dtype) {
+    case D2C_F32: return combine_typed<float>(a, st);
+    case D2C_F16: return combine_typed<__half>(a, st);
+    default: return combine_typed<__nv_bfloat16>(a, st);
+  }
 }
 
 int delta_rows(int dtype, const Args& a, cudaStream_t st) {

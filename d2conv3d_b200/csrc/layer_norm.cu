@@ -36,6 +36,31 @@ __device__ __forceinline__ float param(const void* p, int c, int f32, float none
   return f32 ? __ldg(reinterpret_cast<const float*>(p) + c) : to_f32(reinterpret_cast<const T*>(p)[c]);
 }
 
+// w and b as fp32 in shared memory: read once per block, whatever their type (read from global memory for every row, element by
+// element, they took two thirds of the time of 512 channels in fp16).  b may be NULL.
+template <typename T>
+__device__ __forceinline__ void stage_params(const NormArgs& a, float* w, float* b, int padded) {
+  for (int c = threadIdx.x; c < padded; c += blockDim.x) {
+    w[c] = c < a.C ? param<T>(a.w, c, a.param_f32, 1.f) : 0.f;
+    if (b) b[c] = c < a.C ? param<T>(a.b, c, a.param_f32, 0.f) : 0.f;
+  }
+  __syncthreads();
+}
+// VEC neighbouring channels of them.
+template <int VEC>
+__device__ __forceinline__ void params_at(const float* p, float (&f)[VEC]) {
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + e);
+      f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = p[e];
+  }
+}
+
 // ---- token rows -------------------------------------------------------------------------------------------
 
 // Sum of a and b over the TPR threads of a row (TPR lanes of a warp, or the whole block).
@@ -57,24 +82,37 @@ __device__ __forceinline__ void row_sum(float& a, float& b, float2* red) {
   }
 }
 
-// TPR threads a row, each with EPT channels as EPT / VEC vectors that lie TPR vectors apart.
+// TPR threads a row, each with EPT channels as EPT / VEC vectors that lie TPR vectors apart.  The next rows are asked for before
+// these are worked on.
 template <typename T, int VEC, int EPT, int TPR>
 __global__ void __launch_bounds__(256) norm_rows_fwd_kernel(NormArgs a) {
   constexpr int kChunks = EPT / VEC, kRows = 256 / TPR;
   __shared__ float2 red[8];
-  const int t = threadIdx.x % TPR, C = a.C;
-  const long long rows = a.V * a.batch;
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows) {
-    const long long row = r0 + threadIdx.x / TPR;
-    const bool live = row < rows;
+  extern __shared__ __align__(16) float wb[];
+  const int t = threadIdx.x % TPR, C = a.C, cpad = (C + 3) & ~3;
+  const long long rows = a.V * a.batch, step = (long long)gridDim.x * kRows;
+  auto ask = [&](long long row, Vec<T, VEC> (&v)[kChunks]) {
     const T* x = reinterpret_cast<const T*>(a.x) + row * C;
-    Vec<T, VEC> v[kChunks];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = (k * TPR + t) * VEC;
+      if (row < rows && c < C) v[k] = load_vec<T, VEC>(x + c);
+    }
+  };
+  Vec<T, VEC> v[kChunks], next[kChunks];
+  long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+  ask(row, next);
+  stage_params<T>(a, wb, wb + cpad, cpad);
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += step, row += step) {
+    const bool live = row < rows;
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) v[k] = next[k];
+    ask(row + step, next);
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (live && c < C) {
-        v[k] = load_vec<T, VEC>(x + c);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s += to_f32(v[k].v[e]);
       }
@@ -102,12 +140,12 @@ __global__ void __launch_bounds__(256) norm_rows_fwd_kernel(NormArgs a) {
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (c < C) {
+        float w[VEC], b[VEC];
+        params_at<VEC>(wb + c, w);
+        params_at<VEC>(wb + cpad + c, b);
         Vec<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = (to_f32(v[k].v[e]) - mean) * rstd;
-          o.v[e] = from_f32<T>(fmaf(h, param<T>(a.w, c + e, a.param_f32, 1.f), param<T>(a.b, c + e, a.param_f32, 0.f)));
-        }
+        for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(fmaf((to_f32(v[k].v[e]) - mean) * rstd, w[e], b[e]));
         store_vec<T, VEC>(y + c, o);
       }
     }
@@ -120,36 +158,52 @@ template <typename T, int VEC, int EPT, int TPR>
 __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
   constexpr int kChunks = EPT / VEC, kRows = 256 / TPR;
   __shared__ float2 red[8];
-  extern __shared__ float sums[];          // [kRows][C], where kRows > 1
+  extern __shared__ __align__(16) float sums[];   // [kRows][C] at the end, w before
   const int t = threadIdx.x % TPR, C = a.C;
-  const long long rows = a.V * a.batch;
+  const long long rows = a.V * a.batch, step = (long long)gridDim.x * kRows;
   float aw[EPT], ab[EPT];
 #pragma unroll
   for (int i = 0; i < EPT; ++i) aw[i] = ab[i] = 0.f;
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows) {
-    const long long row = r0 + threadIdx.x / TPR;
-    const bool live = row < rows;
-    const T* x = reinterpret_cast<const T*>(a.x) + row * C;
-    const T* g = reinterpret_cast<const T*>(a.g) + row * C;
-    const float2 st = live ? a.stats[row] : make_float2(0.f, 0.f);
-    Vec<T, VEC> xv[kChunks], gv[kChunks];
+  constexpr bool kAhead = EPT <= 16;       // the next rows are asked for before these are worked on, where registers allow
+  Vec<T, VEC> xv[kChunks], gv[kChunks], xn[kAhead ? kChunks : 1], gn[kAhead ? kChunks : 1];
+  float2 st, stn = make_float2(0.f, 0.f);
+  auto ask = [&](long long row, Vec<T, VEC>* x, Vec<T, VEC>* g, float2& s) {
+    const T* px = reinterpret_cast<const T*>(a.x) + row * C;
+    const T* pg = reinterpret_cast<const T*>(a.g) + row * C;
+    if (row < rows) s = a.stats[row];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
-      if (live && c < C) {
-        xv[k] = load_vec<T, VEC>(x + c);
-        gv[k] = load_vec<T, VEC>(g + c);
+      if (row < rows && c < C) {
+        x[k] = load_vec<T, VEC>(px + c);
+        g[k] = load_vec<T, VEC>(pg + c);
       }
+    }
+  };
+  long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+  if constexpr (kAhead) ask(row, xn, gn, stn);
+  stage_params<T>(a, sums, nullptr, (C + 3) & ~3);
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += step, row += step) {
+    const bool live = row < rows;
+    if constexpr (kAhead) {
+      st = stn;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) { xv[k] = xn[k]; gv[k] = gn[k]; }
+      ask(row + step, xn, gn, stn);
+    } else {
+      ask(row, xv, gv, st);
     }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (live && c < C) {
+        float w[VEC];
+        params_at<VEC>(sums + c, w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float h = (to_f32(xv[k].v[e]) - st.x) * st.y, gg = to_f32(gv[k].v[e]);
-          const float gw = gg * param<T>(a.w, c + e, a.param_f32, 1.f);
+          const float gw = gg * w[e];
           s1 += gw;
           s2 = fmaf(gw, h, s2);
           aw[k * VEC + e] = fmaf(gg, h, aw[k * VEC + e]);
@@ -166,12 +220,13 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (c < C) {
+        float w[VEC];
+        params_at<VEC>(sums + c, w);
         Vec<T, VEC> o;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float h = (to_f32(xv[k].v[e]) - st.x) * st.y;
-          const float gw = to_f32(gv[k].v[e]) * param<T>(a.w, c + e, a.param_f32, 1.f);
-          o.v[e] = from_f32<T>(st.y * (gw - s1 - h * s2));
+          o.v[e] = from_f32<T>(st.y * (to_f32(gv[k].v[e]) * w[e] - s1 - h * s2));
         }
         store_vec<T, VEC>(gx + c, o);
       }
@@ -318,11 +373,7 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
   float* wb = shared;                                                     // [2][C rounded up to whole groups]
   const int cpad = groups * EPT;
   float2* red = reinterpret_cast<float2*>(wb + 2 * cpad);                 // [2][groups][LV * VV]
-  for (int c = threadIdx.x; c < cpad; c += blockDim.x) {
-    wb[c] = c < C ? param<T>(a.w, c, a.param_f32, 1.f) : 0.f;
-    wb[cpad + c] = (!kBackward && c < C) ? param<T>(a.b, c, a.param_f32, 0.f) : 0.f;
-  }
-  __syncthreads();
+  stage_params<T>(a, wb, kBackward ? nullptr : wb + cpad, cpad);
   const int lv = threadIdx.x % LV, grp = threadIdx.x / LV, c0 = grp * EPT;
   const int n = min(max(C - c0, 0), EPT);                                 // channels that this thread has
   constexpr int kTile = LV * VV;
@@ -653,7 +704,8 @@ Plan make_plan(const d2c_layer_norm_desc& d, bool backward, bool aligned, int sm
       const int per = 256 / p.tpr;
       const long long groups = (rows + per - 1) / per, most = (long long)sms * (backward ? 2 : 8);
       p.blocks = (int)(groups < most ? groups : most);
-      p.smem = backward && per > 1 ? sizeof(float) * per * C : 0;
+      const int cpad = (C + 3) / 4 * 4;
+      p.smem = sizeof(float) * (backward ? std::max(per > 1 ? per * C : 0, cpad) : 2 * cpad);
     }
   } else {
     const int most_threads = 512;
@@ -705,7 +757,9 @@ int launch_rows(const NormArgs& a, const Plan& p, bool backward, cudaStream_t st
     if (rc) return rc;
     norm_rows_bwd_kernel<T, VEC, EPT, TPR><<<p.blocks, 256, p.smem, st>>>(a);
   } else {
-    norm_rows_fwd_kernel<T, VEC, EPT, TPR><<<p.blocks, 256, 0, st>>>(a);
+    const int rc = allow_dynamic_smem<norm_rows_fwd_kernel<T, VEC, EPT, TPR>>((int)p.smem);
+    if (rc) return rc;
+    norm_rows_fwd_kernel<T, VEC, EPT, TPR><<<p.blocks, 256, p.smem, st>>>(a);
   }
   D2C_LAUNCH_CHECK();
   return D2C_OK;

@@ -2,8 +2,8 @@
 // rest; pair i of section a turns by the angle p_a * base^(-2 i / n_a), n_a the section's channels, p_a the token's
 // position on that axis; the rest stays.  The gradient is the same with the angle's sign changed.
 //
-// HBM-bound: 2 * sizeof(T) bytes per element.  A thread holds the same pairs of every token it meets, so that their
-// frequencies are formed once; the angle is formed once per token and used for all heads.  Angles: position times
+// HBM-bound: 2 * sizeof(T) bytes per element.  A block forms the frequencies once, a thread holds the same pairs of every token it
+// meets; the angle is formed once per token and used for all heads.  Angles: position times
 // frequency in turns, in 64 bits, its whole turns taken off, then sin and cos in 32 bits: at position 100 000 a 32-bit
 // product would be off by thousandths of a turn.
 #include <algorithm>
@@ -28,74 +28,97 @@ struct RotaryArgs {
   float sign;
 };
 
-// V pairs of a thread: channels u0 .. and v0 .. (halves of a section), or 2 V neighbouring channels.
+// V pairs of a thread: channels u0 .. and v0 .. (halves of a section, which V divides), or 2 V neighbouring channels (which may
+// belong to two sections).  The first heads are asked for before the angles are formed.
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
-  const int j = threadIdx.x * V;                                 // first pair of this thread
-  // section of the pair: the three axes, then the rest
-  int axis = 0, start = 0, i = j;
-  while (axis < 3 && i >= a.n[axis] / 2) {
-    i -= a.n[axis] / 2;
-    start += a.n[axis];
-    ++axis;
+  constexpr int kHeads = 4;                                      // in flight
+  __shared__ double freqs[256];                                  // turns per position of every pair
+  const int pairs = a.dim / 2, j = threadIdx.x * V;              // first pair of this thread
+  int axis[V], u0 = 0, v0 = 0;                                   // 3: the rest, which stays
+  auto place = [&](int pair, int& start, int& i) {
+    int x = 0;
+    start = 0;
+    i = pair;
+    while (x < 3 && i >= a.n[x] / 2) {
+      i -= a.n[x] / 2;
+      start += a.n[x];
+      ++x;
+    }
+    return x;
+  };
+  for (int k = threadIdx.y * blockDim.x + threadIdx.x; k < pairs; k += blockDim.x * blockDim.y) {
+    int start, i;
+    const int x = place(k, start, i);
+    freqs[k] = x < 3 ? exp2(-2.0 * i / a.n[x] * a.log2_base) * 0.15915494309189533577 : 0.0;
   }
-  const bool turns = axis < 3;
-  const int half = (turns ? a.n[axis] : a.dim - start) / 2;
-  if (!turns && i >= half) return;                               // block rounded up to whole warps
-  const int u0 = kInterleaved ? start + 2 * i : start + i, v0 = start + i + half;
-  double freq[V];                                                // turns per position
+  __syncthreads();
+  double freq[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    freq[e] = turns ? exp2(-2.0 * (i + e) / a.n[axis] * a.log2_base) * 0.15915494309189533577 : 0.0;
+  for (int e = 0; e < V; ++e) {
+    int start, i;
+    axis[e] = place(j + e, start, i);
+    freq[e] = freqs[j + e];
+    if (e == 0) {
+      u0 = kInterleaved ? 2 * j : start + i;
+      v0 = start + i + (axis[0] < 3 ? a.n[axis[0]] : a.dim - start) / 2;
+    }
+  }
+  const bool turns = axis[0] < 3;                                // a thread whose first pair stays has none that turns
   for (long long tok = (long long)blockIdx.x * blockDim.y + threadIdx.y; tok < a.tokens; tok += (long long)gridDim.x * blockDim.y) {
     const long long b = tok / a.length;
     const int l = (int)(tok - b * a.length);
-    float c[V], s[V];
-    if (turns) {
-      double pos;
-      if (a.pos_kind == D2C_POS_GRID) {
-        const int row = l / a.grid_w, idx = axis == 2 ? l - row * a.grid_w : (axis == 1 ? row % a.grid_h : row / a.grid_h);
-        pos = idx * a.step[axis] + a.first[axis];
-      } else {
-        const long long at = b * a.pos_batch + (long long)l * 3 + axis;
-        pos = a.pos_kind == D2C_POS_I32   ? (double)reinterpret_cast<const int*>(a.positions)[at]
-              : a.pos_kind == D2C_POS_I64 ? (double)reinterpret_cast<const long long*>(a.positions)[at]
-                                          : (double)reinterpret_cast<const float*>(a.positions)[at];
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const double t = pos * freq[e];
-        sincospif(2.f * (float)(t - rint(t)), &s[e], &c[e]);
-        s[e] *= a.sign;
-      }
-    }
     const T* x = reinterpret_cast<const T*>(a.x) + b * a.sb + (long long)l * a.sl;
     T* y = reinterpret_cast<T*>(a.y) + tok * a.heads * a.dim;
-#pragma unroll 4
-    for (int h = 0; h < a.heads; ++h, x += a.sh, y += a.dim) {
-      if constexpr (kInterleaved) {
-        Vec<T, 2 * V> p = load_vec<T, 2 * V>(x + u0);
+    float c[V], s[V];
+    for (int h0 = 0; h0 < a.heads; h0 += kHeads, x += kHeads * a.sh, y += kHeads * a.dim) {
+      constexpr int kW = kInterleaved ? 2 * V : V;
+      Vec<T, kW> p[kHeads], q[kInterleaved ? 1 : kHeads];
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
+        if (h0 + h < a.heads) {
+          p[h] = load_vec<T, kW>(x + h * a.sh + u0);
+          if constexpr (!kInterleaved) q[h] = load_vec<T, kW>(x + h * a.sh + v0);
+        }
+      if (h0 == 0 && turns) {
+        double pos[3];
+        if (a.pos_kind == D2C_POS_GRID) {
+          const int row = l / a.grid_w;
+          pos[0] = (row / a.grid_h) * a.step[0] + a.first[0];
+          pos[1] = (row % a.grid_h) * a.step[1] + a.first[1];
+          pos[2] = (l - row * a.grid_w) * a.step[2] + a.first[2];
+        } else {
+          const long long at = b * a.pos_batch + (long long)l * 3;
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            pos[k] = a.pos_kind == D2C_POS_I32   ? (double)reinterpret_cast<const int*>(a.positions)[at + k]
+                     : a.pos_kind == D2C_POS_I64 ? (double)reinterpret_cast<const long long*>(a.positions)[at + k]
+                                                 : (double)reinterpret_cast<const float*>(a.positions)[at + k];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const double t = (axis[e] == 0 ? pos[0] : (axis[e] == 1 ? pos[1] : pos[2])) * freq[e];
+          sincospif(2.f * (float)(t - rint(t)), &s[e], &c[e]);
+          s[e] *= a.sign;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        if (h0 + h >= a.heads) break;
         if (turns) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float u = to_f32(p.v[2 * e]), v = to_f32(p.v[2 * e + 1]);
-            p.v[2 * e] = from_f32<T>(u * c[e] - v * s[e]);
-            p.v[2 * e + 1] = from_f32<T>(u * s[e] + v * c[e]);
+            T& ru = kInterleaved ? p[h].v[2 * e] : p[h].v[e];
+            T& rv = kInterleaved ? p[h].v[2 * e + 1] : q[kInterleaved ? 0 : h].v[e];
+            const float u = to_f32(ru), v = to_f32(rv);
+            if (!kInterleaved || axis[e] < 3) {                  // what stays keeps its bits
+              ru = from_f32<T>(u * c[e] - v * s[e]);
+              rv = from_f32<T>(u * s[e] + v * c[e]);
+            }
           }
         }
-        store_vec<T, 2 * V>(y + u0, p);
-      } else {
-        Vec<T, V> p = load_vec<T, V>(x + u0), q = load_vec<T, V>(x + v0);
-        if (turns) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float u = to_f32(p.v[e]), v = to_f32(q.v[e]);
-            p.v[e] = from_f32<T>(u * c[e] - v * s[e]);
-            q.v[e] = from_f32<T>(u * s[e] + v * c[e]);
-          }
-        }
-        store_vec<T, V>(y + u0, p);
-        store_vec<T, V>(y + v0, q);
+        store_vec<T, kW>(y + h * a.dim + u0, p[h]);
+        if constexpr (!kInterleaved) store_vec<T, kW>(y + h * a.dim + v0, q[h]);
       }
     }
   }
@@ -105,7 +128,7 @@ template <typename T, int V, bool kInterleaved>
 int launch(const RotaryArgs& a, cudaStream_t st) {
   int sms = 0;
   if (const int rc = device_sm_count(&sms)) return rc;
-  const int px = a.dim / 2 / V, py = std::max(1, 256 / px);
+  const int px = a.dim / 2 / V, py = std::max(1, 256 / px);      // px <= 256
   const long long blocks = std::min<long long>((a.tokens + py - 1) / py, (long long)sms * 16);
   rotary_kernel<T, V, kInterleaved><<<(unsigned)blocks, dim3(px, py), 0, st>>>(a);
   D2C_LAUNCH_CHECK();
@@ -118,7 +141,7 @@ int run(const d2c_rotary_desc& d, const RotaryArgs& a, cudaStream_t st) {
   auto fits = [&](int v) {
     const int run = d.interleaved ? 2 * v : v;                   // contiguous channels of one access
     for (int k = 0; k < 3; ++k)
-      if ((a.n[k] / 2) % v) return false;
+      if (!d.interleaved && (a.n[k] / 2) % v) return false;
     return (a.dim / 2) % v == 0 && a.sb % run == 0 && a.sl % run == 0 && a.sh % run == 0 &&
            run * (int)sizeof(T) <= 16 && aligned_to(a.x, run * sizeof(T)) && aligned_to(a.y, run * sizeof(T));
   };
