@@ -366,8 +366,23 @@ struct RowPiece {
 // A tile is LV * VV neighbouring positions with all their channels: LV threads, of VV positions each, by groups of EPT
 // neighbouring channels.  A warp's access to one channel is a contiguous run of positions; a thread's channels of a position
 // are contiguous in a token row and move as 32-byte accesses, one full sector each, without a detour through shared memory.
+// EPT channels of a thread's positions, `stride` apart; what is not there is zero.
+template <typename T, int EPT, int VV>
+__device__ __forceinline__ void load_cells(Cell<T, VV> (&v)[EPT], const T* p, long long stride, bool live, bool whole, int n) {
+  if (live && whole) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e, p += stride) v[e].load(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e, p += stride) {
+      if (live && e < n) v[e].load(p);
+      else v[e].clear();
+    }
+  }
+}
+
 template <typename T, int EPT, int LV, int VV, bool kTokens, bool kBackward>
-__global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
+__global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume_kernel(NormArgs a) {
   extern __shared__ float shared[];
   const int C = a.C, groups = blockDim.x / LV;
   float* wb = shared;                                                     // [2][C rounded up to whole groups]
@@ -381,18 +396,20 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
   const long long tiles_b = (a.V + kTile - 1) / kTile, tiles = tiles_b * a.batch;
   constexpr int kKeep = kBackward ? (EPT > LV ? EPT / LV : 1) : 1;
   float aw[kKeep] = {}, ab[kKeep] = {};
+  // tile -> clip, place in it: divided once, then stepped
+  const long long step_b = gridDim.x / tiles_b, step_t = gridDim.x % tiles_b;
+  long long b = blockIdx.x / tiles_b, tb = blockIdx.x % tiles_b;
+  const int parts = (C + EPT - 1) / EPT, last = C - (parts - 1) * EPT;    // groups that have channels; of the last one
+  const bool whole = n == EPT;
   int turn = 0;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-    const long long b = tile / tiles_b, p = (tile % tiles_b) * kTile + lv * VV;
+  for (long long tile = blockIdx.x; tile < tiles;
+       tile += gridDim.x, turn ^= 1, b += step_b, tb += step_t, b += tb >= tiles_b, tb -= tb >= tiles_b ? tiles_b : 0) {
+    const long long p = tb * kTile + lv * VV;
     const bool live = p < a.V;             // VV > 1 only where it divides V
     const long long vol = (b * C + c0) * a.V + p, tok = (b * a.V + p) * C + c0;
     const T* x = reinterpret_cast<const T*>(a.x) + vol;
     Cell<T, VV> xv[EPT];
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      if (live && e < n) xv[e].load(x + e * a.V);
-      else xv[e].clear();
-    }
+    load_cells<T, EPT, VV>(xv, x, a.V, live, whole, n);
     float2* slot = red + turn * groups * kTile;    // the other half is still read by threads that are behind
     if constexpr (!kBackward) {
       // mean and sum of squares around it, of each thread's channels; merged: the squares of the means' distances come in too
@@ -406,7 +423,7 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
           const float d = xv[e].get(i) - m;
-          if (e < n) q = fmaf(d, d, q);
+          if (whole || e < n) q = fmaf(d, d, q);
         }
         slot[grp * kTile + lv * VV + i] = make_float2(m, q);
       }
@@ -415,14 +432,15 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < VV; ++i) {
         float m = 0.f, q = 0.f;
-        for (int k = 0; k < groups; ++k) m = fmaf(slot[k * kTile + lv * VV + i].x, (float)min(max(C - k * EPT, 0), EPT), m);
-        m /= (float)C;
-        for (int k = 0; k < groups; ++k) {
+        for (int k = 0; k < parts - 1; ++k) m += slot[k * kTile + lv * VV + i].x;
+        const float2 end = slot[(parts - 1) * kTile + lv * VV + i];
+        m = (m * (float)EPT + end.x * (float)last) / (float)C;
+        for (int k = 0; k < parts - 1; ++k) {
           const float2 s = slot[k * kTile + lv * VV + i];
           const float d = s.x - m;
-          const int nk = min(max(C - k * EPT, 0), EPT);
-          if (nk) q += fmaf(d * d, (float)nk, s.y);
+          q = fmaf(d * (float)EPT, d, q) + s.y;
         }
+        q = fmaf((end.x - m) * (float)last, end.x - m, q) + end.y;
         mean[i] = m;
         rstd[i] = 1.f / sqrtf(q / (float)C + a.eps);
         if (live && a.stats && grp == 0) a.stats[b * a.V + p + i] = make_float2(m, rstd[i]);
@@ -430,37 +448,46 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
       if (live) {
         if constexpr (kTokens) {
 #pragma unroll
-          for (int i = 0; i < VV; ++i) {
-            T* y = reinterpret_cast<T*>(a.y) + tok + (long long)i * C;
+          for (int e0 = 0; e0 < EPT; e0 += kW) {
+            float w[kW], bb[kW];
+            params_at<kW>(wb + c0 + e0, w);
+            params_at<kW>(wb + cpad + c0 + e0, bb);
 #pragma unroll
-            for (int e0 = 0; e0 < EPT; e0 += kW) {
+            for (int i = 0; i < VV; ++i) {
+              T* y = reinterpret_cast<T*>(a.y) + tok + (long long)i * C + e0;
               RowPiece<T, kW> o;
 #pragma unroll
               for (int k = 0; k < RowPiece<T, kW>::kWords; ++k) {
                 float f[4 / sizeof(T)];
 #pragma unroll
                 for (int j = 0; j < 4 / (int)sizeof(T); ++j) {
-                  const int e = e0 + k * (4 / (int)sizeof(T)) + j;
-                  f[j] = fmaf((xv[e].get(i) - mean[i]) * rstd[i], wb[c0 + e], wb[cpad + c0 + e]);
+                  const int e = k * (4 / (int)sizeof(T)) + j;
+                  f[j] = fmaf((xv[e0 + e].get(i) - mean[i]) * rstd[i], w[e], bb[e]);
                 }
                 Cell<T, 4 / sizeof(T)> c;
                 c.set(f);
                 o.w[k] = *reinterpret_cast<const uint32_t*>(&c.raw);
               }
-              if (!a.vec_tokens) o.store(y + e0, n - e0);
-              else if (e0 < n) o.store(y + e0);
+              if (!a.vec_tokens) o.store(y, n - e0);
+              else if (e0 < n) o.store(y);
             }
           }
         } else {
           T* y = reinterpret_cast<T*>(a.y) + vol;
 #pragma unroll
-          for (int e = 0; e < EPT; ++e) {
-            float f[VV];
+          for (int e0 = 0; e0 < EPT; e0 += 4) {
+            float w[4], bb[4];
+            params_at<4>(wb + c0 + e0, w);
+            params_at<4>(wb + cpad + c0 + e0, bb);
 #pragma unroll
-            for (int i = 0; i < VV; ++i) f[i] = fmaf((xv[e].get(i) - mean[i]) * rstd[i], wb[c0 + e], wb[cpad + c0 + e]);
-            Cell<T, VV> o;
-            o.set(f);
-            if (e < n) o.store(y + e * a.V);
+            for (int k = 0; k < 4; ++k, y += a.V) {
+              float f[VV];
+#pragma unroll
+              for (int i = 0; i < VV; ++i) f[i] = fmaf((xv[e0 + k].get(i) - mean[i]) * rstd[i], w[k], bb[k]);
+              Cell<T, VV> o;
+              o.set(f);
+              if (whole || e0 + k < n) o.store(y);
+            }
           }
         }
       }
@@ -491,11 +518,7 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
         }
       } else {
         const T* g = reinterpret_cast<const T*>(a.g) + vol;
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-          if (live && e < n) gv[e].load(g + e * a.V);
-          else gv[e].clear();
-        }
+        load_cells<T, EPT, VV>(gv, g, a.V, live, whole, n);
       }
       float2 st[VV];
 #pragma unroll
@@ -503,11 +526,14 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
         st[i] = live ? a.stats[b * a.V + p + i] : make_float2(0.f, 0.f);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-          if (e < n) {
-            const float gw = gv[e].get(i) * wb[c0 + e];
+        for (int e0 = 0; e0 < EPT; e0 += 4) {
+          float w[4];
+          params_at<4>(wb + c0 + e0, w);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {                                   // channels that are not there: g = w = 0
+            const float gw = gv[e0 + k].get(i) * w[k];
             s1 += gw;
-            s2 = fmaf(gw, (xv[e].get(i) - st[i].x) * st[i].y, s2);
+            s2 = fmaf(gw, (xv[e0 + k].get(i) - st[i].x) * st[i].y, s2);
           }
         }
         slot[grp * kTile + lv * VV + i] = make_float2(s1, s2);
@@ -536,7 +562,7 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < VV; ++i) {
           float s1 = 0.f, s2 = 0.f;
-          for (int k = 0; k < groups; ++k) {
+          for (int k = 0; k < parts; ++k) {
             const float2 s = slot[k * kTile + lv * VV + i];
             s1 += s.x;
             s2 += s.y;
@@ -546,16 +572,21 @@ __global__ void __launch_bounds__(512) norm_volume_kernel(NormArgs a) {
         }
         T* gx = reinterpret_cast<T*>(a.y) + vol;
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-          float f[VV];
+        for (int e0 = 0; e0 < EPT; e0 += 4) {
+          float w[4];
+          params_at<4>(wb + c0 + e0, w);
 #pragma unroll
-          for (int i = 0; i < VV; ++i) {
-            const float h = (xv[e].get(i) - st[i].x) * st[i].y;
-            f[i] = st[i].y * (gv[e].get(i) * wb[c0 + e] - m1[i] - h * m2[i]);
+          for (int k = 0; k < 4; ++k, gx += a.V) {
+            float f[VV];
+#pragma unroll
+            for (int i = 0; i < VV; ++i) {
+              const float h = (xv[e0 + k].get(i) - st[i].x) * st[i].y;
+              f[i] = st[i].y * (fmaf(gv[e0 + k].get(i), w[k], -m1[i]) - h * m2[i]);
+            }
+            Cell<T, VV> o;
+            o.set(f);
+            if (live && (whole || e0 + k < n)) o.store(gx);
           }
-          Cell<T, VV> o;
-          o.set(f);
-          if (live && e < n) o.store(gx + e * a.V);
         }
       }
     }
@@ -708,10 +739,12 @@ Plan make_plan(const d2c_layer_norm_desc& d, bool backward, bool aligned, int sm
       p.smem = sizeof(float) * (backward ? std::max(per > 1 ? per * C : 0, cpad) : 2 * cpad);
     }
   } else {
-    const int most_threads = 512;
+    // two pairs of positions a thread take 100 registers and more: blocks of 256 threads, so that a SM has several to switch
+    // between (1024 channels in bf16: 46 and 66 us instead of 56 and 72 in blocks of 512)
     p.ept = C <= 64 ? 8 : 32;
     const int groups = (C + p.ept - 1) / p.ept;
     p.vv = (size == 2 && d.positions % 2 == 0 && aligned) ? 2 : 1;
+    const int most_threads = p.vv == 2 && groups <= 32 ? 256 : 512;
     p.lv = 32;
     while (p.lv > 8 && (p.lv * groups > most_threads ||
                         ((d.positions + p.lv * p.vv - 1) / (p.lv * p.vv)) * d.batch < 2 * sms))
