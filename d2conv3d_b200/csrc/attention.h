@@ -48,11 +48,18 @@ int combine(int dtype, const Args& a, cudaStream_t st);          // partial outp
 int delta_rows(int dtype, const Args& a, cudaStream_t st);
 int sum_parts(int dtype, const float* part, int splits, long long n, void* out, cudaStream_t st);
 
-// ---- attention_sm100.cu: 16-bit types, 16-byte rows, positive strides, scale >= 0
-int tc_fwd(int dtype, const Args& a, cudaStream_t st);
-// ---- attention_sm100_bwd.cu: the same, and grad_o's rows
+// ---- tensor cores: operands with positive strides and 16-byte rows, scale > 0
+struct Operand {
+  const void* p;
+  long long s[3];                        // clip, token, head
+};
+// attention_sm100.cu.  fp32: operands staged by split_rows, in `parts` parts
+size_t split_bytes(int B, int L, int H, int D, int parts);
+int split_rows(const Args& a, int parts, void* workspace, Operand (&o)[4], cudaStream_t st);      // q, k, v, and g if there is one
+int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, cudaStream_t st);
+// attention_sm100_bwd.cu
 int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st);              // fp16: [B, Hkv][2], for tc_bwd
-int tc_bwd(int dtype, const Args& a, bool keys, const uint32_t* bounds, cudaStream_t st);
+int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys, const uint32_t* bounds, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace d2c

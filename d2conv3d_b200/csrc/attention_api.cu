@@ -11,21 +11,23 @@ enum class Path { few, exact, tensor };
 struct Plan {
   Path path;
   int splits;
+  int parts;           // tensor: parts of an operand
 };
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Shares of an inner loop of `steps` steps: what costs least in steps, where `slots` blocks run at the same time, a block costs
 // `start` steps besides its loop, and joining costs `join` per share.  (A wave that is not full costs as much as a full one: 64
-// blocks of 102 steps on 148 SMs take 102 steps whole, 4 * 28.5 in 9 shares.)
-int shares(long long blocks, int steps, int slots, double start, double join) {
-  int best = 1;
+// blocks of 102 steps on 148 SMs take 102 steps whole, 4 * 28.5 in 9 shares.)  At least `fewest` of them.
+int shares(long long blocks, int steps, int slots, double start, double join, int fewest) {
+  fewest = std::max(1, std::min(fewest, steps));
+  int best = fewest;
   double least = 0;
-  for (int s = 1; s <= std::min(steps, 128); ++s) {
+  for (int s = fewest; s <= std::min(steps, fewest + 127); ++s) {
     const long long waves = (blocks * s + slots - 1) / slots;
     const double cost = waves * (ceil_div(steps, s) + start) + (s > 1 ? start + join * s : 0.0);
-    if (s == 1 || cost < least) { best = s; least = cost; }
-    if (s > 1 && waves > 16) break;
+    if (s == fewest || cost < least) { best = s; least = cost; }
+    if (s > fewest && waves > 16) break;
   }
   return best;
 }
@@ -46,67 +48,97 @@ bool few_fits(const d2c_attention_desc& d) {
   return d.dim % v == 0 && rows_fit(d, d.q_stride) && rows_fit(d, d.k_stride) && rows_fit(d, d.v_stride);
 }
 
-// What the tensor-core kernels' tensor maps take: 16-bit types, 16-byte rows, no dimension that repeats its elements, strides under
-// 2^40 bytes; and, for the running maximum to be that of the raw scores, a scale above zero.
+// What the tensor-core kernels' tensor maps take: 16-byte rows, no dimension that repeats its elements, strides under 2^40 bytes.
 bool tensor_rows(const d2c_attention_desc& d, const int64_t (&s)[3], int tokens, int heads) {
   const int n[3] = {d.batch, tokens, heads};
   for (int i = 0; i < 3; ++i)
     if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= 1LL << 39)) return false;
   return true;
 }
-bool tensor_fits(const d2c_attention_desc& d) {
-  if (d.dtype == D2C_F32 || d.dim % 8 || !(d.scale > 1e-30f)) return false;
-  return tensor_rows(d, d.q_stride, d.queries, d.q_heads) && tensor_rows(d, d.k_stride, d.keys, d.kv_heads) &&
-         tensor_rows(d, d.v_stride, d.keys, d.kv_heads);
+
+// Parts of the tensor-core kernels' operands; 0 where they do not apply.  fp32 goes by the math mode: hi and lo parts for parity
+// (the gradients' operands fit shared memory up to 64 channels), hi alone, or CUDA cores.  The running maximum is that of the raw
+// scores, so the scale has to be above zero.
+int tensor_parts(const d2c_attention_desc& d, int mode, bool aligned, bool backward) {
+  if (!aligned || !(d.scale > 1e-30f)) return 0;
+  if (d.dtype == D2C_F32) {
+    if (mode == D2C_MATH_FP32) return 0;
+    if (mode == D2C_MATH_BF16) return 1;
+    return backward && d.dim > 64 ? 0 : 2;
+  }
+  return d.dim % 8 == 0 && tensor_rows(d, d.q_stride, d.queries, d.q_heads) && tensor_rows(d, d.k_stride, d.keys, d.kv_heads) &&
+         tensor_rows(d, d.v_stride, d.keys, d.kv_heads) && (!backward || tensor_rows(d, d.g_stride, d.queries, d.q_heads));
+}
+
+// The tensor cores add into their accumulator with truncation: a chain of n accumulating products loses about n * 2^-27 of the
+// result.  With two parts (24 products a tile) a share ends after 12 tiles, 2e-6, and the shares are added in fp32 -- unless their
+// results would take more than 2 GB.
+constexpr int kChainTiles = 12;
+int fewest_shares(int parts, int steps, long long rows, int dim) {
+  if (parts != 2) return 1;
+  return (int)std::min<long long>(ceil_div(steps, kChainTiles), std::max(1LL, (2LL << 30) / (4 * rows * dim)));
+}
+
+Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, int steps_rows, int sms) {
+  const bool tensor = parts > 0;
+  const int tile = tensor ? 128 : kTile;
+  const int steps = ceil_div(steps_rows, tile);
+  return {tensor ? Path::tensor : Path::exact,
+          shares((long long)ceil_div(rows_x, tile * per_block) * heads_x * d.batch, steps, tensor ? sms : 2 * sms, tensor ? 3.0 : 1.0,
+                 join_steps(rows_out, d.dim), fewest_shares(parts, steps, rows_out, d.dim)),
+          parts};
 }
 
 // few: up to 16 query rows on a head's keys; every four rows read the keys once, from L2 after the first.
-Plan plan_fwd(const d2c_attention_desc& d, bool aligned, int sms) {
-  Plan p{Path::exact, 1};
+Plan plan_fwd(const d2c_attention_desc& d, int mode, bool aligned, int sms) {
   const long long rows = (long long)d.q_heads / d.kv_heads * d.queries;
   if (rows <= 16 && few_fits(d) && aligned) {
-    p.path = Path::few;
     const long long blocks = (long long)ceil_div(rows, kFewRows) * d.kv_heads * d.batch;
-    p.splits = std::max(1, std::min({ceil_div(4LL * sms, blocks), ceil_div(d.keys, 128), 128}));
-  } else if (aligned && tensor_fits(d)) {
-    p.path = Path::tensor;
-    p.splits = shares((long long)ceil_div(d.queries, 256) * d.q_heads * d.batch, ceil_div(d.keys, 128), sms, 3.0, join_steps(q_rows(d), d.dim));
-  } else {
-    p.splits = shares((long long)ceil_div(d.queries, kTile) * d.q_heads * d.batch, ceil_div(d.keys, kTile), 2 * sms, 1.0, join_steps(q_rows(d), d.dim));
+    return {Path::few, std::max(1, std::min({ceil_div(4LL * sms, blocks), ceil_div(d.keys, 128), 128})), 0};
   }
-  return p;
+  const int parts = tensor_parts(d, mode, aligned, false);
+  const bool two_tiles = parts > 0 && !(parts == 2 && d.dim > 64);
+  return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), two_tiles ? 2 : 1, d.keys, sms);
 }
 // A gradient kernel's block has a tile of one side and runs over the other.
-Plan plan_bwd(const d2c_attention_desc& d, bool keys, bool aligned, int sms) {
-  Plan p{Path::exact, 1};
-  int tile = kTile;
-  if (aligned && tensor_fits(d) && tensor_rows(d, d.g_stride, d.queries, d.q_heads)) {
-    p.path = Path::tensor;
-    tile = 128;
-  }
-  const int q = ceil_div(d.queries, tile), k = ceil_div(d.keys, tile);
-  const int slots = p.path == Path::tensor ? sms : 2 * sms;
-  const double start = p.path == Path::tensor ? 3.0 : 1.0;
-  p.splits = keys ? shares((long long)k * d.kv_heads * d.batch, q * (d.q_heads / d.kv_heads), slots, start, join_steps(2 * kv_rows(d), d.dim))
-                  : shares((long long)q * d.q_heads * d.batch, k, slots, start, join_steps(q_rows(d), d.dim));
-  return p;
+Plan plan_bwd(const d2c_attention_desc& d, int mode, bool keys, bool aligned, int sms) {
+  const int parts = tensor_parts(d, mode, aligned, true);
+  if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, sms);
+  const int tile = parts ? 128 : kTile;
+  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), sms);
 }
 
 size_t fwd_bytes(const d2c_attention_desc& d, const Plan& p) {
-  if (p.splits == 1) return 0;
-  return align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256) + align_up(sizeof(float) * p.splits * q_rows(d), 256);
+  size_t n = 0;
+  if (p.path == Path::tensor && d.dtype == D2C_F32)
+    n += split_bytes(d.batch, d.queries, d.q_heads, d.dim, p.parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, p.parts);
+  if (p.splits > 1)
+    n += align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256) + align_up(sizeof(float) * p.splits * q_rows(d), 256);
+  return n;
 }
-size_t bwd_part_bytes(const d2c_attention_desc& d, int sms) {
-  size_t most = 0;                    // whatever the pointers' alignment, and so the plan, turns out to be
-  for (int al = 0; al < 2; ++al) {
-    const int sq = plan_bwd(d, false, al, sms).splits, skv = plan_bwd(d, true, al, sms).splits;
-    if (sq > 1) most = std::max<size_t>(most, sizeof(float) * sq * q_rows(d) * d.dim);
-    if (skv > 1) most = std::max<size_t>(most, sizeof(float) * 2 * skv * kv_rows(d) * d.dim);
-  }
-  return align_up(most, 256);
+size_t fwd_workspace(const d2c_attention_desc& d, int mode, int sms) {
+  size_t n = 0;                       // whatever the pointers' alignment, and so the plan, turns out to be
+  for (int al = 0; al < 2; ++al) n = std::max(n, fwd_bytes(d, plan_fwd(d, mode, al, sms)));
+  return n;
 }
+
 size_t delta_bytes(const d2c_attention_desc& d) { return align_up(sizeof(float) * q_rows(d), 256); }
 size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 2 * d.batch * d.kv_heads, 256); }
+size_t staged_bytes(const d2c_attention_desc& d, int parts) {
+  if (d.dtype != D2C_F32 || !parts) return 0;
+  return 2 * split_bytes(d.batch, d.queries, d.q_heads, d.dim, parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, parts);
+}
+size_t bwd_bytes(const d2c_attention_desc& d, const Plan& pq, const Plan& pk) {
+  size_t part = 0;                    // one gradient kernel's shares at a time
+  if (pq.splits > 1) part = std::max<size_t>(part, sizeof(float) * pq.splits * q_rows(d) * d.dim);
+  if (pk.splits > 1) part = std::max<size_t>(part, sizeof(float) * 2 * pk.splits * kv_rows(d) * d.dim);
+  return delta_bytes(d) + bound_bytes(d) + staged_bytes(d, pq.parts) + align_up(part, 256);
+}
+size_t bwd_workspace(const d2c_attention_desc& d, int mode, int sms) {
+  size_t n = 0;
+  for (int al = 0; al < 2; ++al) n = std::max(n, bwd_bytes(d, plan_bwd(d, mode, false, al, sms), plan_bwd(d, mode, true, al, sms)));
+  return n;
+}
 
 int checked(const d2c_attention_desc* d) {
   if (!d) return D2C_ERR_NULL;
@@ -134,42 +166,65 @@ Args make_args(const d2c_attention_desc& d, const void* q, const void* k, const 
 
 bool ws_ok(const void* ws, size_t have, size_t need) { return need == 0 || (ws && aligned_to(ws, 256) && have >= need); }
 
-int run_fwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaStream_t st) {
-  const Plan p = plan_fwd(d, aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.o, 16), sms);
+// The tensors themselves as operands (16-bit types).
+void own_operands(const Args& a, Operand (&o)[4]) {
+  const void* p[4] = {a.q, a.k, a.v, a.g};
+  const long long* s[4] = {a.qs, a.ks, a.vs, a.gs};
+  for (int i = 0; i < 4; ++i) o[i] = {p[i], {s[i][0], s[i][1], s[i][2]}};
+}
+
+int run_fwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int sms, cudaStream_t st) {
+  const Plan p = plan_fwd(d, mode, aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.o, 16), sms);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.splits = p.splits;
   if (p.splits > 1) {
-    a.part = reinterpret_cast<float*>(workspace);
-    a.part_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) +
-                                          align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256));
+    a.part = reinterpret_cast<float*>(ws);
+    ws += align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256);
+    a.part_lse = reinterpret_cast<float*>(ws);
+    ws += align_up(sizeof(float) * p.splits * q_rows(d), 256);
   }
-  const int rc = p.path == Path::few      ? few_fwd(d.dtype, a, st)
-                 : p.path == Path::tensor ? tc_fwd(d.dtype, a, st)
-                                          : exact_fwd(d.dtype, a, st);
+  int rc;
+  if (p.path == Path::tensor) {
+    Operand x[4];
+    own_operands(a, x);
+    if (d.dtype == D2C_F32 && (rc = split_rows(a, p.parts, ws, x, st))) return rc;
+    rc = tc_fwd(d.dtype, a, x, p.parts, st);
+  } else {
+    rc = p.path == Path::few ? few_fwd(d.dtype, a, st) : exact_fwd(d.dtype, a, st);
+  }
   if (rc || p.splits == 1) return rc;
   return combine(d.dtype, a, st);
 }
 
-int run_bwd(const d2c_attention_desc& d, Args a, void* workspace, int sms, cudaStream_t st) {
-  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  a.delta = reinterpret_cast<float*>(ws);
-  uint32_t* bounds = reinterpret_cast<uint32_t*>(ws + delta_bytes(d));
-  a.part = reinterpret_cast<float*>(ws + delta_bytes(d) + bound_bytes(d));
+int run_bwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int sms, cudaStream_t st) {
   const bool aligned = aligned_to(a.q, 16) && aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.g, 16) &&
                        aligned_to(a.gq, 16) && aligned_to(a.gk, 16) && aligned_to(a.gv, 16);
-  int rc = delta_rows(d.dtype, a, st);
-  if (rc) return rc;
-  const Plan pk = plan_bwd(d, true, aligned, sms), pq = plan_bwd(d, false, aligned, sms);
+  const Plan pk = plan_bwd(d, mode, true, aligned, sms), pq = plan_bwd(d, mode, false, aligned, sms);
   const bool tensor = pk.path == Path::tensor;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.delta = reinterpret_cast<float*>(ws);
+  ws += delta_bytes(d);
+  uint32_t* bounds = reinterpret_cast<uint32_t*>(ws);
+  ws += bound_bytes(d);
+  Operand x[4];
+  own_operands(a, x);
+  int rc;
+  if (tensor && d.dtype == D2C_F32) {
+    if ((rc = split_rows(a, pk.parts, ws, x, st))) return rc;
+    ws += staged_bytes(d, pk.parts);
+  }
+  a.part = reinterpret_cast<float*>(ws);
+  if ((rc = delta_rows(d.dtype, a, st))) return rc;
   if (tensor && d.dtype == D2C_F16 && (rc = tc_bounds(a, bounds, st))) return rc;
   a.splits = pk.splits;
-  if ((rc = tensor ? tc_bwd(d.dtype, a, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
+  if ((rc = tensor ? tc_bwd(d.dtype, a, x, pk.parts, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
   if (a.splits > 1) {
     const long long n = kv_rows(d) * d.dim;
     if ((rc = sum_parts(d.dtype, a.part, a.splits, n, a.gk, st))) return rc;
     if ((rc = sum_parts(d.dtype, a.part + a.splits * n, a.splits, n, a.gv, st))) return rc;
   }
   a.splits = pq.splits;
-  if ((rc = tensor ? tc_bwd(d.dtype, a, false, bounds, st) : exact_bwd_q(d.dtype, a, st))) return rc;
+  if ((rc = tensor ? tc_bwd(d.dtype, a, x, pq.parts, false, bounds, st) : exact_bwd_q(d.dtype, a, st))) return rc;
   if (a.splits > 1) return sum_parts(d.dtype, a.part, a.splits, q_rows(d) * d.dim, a.gq, st);
   return D2C_OK;
 }
@@ -186,9 +241,7 @@ size_t d2c_attention_fwd_workspace_bytes(const d2c_attention_desc* desc) {
   using namespace d2c;
   int sms = 0;
   if (attn::checked(desc) || device_sm_count(&sms)) return 0;
-  size_t n = 0;                       // whatever the pointers' alignment, and so the plan, turns out to be
-  for (int al = 0; al < 2; ++al) n = std::max(n, attn::fwd_bytes(*desc, attn::plan_fwd(*desc, al, sms)));
-  return n;
+  return attn::fwd_workspace(*desc, d2c_get_math_mode(), sms);
 }
 
 int d2c_attention_fwd(const d2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* key_lengths,
@@ -197,13 +250,14 @@ int d2c_attention_fwd(const d2c_attention_desc* desc, const void* q, const void*
   if (const int rc = take_device_status()) return rc;
   if (const int rc = attn::checked(desc)) return rc;
   if (!q || !k || !v || !o) return D2C_ERR_NULL;
-  if (!attn::ws_ok(workspace, workspace_bytes, d2c_attention_fwd_workspace_bytes(desc))) return D2C_ERR_WORKSPACE;
   int sms = 0;
   if (const int rc = device_sm_count(&sms)) return rc;
+  const int mode = d2c_get_math_mode();
+  if (!attn::ws_ok(workspace, workspace_bytes, attn::fwd_workspace(*desc, mode, sms))) return D2C_ERR_WORKSPACE;
   attn::Args a = attn::make_args(*desc, q, k, v, key_lengths);
   a.o = o; a.lse = reinterpret_cast<float*>(lse);
   prof_mark((cudaStream_t)stream, "attention");
-  const int rc = attn::run_fwd(*desc, a, workspace, sms, (cudaStream_t)stream);
+  const int rc = attn::run_fwd(*desc, a, mode, workspace, sms, (cudaStream_t)stream);
   prof_mark((cudaStream_t)stream, nullptr);
   return rc;
 }
@@ -212,7 +266,7 @@ size_t d2c_attention_bwd_workspace_bytes(const d2c_attention_desc* desc) {
   using namespace d2c;
   int sms = 0;
   if (attn::checked(desc) || device_sm_count(&sms)) return 0;
-  return attn::delta_bytes(*desc) + attn::bound_bytes(*desc) + attn::bwd_part_bytes(*desc, sms);
+  return attn::bwd_workspace(*desc, d2c_get_math_mode(), sms);
 }
 
 int d2c_attention_bwd(const d2c_attention_desc* desc, const void* grad_o, const void* q, const void* k, const void* v,
@@ -222,14 +276,15 @@ int d2c_attention_bwd(const d2c_attention_desc* desc, const void* grad_o, const 
   if (const int rc = take_device_status()) return rc;
   if (const int rc = attn::checked(desc)) return rc;
   if (!grad_o || !q || !k || !v || !o || !lse || !grad_q || !grad_k || !grad_v) return D2C_ERR_NULL;
-  if (!attn::ws_ok(workspace, workspace_bytes, d2c_attention_bwd_workspace_bytes(desc))) return D2C_ERR_WORKSPACE;
   int sms = 0;
   if (const int rc = device_sm_count(&sms)) return rc;
+  const int mode = d2c_get_math_mode();
+  if (!attn::ws_ok(workspace, workspace_bytes, attn::bwd_workspace(*desc, mode, sms))) return D2C_ERR_WORKSPACE;
   attn::Args a = attn::make_args(*desc, q, k, v, key_lengths);
   a.g = grad_o; a.o_in = o; a.lse = const_cast<float*>(reinterpret_cast<const float*>(lse));
   a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
   prof_mark((cudaStream_t)stream, "attention_bwd");
-  const int rc = attn::run_bwd(*desc, a, workspace, sms, (cudaStream_t)stream);
+  const int rc = attn::run_bwd(*desc, a, mode, workspace, sms, (cudaStream_t)stream);
   prof_mark((cudaStream_t)stream, nullptr);
   return rc;
 }

@@ -1,10 +1,12 @@
-// Cross attention on tensor cores (fp16 and bf16 tensors, head widths that are multiples of 8 up to 128).
+// Cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, and fp32 tensors staged as bf16
+// (split_rows: hi and lo parts, three products, for fp32 parity; or hi alone), up to 128 channels.
 //
 // Forward: a block has two tiles of 128 queries of a head and runs over tiles of 128 keys.  S_t = Q_t K^T lands in tensor memory;
 // four warps a tile (a thread a row) form p = 2^(s scale log2 e - m) with the running maximum and sum, and write it over S as the
 // 16-bit A operand of O_t += P_t V, whose accumulator stays in tensor memory too.  While one tile's warps work on their scores the
 // tensor cores work for the other tile.  The maximum that p refers to is raised, and O rescaled, only when the row's maximum has
 // outgrown it by 2^8: p is then at most 256, which both types hold, and most tiles skip the pass over O.
+// Operands in two parts of 128 channels: one tile of queries, shared memory has no room for more.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,6 +18,7 @@ namespace {
 
 struct TcParams {
   int B, Lq, Lk, Hq, Hkv, D;
+  int width;                     // channels of the operands: D, or D rounded up to 8 where they are staged
   float c;                       // scale * log2(e), not negative
   int splits, qblocks;
   void* o;
@@ -26,23 +29,25 @@ struct TcParams {
 
 constexpr int kFwdThreads = 384;                  // 8 softmax warps; MMA issuer, loader, two idle (see registers_up)
 constexpr int kFwdMmaWarp = 8, kFwdLoadWarp = 9;
-template <int DP>
-constexpr int kFwdStages = DP == 64 ? 6 : 4;
-template <int DP>
-constexpr int kFwdSmem = kTileBytes<DP> * (2 + kFwdStages<DP>) + 1024 + 256;
+template <int DP, int kParts>
+constexpr int kQTiles = DP * kParts > 128 ? 1 : 2;
+template <int DP, int kParts>
+constexpr int kFwdStages = DP * kParts == 64 ? 6 : (DP * kParts == 128 ? 4 : 2);
+template <int DP, int kParts>
+constexpr int kFwdSmem = kTileBytes<DP> * kParts * (kQTiles<DP, kParts> + kFwdStages<DP, kParts>) + 1024;
 
-template <typename T, int DP>
+template <typename T, typename Out, int DP, int kParts>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
               const __grid_constant__ TcParams p) {
-  constexpr int kStages = kFwdStages<DP>, kTB = kTileBytes<DP>;
+  constexpr int kStages = kFwdStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kQ = kQTiles<DP, kParts>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kStages + 8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t sq = base, ring = base + 2 * kTB;
+  const uint32_t sq = base, ring = base + kQ * kTB;
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8 * s; };
   auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
@@ -55,7 +60,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
   const int qb = (int)(id % p.qblocks); id /= p.qblocks;
   const int split = (int)(id % p.splits); id /= p.splits;
   const int head = (int)(id % p.Hq), b = (int)(id / p.Hq), hk = head / (p.Hq / p.Hkv);
-  const int q0 = qb * 2 * kRows, nt = p.Lq - q0 > kRows ? 2 : 1;
+  const int q0 = qb * kQ * kRows, nt = kQ == 2 && p.Lq - q0 > kRows ? 2 : 1;
   const int len = key_length(p.a, b), tiles = (len + kRows - 1) / kRows;
   int j0, j1;
   share(tiles, p.splits, split, j0, j1);
@@ -88,7 +93,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     if (n > 0) {
       if (lane == 0) {
         ptx::mbar_arrive_expect_tx(q_full, nt * kTB);
-        for (int t = 0; t < nt; ++t) tma_tile<DP>(sq + t * kTB, &mq, head, q0 + t * kRows, b, q_full);
+        for (int t = 0; t < nt; ++t) tma_tile<DP, kParts>(sq + t * kTB, &mq, head, q0 + t * kRows, b, p.B, q_full);
       }
       q_asked = true;
       for (; i < 2 * n; ++i) {
@@ -101,11 +106,11 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         const uint32_t bar = patch ? tail : full(s), dst = ring + s * kTB;
         if (lane == 0) {
           ptx::mbar_arrive_expect_tx(bar, kTB);
-          tma_tile<DP>(dst, value ? &mv : &mk, hk, j * kRows, b, bar);
+          tma_tile<DP, kParts>(dst, value ? &mv : &mk, hk, j * kRows, b, p.B, bar);
         }
         if (patch) {                              // the last tile: once per block
           drain(tail, 0);
-          clear_rows<DP>(dst, valid);
+          clear_rows<DP, kParts>(dst, valid);
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(full(s));
@@ -118,13 +123,13 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     }
   } else if (warp == kFwdMmaWarp) {
     if (lane == 0 && n > 0) {
-      const uint32_t id_s = idesc_of<T>(kRows, false), id_o = idesc_of<T>((p.D + 15) & ~15, true);
-      const int ksteps = (p.D + 15) >> 4;
+      const uint32_t id_s = idesc_of<T>(kRows, false), id_o = idesc_of<T>((p.width + 15) & ~15, true);
+      const int ksteps = (p.width + 15) >> 4;
       auto run = [&]() {
         if (!ptx::mbar_wait(q_full, 0, abort_flag) || !ptx::mbar_wait(full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
         for (int t = 0; t < nt; ++t) {
-          mma_scores(tS + 128 * t, sq + t * kTB, ring, id_s, ksteps);
+          mma_scores<DP, kParts>(tS + 128 * t, sq + t * kTB, ring, id_s, ksteps);
           ptx::umma_commit(s_full(t));
         }
         ptx::umma_commit(empty(0));
@@ -135,10 +140,10 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           for (int t = 0; t < nt; ++t) {
             if (!ptx::mbar_wait(p_ready(t), j & 1, abort_flag)) return;
             ptx::tc_fence_after();
-            mma_weigh(tO + DP * t, tS + 128 * t, ring + sv * kTB, id_o, j > 0);
+            mma_weigh<DP, kParts>(tO + DP * t, tS + 128 * t, 0, 64, ring + sv * kTB, id_o, j > 0);
             if (more) {
               if (t == 0 && !ptx::mbar_wait(full(sk), (ik / kStages) & 1, abort_flag)) return;
-              mma_scores(tS + 128 * t, sq + t * kTB, ring + sk * kTB, id_s, ksteps);
+              mma_scores<DP, kParts>(tS + 128 * t, sq + t * kTB, ring + sk * kTB, id_s, ksteps);
             }
             ptx::umma_commit(s_full(t));          // after the last tile: O_t is complete
           }
@@ -156,7 +161,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     const int t = warp >> 2, row = (warp & 3) * 32 + lane, qi = q0 + t * kRows + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tS + 128 * t + lanes, o_at = tO + DP * t + lanes;
-    const int dcols = (p.D + 15) & ~15;
+    const int dcols = (p.width + 15) & ~15;
     float m = 0.f, l = 0.f;
     bool ok = t < nt;
     for (int j = 0; ok && j < n; ++j) {
@@ -198,7 +203,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+        uint32_t w[32], rest[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int i0 = 64 * h + 2 * e;
@@ -207,8 +212,10 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           sum[e & 1] += x;
           sum[2 + (e & 1)] += y;
           w[e] = pack2<T>(x, y);
+          if constexpr (kParts == 2) rest[e] = pack2_rest(x, y, w[e]);
         }
         tmem_st_32x32(s_at + 32 * h, w);
+        if constexpr (kParts == 2) tmem_st_32x32(s_at + 64 + 32 * h, rest);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
@@ -242,14 +249,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           float f[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e + i]) * inv;
-          if (p.splits > 1) {
-            float* dst = p.part + ((long long)split * rows + out) * p.D + c0 + e;
-            *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
-          } else {
-            uint4 w = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + out * p.D + c0 + e) = w;
-          }
+          if (p.splits > 1) store8(p.part + ((long long)split * rows + out) * p.D + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
+          else store8(reinterpret_cast<Out*>(p.o) + out * p.D + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
         }
       }
       if (live) {
@@ -288,12 +289,64 @@ int encoder(EncodeTiled* out) {
   return D2C_OK;
 }
 
-template <typename T, int DP>
-int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, unsigned grid, cudaStream_t st) {
-  if (const int rc = allow_dynamic_smem<fwd_tc_kernel<T, DP>>(kFwdSmem<DP>)) return rc;
-  fwd_tc_kernel<T, DP><<<grid, kFwdThreads, kFwdSmem<DP>, st>>>(mq, mk, mv, p);
+template <typename T, typename Out, int DP, int kParts>
+int launch_fwd(const CUtensorMap (&m)[3], TcParams p, cudaStream_t st) {
+  p.qblocks = (p.Lq + kQTiles<DP, kParts> * kRows - 1) / (kQTiles<DP, kParts> * kRows);
+  const long long blocks = (long long)p.qblocks * p.splits * p.Hq * p.B;
+  if (blocks > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
+  constexpr int smem = kFwdSmem<DP, kParts>;
+  if (const int rc = allow_dynamic_smem<fwd_tc_kernel<T, Out, DP, kParts>>(smem)) return rc;
+  fwd_tc_kernel<T, Out, DP, kParts><<<(unsigned)blocks, kFwdThreads, smem, st>>>(m[0], m[1], m[2], p);
   D2C_LAUNCH_CHECK();
   return D2C_OK;
+}
+template <typename T, typename Out, int kParts>
+int fwd_by_width(const CUtensorMap (&m)[3], const TcParams& p, cudaStream_t st) {
+  return p.width <= 64 ? launch_fwd<T, Out, 64, kParts>(m, p, st) : launch_fwd<T, Out, 128, kParts>(m, p, st);
+}
+
+// x [B, L, H, D] fp32 with any strides -> [parts][B, L, H, width] bf16: hi = bf16(x), lo = bf16(x - hi); zeros from D on.
+// Up to four tensors in one launch.  A thread writes 8 channels.
+struct SplitArgs {
+  const float* x[4];
+  __nv_bfloat16* out[4];
+  long long s[4][3];
+  int L[4], H[4];
+  int B, D, width, parts;
+};
+__global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__ SplitArgs a) {
+  const int which = blockIdx.y, L = a.L[which], H = a.H[which], per = a.width / 8;
+  const long long n = (long long)a.B * L * H * per;
+  const float* x = a.x[which];
+  uint4* out = reinterpret_cast<uint4*>(a.out[which]);
+  const bool wide = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && a.s[which][0] % 4 == 0 && a.s[which][1] % 4 == 0 &&
+                    a.s[which][2] % 4 == 0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int c = (int)(i % per) * 8;
+    long long r = i / per;
+    const int h = (int)(r % H);
+    r /= H;
+    const int l = (int)(r % L);
+    const float* src = x + r / L * a.s[which][0] + l * a.s[which][1] + h * a.s[which][2] + c;
+    float f[8];
+    if (wide && c + 8 <= a.D) {
+      const float4 p = *reinterpret_cast<const float4*>(src), q = *reinterpret_cast<const float4*>(src + 4);
+      f[0] = p.x; f[1] = p.y; f[2] = p.z; f[3] = p.w; f[4] = q.x; f[5] = q.y; f[6] = q.z; f[7] = q.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = c + e < a.D ? src[e] : 0.f;
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi[e] = ptx::pack_bf16x2(f[2 * e], f[2 * e + 1]);
+      const float x0 = ptx::bf16_lo(hi[e]), x1 = ptx::bf16_hi(hi[e]);
+      // infinity has no rest
+      lo[e] = ptx::pack_bf16x2(fabsf(x0) == INFINITY ? 0.f : f[2 * e] - x0, fabsf(x1) == INFINITY ? 0.f : f[2 * e + 1] - x1);
+    }
+    out[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (a.parts == 2) out[n + i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
 }
 
 }  // namespace
@@ -307,40 +360,66 @@ int status_pointer(int** out) {
   return rc ? rc : check_cuda(back);
 }
 
-// [clips, tokens, heads, D] with element strides s (clip, token, head); a dimension of one element has no stride.
-int tile_map(CUtensorMap* map, int dtype, const void* p, int D, int heads, int tokens, int clips, const long long (&s)[3]) {
+// [clips, tokens, heads, D] 16-bit; a dimension of one element has no stride.
+int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips) {
   EncodeTiled f;
   if (const int rc = encoder(&f)) return rc;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)clips};
   auto bytes = [&](long long st, int n) { return (cuuint64_t)(n == 1 ? 256 : 2 * st); };
-  const cuuint64_t strides[3] = {bytes(s[2], heads), bytes(s[1], tokens), bytes(s[0], clips)};
+  const cuuint64_t strides[3] = {bytes(o.s[2], heads), bytes(o.s[1], tokens), bytes(o.s[0], clips)};
   const cuuint32_t box[4] = {64, 1, kRows, 1}, ones[4] = {1, 1, 1, 1};
-  const CUresult rc = f(map, dtype == D2C_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                        const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult rc = f(map, dtype == D2C_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                        const_cast<void*>(o.p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? D2C_OK : check_cuda(cudaErrorInvalidValue);
 }
 
-int tc_fwd(int dtype, const Args& a, cudaStream_t st) {
-  CUtensorMap mq, mk, mv;
-  int rc;
-  if ((rc = tile_map(&mq, dtype, a.q, a.D, a.Hq, a.Lq, a.B, a.qs))) return rc;
-  if ((rc = tile_map(&mk, dtype, a.k, a.D, a.Hkv, a.Lk, a.B, a.ks))) return rc;
-  if ((rc = tile_map(&mv, dtype, a.v, a.D, a.Hkv, a.Lk, a.B, a.vs))) return rc;
+size_t split_bytes(int B, int L, int H, int D, int parts) {
+  return align_up((size_t)2 * parts * B * L * H * ((D + 7) / 8 * 8), 256);
+}
+
+// Stages q, k, v and, if it is there, g; o[0..3] become the staged operands.
+int split_rows(const Args& a, int parts, void* workspace, Operand (&o)[4], cudaStream_t st) {
+  SplitArgs s{};
+  s.B = a.B; s.D = a.D; s.width = (a.D + 7) / 8 * 8; s.parts = parts;
+  const void* src[4] = {a.q, a.k, a.v, a.g};
+  const long long* strides[4] = {a.qs, a.ks, a.vs, a.gs};
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  const int n = a.g ? 4 : 3;
+  long long most = 0;
+  for (int i = 0; i < n; ++i) {
+    s.L[i] = i == 0 || i == 3 ? a.Lq : a.Lk;
+    s.H[i] = i == 0 || i == 3 ? a.Hq : a.Hkv;
+    s.x[i] = reinterpret_cast<const float*>(src[i]);
+    s.out[i] = reinterpret_cast<__nv_bfloat16*>(ws);
+    for (int d = 0; d < 3; ++d) s.s[i][d] = strides[i][d];
+    o[i] = {ws, {(long long)s.L[i] * s.H[i] * s.width, (long long)s.H[i] * s.width, s.width}};
+    ws += split_bytes(a.B, s.L[i], s.H[i], a.D, parts);
+    most = std::max(most, (long long)a.B * s.L[i] * s.H[i] * (s.width / 8));
+  }
+  const unsigned blocks = (unsigned)std::min<long long>((most + 255) / 256, 148 * 8);
+  split_rows_kernel<<<dim3(blocks, n), 256, 0, st>>>(s);
+  D2C_LAUNCH_CHECK();
+  return D2C_OK;
+}
+
+int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, cudaStream_t st) {
   TcParams p{};
   p.B = a.B; p.Lq = a.Lq; p.Lk = a.Lk; p.Hq = a.Hq; p.Hkv = a.Hkv; p.D = a.D;
+  p.width = (a.D + 7) / 8 * 8;
+  CUtensorMap m[3];
+  int rc;
+  if ((rc = tile_map(&m[0], x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
+  if ((rc = tile_map(&m[1], x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
+  if ((rc = tile_map(&m[2], x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
   p.c = a.scale * kLog2e;
   p.splits = a.splits;
-  p.qblocks = (a.Lq + 2 * kRows - 1) / (2 * kRows);
   p.o = a.o; p.lse = a.lse; p.part = a.part; p.part_lse = a.part_lse;
   p.a = a;
   if ((rc = status_pointer(&p.status))) return rc;
-  const long long blocks = (long long)p.qblocks * p.splits * p.Hq * p.B;
-  if (blocks > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
-  const unsigned grid = (unsigned)blocks;
-  if (dtype == D2C_BF16)
-    return a.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(mq, mk, mv, p, grid, st) : launch_fwd<__nv_bfloat16, 128>(mq, mk, mv, p, grid, st);
-  return a.D <= 64 ? launch_fwd<__half, 64>(mq, mk, mv, p, grid, st) : launch_fwd<__half, 128>(mq, mk, mv, p, grid, st);
+  if (dtype == D2C_BF16) return fwd_by_width<__nv_bfloat16, __nv_bfloat16, 1>(m, p, st);
+  if (dtype == D2C_F16) return fwd_by_width<__half, __half, 1>(m, p, st);
+  return parts == 2 ? fwd_by_width<__nv_bfloat16, float, 2>(m, p, st) : fwd_by_width<__nv_bfloat16, float, 1>(m, p, st);
 }
 
 }  // namespace attn

@@ -1,4 +1,5 @@
-// Gradients of cross attention on tensor cores (fp16 and bf16 tensors, head widths that are multiples of 8 up to 128).
+// Gradients of cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, up to 128 channels; fp32
+// tensors staged as bf16 (attention_sm100.cu: split_rows), in two parts up to 64 channels, in one up to 128.
 //
 // One kernel, two uses.  A block keeps a tile of 128 rows X (X1, X2) and runs over tiles of 128 rows Y (Y1, Y2):
 //   S = X1 Y1^T,  dP = X2 Y2^T,  P = 2^(S scale log2 e - lse),  dS = P (dP - delta)
@@ -23,6 +24,7 @@ namespace {
 
 struct BwdParams {
   int B, Lq, Lk, Hq, Hkv, D;
+  int width;                     // channels of the operands
   float c, scale;
   int splits, blocks_x;          // tiles of X per head
   const float *lse, *delta;
@@ -35,16 +37,16 @@ struct BwdParams {
 
 constexpr int kThreads = 384;                     // 8 working warps; MMA issuer, loader, two idle (see registers_up)
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
-template <int DP>
-constexpr int kStages = DP == 64 ? 8 : 4;
-template <int DP>
-constexpr int kSmem = kTileBytes<DP> * (2 + kStages<DP>) + 1024;
+template <int DP, int kParts>
+constexpr int kStages = DP * kParts == 64 ? 8 : 4;
+template <int DP, int kParts>
+constexpr int kSmem = kTileBytes<DP> * kParts * (2 + kStages<DP, kParts>) + 1024;
 
-template <typename T, int DP, bool kKeys>
+template <typename T, typename Out, int DP, int kParts, bool kKeys>
 __global__ void __launch_bounds__(kThreads, 1)
 bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2, const __grid_constant__ CUtensorMap my1,
               const __grid_constant__ CUtensorMap my2, const __grid_constant__ BwdParams p) {
-  constexpr int kSt = kStages<DP>, kTB = kTileBytes<DP>;
+  constexpr int kSt = kStages<DP, kParts>, kTB = kTileBytes<DP> * kParts;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
   extern __shared__ uint8_t raw[];
@@ -105,8 +107,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       if (n > 0) {
         if (lane == 0) {
           ptx::mbar_arrive_expect_tx(x_full, 2 * kTB);
-          tma_tile<DP>(sx, &mx1, head, x0, b, x_full);
-          tma_tile<DP>(sx + kTB, &mx2, head, x0, b, x_full);
+          tma_tile<DP, kParts>(sx, &mx1, head, x0, b, p.B, x_full);
+          tma_tile<DP, kParts>(sx + kTB, &mx2, head, x0, b, p.B, x_full);
         }
         for (; i < 2 * n; ++i) {
           const int s = i % kSt, y = i0 + (i >> 1), h = y_head(y), r0 = y_row(y);
@@ -130,11 +132,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           const uint32_t bar = patch ? tail : full(s), dst = ring + s * kTB;
           if (lane == 0) {
             ptx::mbar_arrive_expect_tx(bar, kTB);
-            tma_tile<DP>(dst, second ? &my2 : &my1, h, r0, b, bar);
+            tma_tile<DP, kParts>(dst, second ? &my2 : &my1, h, r0, b, p.B, bar);
           }
           if (patch) {                            // the last tile: once per block
             drain(tail, 0);
-            clear_rows<DP>(dst, len - r0);
+            clear_rows<DP, kParts>(dst, len - r0);
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(full(s));
@@ -146,22 +148,20 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         }
       }
     } else if (warp == kMmaWarp && lane == 0 && n > 0) {
-      const uint32_t id_s = idesc_of<T>(kRows, false), id_a = idesc_of<T>((p.D + 15) & ~15, true);
-      const int ksteps = (p.D + 15) >> 4;
+      const uint32_t id_s = idesc_of<T>(kRows, false), id_a = idesc_of<T>((p.width + 15) & ~15, true);
+      const int ksteps = (p.width + 15) >> 4;
       auto slot = [&](int i) { return ring + (i % kSt) * kTB; };
       auto there = [&](int i) { return ptx::mbar_wait(full(i % kSt), (i / kSt) & 1, abort_flag); };
-      auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {
-#pragma unroll
-        for (int k = 0; k < kRows / 16; ++k)      // each half of the columns has its 16-bit values at its own start
-          umma_ts(acc, w + 8 * k + (k >= 4 ? 32 : 0), ptx::umma_desc_mnmajor_sw128(y + 2048 * k, kHalfBytes, 1024), id_a, more || k > 0);
+      auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {   // each half of the columns has its parts at its own start
+        mma_weigh<DP, kParts>(acc, w, 32, 32, y, id_a, more);
       };
       auto run = [&]() {
         if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
         ptx::tc_fence_after();
-        mma_scores(tS, sx, slot(0), id_s, ksteps);
+        mma_scores<DP, kParts>(tS, sx, slot(0), id_s, ksteps);
         ptx::umma_commit(s_full);
         if (!there(1)) return;
-        mma_scores(tD, sx + kTB, slot(1), id_s, ksteps);
+        mma_scores<DP, kParts>(tD, sx + kTB, slot(1), id_s, ksteps);
         ptx::umma_commit(dp_full);
         if (!kKeys) ptx::umma_commit(empty(1));
         for (int i = 0; i < n; ++i) {
@@ -175,7 +175,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           if (more) {
             if (!there(y1 + 2)) return;
-            mma_scores(tS, sx, slot(y1 + 2), id_s, ksteps);
+            mma_scores<DP, kParts>(tS, sx, slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
           }
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
@@ -184,7 +184,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           ptx::umma_commit(empty(y1 % kSt));
           if (more) {
             if (!there(y2 + 2)) return;
-            mma_scores(tD, sx + kTB, slot(y2 + 2), id_s, ksteps);
+            mma_scores<DP, kParts>(tD, sx + kTB, slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
             if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
           }
@@ -246,11 +246,15 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
         }
       if constexpr (kKeys) {
-        uint32_t w[32];
+        uint32_t w[32], rest[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          w[e] = pack2<T>(__uint_as_float(s[e >> 4][2 * e & 31]), __uint_as_float(s[e >> 4][(2 * e & 31) + 1]));
+        for (int e = 0; e < 32; ++e) {
+          const float x = __uint_as_float(s[e >> 4][2 * e & 31]), y = __uint_as_float(s[e >> 4][(2 * e & 31) + 1]);
+          w[e] = pack2<T>(x, y);
+          if constexpr (kParts == 2) rest[e] = pack2_rest(x, y, w[e]);
+        }
         tmem_st_32x32(s_at, w);
+        if constexpr (kParts == 2) tmem_st_32x32(s_at + 32, rest);
         tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
@@ -258,7 +262,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       }
       if (!warp_wait(dp_full, i & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
-      uint32_t w[32];
+      uint32_t w[32], rest[kParts == 2 ? 32 : 1];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint32_t d[32];
@@ -278,9 +282,14 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
           w[16 * k + e / 2 + 1] = pack2<T>(v[2], v[3]);
+          if constexpr (kParts == 2) {
+            rest[16 * k + e / 2] = pack2_rest(v[0], v[1], w[16 * k + e / 2]);
+            rest[16 * k + e / 2 + 1] = pack2_rest(v[2], v[3], w[16 * k + e / 2 + 1]);
+          }
         }
       }
       tmem_st_32x32(d_at, w);
+      if constexpr (kParts == 2) tmem_st_32x32(d_at + 32, rest);
       tmem_st_wait();
       ptx::tc_fence_before();
       __syncwarp();
@@ -297,7 +306,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       const bool first = kKeys && half == 0;
       const float mul = first ? exp2f(-kUp) : p.scale * ds_back;
       const uint32_t acc = (first ? tA1 : tA2) + lanes;
-      T* dst = reinterpret_cast<T*>(first ? p.g1 : p.g2) + out * p.D;
+      Out* dst = reinterpret_cast<Out*>(first ? p.g1 : p.g2) + out * p.D;
       float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
       const int c_end = kKeys ? p.D : min(p.D, (half + 1) * (DP / 2));
       for (int c0 = kKeys ? 0 : half * (DP / 2); c0 < c_end; c0 += 32) {
@@ -316,12 +325,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           float f[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(r[e + u]) * mul;
-          if (part) {
-            *reinterpret_cast<float4*>(part + c0 + e) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4*>(part + c0 + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
-          } else {
-            *reinterpret_cast<uint4*>(dst + c0 + e) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-          }
+          if (part) store8(part + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
+          else store8(dst + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
         }
       }
     }
@@ -359,19 +364,23 @@ __global__ void __launch_bounds__(256) row_bound_kernel(Args a, const __half* x,
   if (lane == 0 && len > 0) atomicMax(out + 2 * ((long long)b * a.Hkv + hk), bad ? 0x7fffffffu : __float_as_uint(most));
 }
 
-template <typename T, int DP, bool kKeys>
+template <typename T, typename Out, int DP, int kParts, bool kKeys>
 int launch(const CUtensorMap (&m)[4], const BwdParams& p, cudaStream_t st) {
   const long long blocks = (long long)p.blocks_x * p.splits * (kKeys ? p.Hkv : p.Hq) * p.B;
   if (blocks > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
-  if (const int rc = allow_dynamic_smem<bwd_tc_kernel<T, DP, kKeys>>(kSmem<DP>)) return rc;
-  bwd_tc_kernel<T, DP, kKeys><<<(unsigned)blocks, kThreads, kSmem<DP>, st>>>(m[0], m[1], m[2], m[3], p);
+  constexpr int smem = kSmem<DP, kParts>;
+  if (const int rc = allow_dynamic_smem<bwd_tc_kernel<T, Out, DP, kParts, kKeys>>(smem)) return rc;
+  bwd_tc_kernel<T, Out, DP, kParts, kKeys><<<(unsigned)blocks, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], p);
   D2C_LAUNCH_CHECK();
   return D2C_OK;
 }
-template <typename T>
+template <typename T, typename Out, int DP, int kParts>
+int by_side(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStream_t st) {
+  return keys ? launch<T, Out, DP, kParts, true>(m, p, st) : launch<T, Out, DP, kParts, false>(m, p, st);
+}
+template <typename T, typename Out>
 int by_width(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStream_t st) {
-  if (keys) return p.D <= 64 ? launch<T, 64, true>(m, p, st) : launch<T, 128, true>(m, p, st);
-  return p.D <= 64 ? launch<T, 64, false>(m, p, st) : launch<T, 128, false>(m, p, st);
+  return p.width <= 64 ? by_side<T, Out, 64, 1>(m, p, keys, st) : by_side<T, Out, 128, 1>(m, p, keys, st);
 }
 
 }  // namespace
@@ -390,16 +399,17 @@ int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st) {
   return D2C_OK;
 }
 
-int tc_bwd(int dtype, const Args& a, bool keys, const uint32_t* bounds, cudaStream_t st) {
-  CUtensorMap q, k, v, g;
-  int rc;
-  if ((rc = tile_map(&q, dtype, a.q, a.D, a.Hq, a.Lq, a.B, a.qs))) return rc;
-  if ((rc = tile_map(&k, dtype, a.k, a.D, a.Hkv, a.Lk, a.B, a.ks))) return rc;
-  if ((rc = tile_map(&v, dtype, a.v, a.D, a.Hkv, a.Lk, a.B, a.vs))) return rc;
-  if ((rc = tile_map(&g, dtype, a.g, a.D, a.Hq, a.Lq, a.B, a.gs))) return rc;
-  const CUtensorMap maps[4] = {keys ? k : q, keys ? v : g, keys ? q : k, keys ? g : v};
+int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys, const uint32_t* bounds, cudaStream_t st) {
   BwdParams p{};
   p.B = a.B; p.Lq = a.Lq; p.Lk = a.Lk; p.Hq = a.Hq; p.Hkv = a.Hkv; p.D = a.D;
+  p.width = (a.D + 7) / 8 * 8;
+  CUtensorMap q, k, v, g;
+  int rc;
+  if ((rc = tile_map(&q, x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
+  if ((rc = tile_map(&k, x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
+  if ((rc = tile_map(&v, x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
+  if ((rc = tile_map(&g, x[3], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
+  const CUtensorMap maps[4] = {keys ? k : q, keys ? v : g, keys ? q : k, keys ? g : v};
   p.c = a.scale * kLog2e; p.scale = a.scale;
   p.splits = a.splits;
   p.blocks_x = ((keys ? a.Lk : a.Lq) + kRows - 1) / kRows;
@@ -408,7 +418,9 @@ int tc_bwd(int dtype, const Args& a, bool keys, const uint32_t* bounds, cudaStre
   p.part = a.part;
   p.a = a;
   if ((rc = status_pointer(&p.status))) return rc;
-  return dtype == D2C_BF16 ? by_width<__nv_bfloat16>(maps, p, keys, st) : by_width<__half>(maps, p, keys, st);
+  if (dtype == D2C_BF16) return by_width<__nv_bfloat16, __nv_bfloat16>(maps, p, keys, st);
+  if (dtype == D2C_F16) return by_width<__half, __half>(maps, p, keys, st);
+  return parts == 2 ? by_side<__nv_bfloat16, float, 64, 2>(maps, p, keys, st) : by_width<__nv_bfloat16, float>(maps, p, keys, st);
 }
 
 }  // namespace attn

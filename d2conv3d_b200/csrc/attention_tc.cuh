@@ -21,25 +21,31 @@ constexpr int kHalfBytes = kRows * 128;          // 64 channels of it
 template <int DP>
 constexpr int kTileBytes = kHalfBytes * (DP / 64);
 
+// fp32 tensors are staged as bf16: `kParts` = 2 operand tiles behind one another, hi = bf16(x) and lo = bf16(x - hi), whose products
+// hi hi + lo hi + hi lo keep 16 bits of each factor; or hi alone.  The parts are the outer half of a tensor map's clips.
+//
 // One box of 64 channels x 1 head x 128 tokens x 1 clip; what lies outside the tensor arrives as zeros.  x is 0 or 64.
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, int clip, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(token), "r"(clip), "r"(bar)
                : "memory");
 }
-template <int DP>
-__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int head, int token, int clip, uint32_t bar) {
+template <int DP, int kParts>
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int head, int token, int clip, int clips, uint32_t bar) {
 #pragma unroll
-  for (int h = 0; h < DP / 64; ++h) tma_box(dst + h * kHalfBytes, map, h * 64, head, token, clip, bar);
+  for (int part = 0; part < kParts; ++part)
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h)
+      tma_box(dst + part * kTileBytes<DP> + h * kHalfBytes, map, h * 64, head, token, part * clips + clip, bar);
 }
 
 // Zeroes rows [from, 128) of a tile (one warp).
-template <int DP>
+template <int DP, int kParts>
 __device__ __forceinline__ void clear_rows(uint32_t tile, int from) {
   const int lane = threadIdx.x & 31;
   for (int i = from * 8 + lane; i < kRows * 8; i += 32) {        // 16-byte pieces: the swizzle stays inside a row
 #pragma unroll
-    for (int h = 0; h < DP / 64; ++h) ptx::sts_v4(tile + h * kHalfBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
+    for (int h = 0; h < kParts * DP / 64; ++h) ptx::sts_v4(tile + h * kHalfBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
   }
 }
 
@@ -75,17 +81,29 @@ __device__ __forceinline__ uint32_t idesc_of(int N, bool b_mn) {
 }
 
 // D (128 x 128) = X Y^T over the channels, both K-major; ksteps = channels / 16 rounded up (zero-filled above D).
+template <int DP, int kParts>
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ksteps) {
-  for (int k = 0; k < ksteps; ++k) {
-    const uint32_t at = (uint32_t)((k >> 2) * kHalfBytes + (k & 3) * 32);
-    ptx::umma_bf16(d_tmem, ptx::umma_desc_kmajor_sw128(x + at), ptx::umma_desc_kmajor_sw128(y + at), idesc, k > 0);
+#pragma unroll
+  for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
+    const uint32_t xp = x + (pass == 1 ? kTileBytes<DP> : 0), yp = y + (pass == 2 ? kTileBytes<DP> : 0);
+    for (int k = 0; k < ksteps; ++k) {
+      const uint32_t at = (uint32_t)((k >> 2) * kHalfBytes + (k & 3) * 32);
+      ptx::umma_bf16(d_tmem, ptx::umma_desc_kmajor_sw128(xp + at), ptx::umma_desc_kmajor_sw128(yp + at), idesc, pass > 0 || k > 0);
+    }
   }
 }
-// D (128 x N) (+)= A Y, A 128 x 128 in tensor memory, Y's 128 rows the reduction.
-__device__ __forceinline__ void mma_weigh(uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, uint32_t accumulate) {
+// D (128 x N) (+)= A Y, A 128 x 128 in tensor memory, Y's 128 rows the reduction.  A's second 64 columns start `jump` 32-bit columns
+// behind where the first would go on; its lo part lies `lo` columns further.
+template <int DP, int kParts>
+__device__ __forceinline__ void mma_weigh(uint32_t d_tmem, uint32_t a_tmem, int jump, int lo, uint32_t y, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int k = 0; k < kRows / 16; ++k)
-    umma_ts(d_tmem, a_tmem + 8 * k, ptx::umma_desc_mnmajor_sw128(y + 2048 * k, kHalfBytes, 1024), idesc, accumulate | (k > 0));
+  for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
+    const uint32_t ap = a_tmem + (pass == 1 ? lo : 0), yp = y + (pass == 2 ? kTileBytes<DP> : 0);
+#pragma unroll
+    for (int k = 0; k < kRows / 16; ++k)
+      umma_ts(d_tmem, ap + 8 * k + (k >= 4 ? jump : 0), ptx::umma_desc_mnmajor_sw128(yp + 2048 * k, kHalfBytes, 1024), idesc,
+              accumulate || pass > 0 || k > 0);
+  }
 }
 
 template <typename T>
@@ -96,6 +114,26 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+  }
+}
+// What bf16 rounding left over of two values, rounded again.
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t packed) {
+  return ptx::pack_bf16x2(lo - ptx::bf16_lo(packed), hi - ptx::bf16_hi(packed));
+}
+// Eight neighbouring results of a row, the first `n` of them (16-byte stores where all are there; dst is then 16-byte aligned).
+template <typename Out>
+__device__ __forceinline__ void store8(Out* dst, const float (&f)[8], int n, bool wide) {
+  if (wide && n >= 8) {
+    if constexpr (sizeof(Out) == 4) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<Out>(f[0], f[1]), pack2<Out>(f[2], f[3]), pack2<Out>(f[4], f[5]), pack2<Out>(f[6], f[7]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) dst[i] = from_f32<Out>(f[i]);
   }
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -131,7 +169,7 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
 
 // attention_sm100.cu: host helpers
 int status_pointer(int** out);
-int tile_map(CUtensorMap* map, int dtype, const void* p, int D, int heads, int tokens, int clips, const long long (&s)[3]);
+int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips);
 
 }  // namespace attn
 }  // namespace d2c

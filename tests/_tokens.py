@@ -81,9 +81,10 @@ def rotary_oracle(x, positions, axis_dims, base, interleaved, inverse=False):
     return out, size * (2 * math.pi * U / 2 + 5 * U + far * 2 * math.pi * 2.0 ** -50)
 
 
-def attention_oracle(q, k, v, g, lengths, scale, p_half):
+def attention_oracle(q, k, v, g, lengths, scale, p_half, product=0.0):
     """{o, gq, gk, gv: (value, bound before the last rounding)}.  p_half: half a step of the type that probabilities and score
-    gradients are rounded to before they are multiplied (u where they stay in fp32)."""
+    gradients are rounded to before they are multiplied (u where they stay in fp32).  product: what the operands' rounding
+    takes from a product, relative to its size (fp32 tensors whose products run on tensor cores)."""
     dtype = q.dtype
     q, k, v, g = (t.detach().double().cpu() for t in (q, k, v, g))
     B, Lq, Hq, D = q.shape
@@ -102,22 +103,22 @@ def attention_oracle(q, k, v, g, lengths, scale, p_half):
             p = torch.softmax(s, -1)
             o = p @ V
             # a score: D products added in fp32 (tensor cores may truncate: twice u), scaled; its exponential and the row's sum
-            ds = (2 * D + 8) * U * (Q.abs() @ K.abs().T) * abs(scale)
+            ds = ((2 * D + 8) * U + product) * (Q.abs() @ K.abs().T) * abs(scale)
             rel = 2 * ds.max(-1, keepdim=True).values + (s.abs().max() * 4 + 16) * U + (m / 64 + 64) * 2 * U
             chain = (m / 8 + 64) * 2 * U                                 # additions along the keys
             val["o"][b, :, h] = o
-            err["o"][b, :, h] = (p * (rel + 2 * p_half + chain)) @ V.abs() + 4 * U * o.abs()
+            err["o"][b, :, h] = (p * (rel + 2 * p_half + product + chain)) @ V.abs() + 4 * U * o.abs()
             dp = G @ V.T
             delta = (G * o).sum(-1, keepdim=True)
             e_delta = (G.abs() * (err["o"][b, :, h] + half(dtype) * o.abs())).sum(-1, keepdim=True) + 2 * D * U * (G * o).abs().sum(-1, keepdim=True)
-            e_dp = (2 * D + 4) * U * (G.abs() @ V.abs().T)
+            e_dp = ((2 * D + 4) * U + product) * (G.abs() @ V.abs().T)
             d = p * (dp - delta)
             e_d = p * ((dp - delta).abs() * (rel + 2 * p_half + 4 * U) + (e_dp + e_delta) * (1 + rel + p_half))
             rows = (Lq / 8 + 64) * 2 * U * n                             # additions along the queries
             val["gq"][b, :, h] = d @ K * scale
-            err["gq"][b, :, h] = ((e_d + d.abs() * chain) @ K.abs()) * abs(scale)
+            err["gq"][b, :, h] = ((e_d + d.abs() * (chain + product)) @ K.abs()) * abs(scale)
             val["gk"][b, :m, h // n] += d.T @ Q * scale
-            err["gk"][b, :m, h // n] += ((e_d + d.abs() * rows).T @ Q.abs()) * abs(scale)
+            err["gk"][b, :m, h // n] += ((e_d + d.abs() * (rows + product)).T @ Q.abs()) * abs(scale)
             val["gv"][b, :m, h // n] += p.T @ G
-            err["gv"][b, :m, h // n] += (p * (rel + 2 * p_half + rows)).T @ G.abs()
+            err["gv"][b, :m, h // n] += (p * (rel + 2 * p_half + product + rows)).T @ G.abs()
     return {key: (val[key], err[key]) for key in val}

@@ -22,16 +22,28 @@ def run(q, k, v, g, lengths=None, scale=None):
     return (o.detach(),) + torch.autograd.grad(o, leaves, g)
 
 
+# fp32 by math mode: (half a step of the probabilities, what the operands' rounding takes from a product).  "auto": hi + lo bf16
+# parts keep a factor to 2^-18 (half a step of the second part, 2^-9 of at most 2^-9), and lo lo, at most 2^-18, is left out.
+# "bf16": each factor to 2^-9.
+FP32_MODES = {"fp32": (U, 0.0), "auto": (2.0 ** -18, 3 * 2.0 ** -18), "bf16": (2.0 ** -9, 2.0 ** -8 + 2.0 ** -18)}
+
+
 def check(q, k, v, g, lengths=None, scale=None):
-    got = run(q, k, v, g, lengths, scale)
-    with torch.no_grad():
-        served = d2c.cross_attention(q, k, v, lengths, scale)
-    p_half = U if q.dtype == torch.float32 else half(q.dtype)
-    want = attention_oracle(q, k, v, g, lengths, 1 / math.sqrt(q.shape[-1]) if scale is None else scale, p_half)
-    for name, t in zip(("o", "gq", "gk", "gv"), got):
-        assert t.dtype == q.dtype
-        assert_within(t, want[name][0], rounded(*want[name], q.dtype), name)
-    assert torch.equal(served, got[0])
+    before = d2c.get_math_mode()
+    for mode in FP32_MODES if q.dtype == torch.float32 else ("auto",):
+        p_half, product = FP32_MODES[mode] if q.dtype == torch.float32 else (half(q.dtype), 0.0)
+        try:
+            d2c.set_math_mode(mode)
+            got = run(q, k, v, g, lengths, scale)
+            with torch.no_grad():
+                served = d2c.cross_attention(q, k, v, lengths, scale)
+        finally:
+            d2c.set_math_mode(before)
+        want = attention_oracle(q, k, v, g, lengths, 1 / math.sqrt(q.shape[-1]) if scale is None else scale, p_half, product)
+        for name, t in zip(("o", "gq", "gk", "gv"), got):
+            assert t.dtype == q.dtype
+            assert_within(t, want[name][0], rounded(*want[name], q.dtype), f"{name} {mode}")
+        assert torch.equal(served, got[0])
 
 
 # lengths from one to several tiles, on both sides of the tiles' edges
