@@ -53,12 +53,13 @@ struct Operand {
   const void* p;
   long long s[3];                        // clip, token, head
 };
-// attention_sm100.cu.  fp32: operands staged by split_rows, in `parts` parts
+// attention_sm100.cu.  fp32: operands staged by split_rows, in `parts` parts.  bounds [4][B, Hkv]: by largest_sizes, for two parts and for
+// the gradients of fp16 tensors
+int largest_sizes(int dtype, const Args& a, bool values_only, uint32_t* bounds, cudaStream_t st);
 size_t split_bytes(int B, int L, int H, int D, int parts);
-int split_rows(const Args& a, int parts, void* workspace, Operand (&o)[4], cudaStream_t st);      // q, k, v, and g if there is one
-int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, cudaStream_t st);
+int split_rows(const Args& a, int parts, uint32_t* bounds, void* workspace, Operand (&o)[4], cudaStream_t st);   // q, k, v, and g if there is one
+int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, const uint32_t* bounds, cudaStream_t st);
 // attention_sm100_bwd.cu
-int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st);              // fp16: [B, Hkv][2], for tc_bwd
 int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys, const uint32_t* bounds, cudaStream_t st);
 
 }  // namespace attn

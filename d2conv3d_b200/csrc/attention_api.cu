@@ -71,9 +71,9 @@ int tensor_parts(const d2c_attention_desc& d, int mode, bool aligned, bool backw
 }
 
 // The tensor cores add into their accumulator with truncation: a chain of n accumulating products loses about n * 2^-27 of the
-// result.  With two parts (24 products a tile) a share ends after 12 tiles, 2e-6, and the shares are added in fp32 -- unless their
-// results would take more than 2 GB.
-constexpr int kChainTiles = 12;
+// result.  With two parts (24 products a tile) a share ends after 8 tiles, 1.5e-6, and the shares are added in fp32 -- unless their
+// results would take more than 2 GB.  (Measured at 1215 x 3240, 64 channels: gradients 5e-6 off with 12 tiles.)
+constexpr int kChainTiles = 8;
 int fewest_shares(int parts, int steps, long long rows, int dim) {
   if (parts != 2) return 1;
   return (int)std::min<long long>(ceil_div(steps, kChainTiles), std::max(1LL, (2LL << 30) / (4 * rows * dim)));
@@ -108,10 +108,11 @@ Plan plan_bwd(const d2c_attention_desc& d, int mode, bool keys, bool aligned, in
   return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), sms);
 }
 
+size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 4 * d.batch * d.kv_heads, 256); }
 size_t fwd_bytes(const d2c_attention_desc& d, const Plan& p) {
   size_t n = 0;
   if (p.path == Path::tensor && d.dtype == D2C_F32)
-    n += split_bytes(d.batch, d.queries, d.q_heads, d.dim, p.parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, p.parts);
+    n += bound_bytes(d) + split_bytes(d.batch, d.queries, d.q_heads, d.dim, p.parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, p.parts);
   if (p.splits > 1)
     n += align_up(sizeof(float) * p.splits * q_rows(d) * d.dim, 256) + align_up(sizeof(float) * p.splits * q_rows(d), 256);
   return n;
@@ -123,7 +124,6 @@ size_t fwd_workspace(const d2c_attention_desc& d, int mode, int sms) {
 }
 
 size_t delta_bytes(const d2c_attention_desc& d) { return align_up(sizeof(float) * q_rows(d), 256); }
-size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 2 * d.batch * d.kv_heads, 256); }
 size_t staged_bytes(const d2c_attention_desc& d, int parts) {
   if (d.dtype != D2C_F32 || !parts) return 0;
   return 2 * split_bytes(d.batch, d.queries, d.q_heads, d.dim, parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, parts);
@@ -187,8 +187,12 @@ int run_fwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int 
   if (p.path == Path::tensor) {
     Operand x[4];
     own_operands(a, x);
-    if (d.dtype == D2C_F32 && (rc = split_rows(a, p.parts, ws, x, st))) return rc;
-    rc = tc_fwd(d.dtype, a, x, p.parts, st);
+    uint32_t* bounds = reinterpret_cast<uint32_t*>(ws);
+    if (d.dtype == D2C_F32) {
+      if (p.parts == 2 && (rc = largest_sizes(d.dtype, a, false, bounds, st))) return rc;
+      if ((rc = split_rows(a, p.parts, bounds, ws + bound_bytes(d), x, st))) return rc;
+    }
+    rc = tc_fwd(d.dtype, a, x, p.parts, bounds, st);
   } else {
     rc = p.path == Path::few ? few_fwd(d.dtype, a, st) : exact_fwd(d.dtype, a, st);
   }
@@ -209,13 +213,13 @@ int run_bwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int 
   Operand x[4];
   own_operands(a, x);
   int rc;
+  if (tensor && (d.dtype == D2C_F16 || pk.parts == 2) && (rc = largest_sizes(d.dtype, a, d.dtype == D2C_F16, bounds, st))) return rc;
   if (tensor && d.dtype == D2C_F32) {
-    if ((rc = split_rows(a, pk.parts, ws, x, st))) return rc;
+    if ((rc = split_rows(a, pk.parts, bounds, ws, x, st))) return rc;
     ws += staged_bytes(d, pk.parts);
   }
   a.part = reinterpret_cast<float*>(ws);
   if ((rc = delta_rows(d.dtype, a, st))) return rc;
-  if (tensor && d.dtype == D2C_F16 && (rc = tc_bounds(a, bounds, st))) return rc;
   a.splits = pk.splits;
   if ((rc = tensor ? tc_bwd(d.dtype, a, x, pk.parts, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
   if (a.splits > 1) {

@@ -1,5 +1,5 @@
-// Cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, and fp32 tensors staged as bf16
-// (split_rows: hi and lo parts, three products, for fp32 parity; or hi alone), up to 128 channels.
+// Cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, and fp32 tensors staged in 16 bits
+// (split_rows: two fp16 parts, three products, for fp32 parity; or one bf16 part), up to 128 channels.
 //
 // Forward: a block has two tiles of 128 queries of a head and runs over tiles of 128 keys.  S_t = Q_t K^T lands in tensor memory;
 // four warps a tile (a thread a row) form p = 2^(s scale log2 e - m) with the running maximum and sum, and write it over S as the
@@ -24,6 +24,7 @@ struct TcParams {
   void* o;
   float *lse, *part, *part_lse;
   Args a;                        // lengths
+  const uint32_t* bounds;        // two parts: see largest_sizes
   int* status;
 };
 
@@ -162,6 +163,13 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tS + 128 * t + lanes, o_at = tO + DP * t + lanes;
     const int dcols = (p.width + 15) & ~15;
+    float c = p.c, o_mul = 1.f;
+    if constexpr (kParts == 2) {                  // the operands are scaled by powers of two
+      const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
+      const int n_heads = p.B * p.Hkv;
+      c = ldexpf(c, -scale_exponent(q[0]) - scale_exponent(q[n_heads]));
+      o_mul = pow2(-scale_exponent(q[2 * n_heads]));
+    }
     float m = 0.f, l = 0.f;
     bool ok = t < nt;
     for (int j = 0; ok && j < n; ++j) {
@@ -184,7 +192,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(s[k][e]));
-      mx *= p.c;
+      mx *= c;
       if (j == 0) {
         m = mx == -INFINITY ? 0.f : mx;
       } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
@@ -207,8 +215,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int i0 = 64 * h + 2 * e;
-          const float x = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][i0 & 31]), p.c, -m));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][(i0 & 31) + 1]), p.c, -m));
+          const float x = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][i0 & 31]), c, -m));
+          const float y = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][(i0 & 31) + 1]), c, -m));
           sum[e & 1] += x;
           sum[2 + (e & 1)] += y;
           w[e] = pack2<T>(x, y);
@@ -248,7 +256,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           if (c0 + e >= p.D) break;
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e + i]) * inv;
+          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e + i]) * inv * o_mul;
           if (p.splits > 1) store8(p.part + ((long long)split * rows + out) * p.D + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
           else store8(reinterpret_cast<Out*>(p.o) + out * p.D + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
         }
@@ -305,29 +313,68 @@ int fwd_by_width(const CUtensorMap (&m)[3], const TcParams& p, cudaStream_t st) 
   return p.width <= 64 ? launch_fwd<T, Out, 64, kParts>(m, p, st) : launch_fwd<T, Out, 128, kParts>(m, p, st);
 }
 
-// x [B, L, H, D] fp32 with any strides -> [parts][B, L, H, width] bf16: hi = bf16(x), lo = bf16(x - hi); zeros from D on.
-// Up to four tensors in one launch.  A thread writes 8 channels.
-struct SplitArgs {
-  const float* x[4];
-  __nv_bfloat16* out[4];
+// Up to four tensors [B, L, H, D] of one launch: q, k, v, grad_o (which: their places in `bounds`).
+struct RowsArgs {
+  const void* x[4];
+  void* out[4];
   long long s[4][3];
-  int L[4], H[4];
+  int L[4], H[4], which[4], keys[4];
   int B, D, width, parts;
+  Args a;                        // lengths
+  uint32_t* bounds;              // [4][B, Hkv]
 };
-__global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__ SplitArgs a) {
-  const int which = blockIdx.y, L = a.L[which], H = a.H[which], per = a.width / 8;
+
+// Largest size of an element among the valid rows of a clip and key head.  Bits of a float that is not negative order like the float, so
+// that the maximum does not depend on the order of the atomics, one per block.  Elements that are not finite are left out: what they
+// touch is lost anyway, the rest is not.  A warp a row, four rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) bound_kernel(const __grid_constant__ RowsArgs p) {
+  constexpr int kU = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.z, H = p.H[i];
+  if ((int)blockIdx.y >= p.B * H) return;
+  const int h = blockIdx.y % H, b = blockIdx.y / H, hk = h / (H / p.a.Hkv);
+  const int len = p.keys[i] ? key_length(p.a, b) : p.L[i], step = gridDim.x * 8;
+  const T* x = reinterpret_cast<const T*>(p.x[i]) + b * p.s[i][0] + h * p.s[i][2];
+  float most = 0.f;
+  for (int r = blockIdx.x * 8 + warp; r < len; r += step * kU) {
+    float v[kU][4];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[u][e] = r + u * step < len && lane + 32 * e < p.D ? fabsf(to_f32(x[(long long)(r + u * step) * p.s[i][1] + lane + 32 * e])) : 0.f;
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[u][e] < INFINITY) most = fmaxf(most, v[u][e]);
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  __shared__ float all[8];
+  if (lane == 0) all[warp] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) most = fmaxf(most, all[w]);
+    if (most > 0.f) atomicMax(p.bounds + ((long long)p.which[i] * p.B + b) * p.a.Hkv + hk, __float_as_uint(most));
+  }
+}
+
+// x fp32 with any strides -> [parts][B, L, H, width]: fp16 hi and lo of x 2^e, or bf16; zeros from D on.  A thread writes 8 channels.
+__global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__ RowsArgs a) {
+  const int t = blockIdx.y, L = a.L[t], H = a.H[t], per = a.width / 8;
   const long long n = (long long)a.B * L * H * per;
-  const float* x = a.x[which];
-  uint4* out = reinterpret_cast<uint4*>(a.out[which]);
-  const bool wide = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && a.s[which][0] % 4 == 0 && a.s[which][1] % 4 == 0 &&
-                    a.s[which][2] % 4 == 0;
+  const float* x = reinterpret_cast<const float*>(a.x[t]);
+  uint4* out = reinterpret_cast<uint4*>(a.out[t]);
+  const bool wide = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && a.s[t][0] % 4 == 0 && a.s[t][1] % 4 == 0 &&
+                    a.s[t][2] % 4 == 0;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const int c = (int)(i % per) * 8;
     long long r = i / per;
     const int h = (int)(r % H);
     r /= H;
-    const int l = (int)(r % L);
-    const float* src = x + r / L * a.s[which][0] + l * a.s[which][1] + h * a.s[which][2] + c;
+    const int l = (int)(r % L), b = (int)(r / L);
+    const float* src = x + b * a.s[t][0] + l * a.s[t][1] + h * a.s[t][2] + c;
     float f[8];
     if (wide && c + 8 <= a.D) {
       const float4 p = *reinterpret_cast<const float4*>(src), q = *reinterpret_cast<const float4*>(src + 4);
@@ -337,16 +384,41 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__
       for (int e = 0; e < 8; ++e) f[e] = c + e < a.D ? src[e] : 0.f;
     }
     uint32_t hi[4], lo[4];
+    if (a.parts == 2) {
+      const float up = pow2(scale_exponent(a.bounds[((long long)a.which[t] * a.B + b) * a.a.Hkv + h / (H / a.a.Hkv)]));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      hi[e] = ptx::pack_bf16x2(f[2 * e], f[2 * e + 1]);
-      const float x0 = ptx::bf16_lo(hi[e]), x1 = ptx::bf16_hi(hi[e]);
-      // infinity has no rest
-      lo[e] = ptx::pack_bf16x2(fabsf(x0) == INFINITY ? 0.f : f[2 * e] - x0, fabsf(x1) == INFINITY ? 0.f : f[2 * e + 1] - x1);
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = f[2 * e] * up, x1 = f[2 * e + 1] * up;
+        hi[e] = pack2<__half>(x0, x1);
+        const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+        lo[e] = pack2<__half>(fabsf(h2.x) == INFINITY ? 0.f : x0 - h2.x, fabsf(h2.y) == INFINITY ? 0.f : x1 - h2.y);   // infinity has no rest
+      }
+      out[n + i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hi[e] = ptx::pack_bf16x2(f[2 * e], f[2 * e + 1]);
     }
     out[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if (a.parts == 2) out[n + i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
+}
+
+RowsArgs rows_args(const Args& a, uint32_t* bounds) {
+  RowsArgs s{};
+  s.B = a.B; s.D = a.D; s.width = (a.D + 7) / 8 * 8;
+  s.a = a;
+  s.bounds = bounds;
+  return s;
+}
+void add_rows(RowsArgs& s, int i, const Args& a, int which) {
+  const void* src[4] = {a.q, a.k, a.v, a.g};
+  const long long* strides[4] = {a.qs, a.ks, a.vs, a.gs};
+  const bool keys = which == 1 || which == 2;
+  s.x[i] = src[which];
+  s.which[i] = which;
+  s.keys[i] = keys;
+  s.L[i] = keys ? a.Lk : a.Lq;
+  s.H[i] = keys ? a.Hkv : a.Hq;
+  for (int d = 0; d < 3; ++d) s.s[i][d] = strides[which][d];
 }
 
 }  // namespace
@@ -378,21 +450,35 @@ size_t split_bytes(int B, int L, int H, int D, int parts) {
   return align_up((size_t)2 * parts * B * L * H * ((D + 7) / 8 * 8), 256);
 }
 
-// Stages q, k, v and, if it is there, g; o[0..3] become the staged operands.
-int split_rows(const Args& a, int parts, void* workspace, Operand (&o)[4], cudaStream_t st) {
-  SplitArgs s{};
-  s.B = a.B; s.D = a.D; s.width = (a.D + 7) / 8 * 8; s.parts = parts;
-  const void* src[4] = {a.q, a.k, a.v, a.g};
-  const long long* strides[4] = {a.qs, a.ks, a.vs, a.gs};
+// [4][B, Hkv]: the largest sizes of elements of q, k, v and, if it is there, grad_o; with `values_only` of v and grad_o alone.
+int largest_sizes(int dtype, const Args& a, bool values_only, uint32_t* bounds, cudaStream_t st) {
+  D2C_CUDA_TRY(cudaMemsetAsync(bounds, 0, sizeof(uint32_t) * 4 * a.B * a.Hkv, st));
+  RowsArgs s = rows_args(a, bounds);
+  int n = 0;
+  for (int which = values_only ? 2 : 0; which < (a.g ? 4 : 3); ++which) add_rows(s, n++, a, which);
+  const long long heads = (long long)a.B * a.Hq;                 // <= 65535, and not fewer than the key heads
+  const long long rows = (std::max(a.Lq, a.Lk) + 31) / 32;       // steps of a block
+  const unsigned x = (unsigned)std::max<long long>(1, std::min<long long>(rows, (148 * 4 + heads * n - 1) / (heads * n)));
+  const dim3 grid(x, (unsigned)heads, n);
+  switch (dtype) {
+    case D2C_F32: bound_kernel<float><<<grid, 256, 0, st>>>(s); break;
+    case D2C_F16: bound_kernel<__half><<<grid, 256, 0, st>>>(s); break;
+    default: return D2C_ERR_DTYPE;
+  }
+  D2C_LAUNCH_CHECK();
+  return D2C_OK;
+}
+
+// Stages fp32 q, k, v and, if it is there, grad_o; o[0..3] become the staged operands.  Two parts: largest_sizes before.
+int split_rows(const Args& a, int parts, uint32_t* bounds, void* workspace, Operand (&o)[4], cudaStream_t st) {
+  RowsArgs s = rows_args(a, bounds);
+  s.parts = parts;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   const int n = a.g ? 4 : 3;
   long long most = 0;
   for (int i = 0; i < n; ++i) {
-    s.L[i] = i == 0 || i == 3 ? a.Lq : a.Lk;
-    s.H[i] = i == 0 || i == 3 ? a.Hq : a.Hkv;
-    s.x[i] = reinterpret_cast<const float*>(src[i]);
-    s.out[i] = reinterpret_cast<__nv_bfloat16*>(ws);
-    for (int d = 0; d < 3; ++d) s.s[i][d] = strides[i][d];
+    add_rows(s, i, a, i);
+    s.out[i] = ws;
     o[i] = {ws, {(long long)s.L[i] * s.H[i] * s.width, (long long)s.H[i] * s.width, s.width}};
     ws += split_bytes(a.B, s.L[i], s.H[i], a.D, parts);
     most = std::max(most, (long long)a.B * s.L[i] * s.H[i] * (s.width / 8));
@@ -403,12 +489,14 @@ int split_rows(const Args& a, int parts, void* workspace, Operand (&o)[4], cudaS
   return D2C_OK;
 }
 
-int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, cudaStream_t st) {
+int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, const uint32_t* bounds, cudaStream_t st) {
   TcParams p{};
   p.B = a.B; p.Lq = a.Lq; p.Lk = a.Lk; p.Hq = a.Hq; p.Hkv = a.Hkv; p.D = a.D;
   p.width = (a.D + 7) / 8 * 8;
   CUtensorMap m[3];
   int rc;
+  bool staged = false;                           // from fp32
+  if (dtype == D2C_F32) dtype = parts == 2 ? D2C_F16 : D2C_BF16, staged = true;
   if ((rc = tile_map(&m[0], x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
   if ((rc = tile_map(&m[1], x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
   if ((rc = tile_map(&m[2], x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
@@ -416,10 +504,10 @@ int tc_fwd(int dtype, const Args& a, const Operand (&x)[4], int parts, cudaStrea
   p.splits = a.splits;
   p.o = a.o; p.lse = a.lse; p.part = a.part; p.part_lse = a.part_lse;
   p.a = a;
+  p.bounds = bounds;
   if ((rc = status_pointer(&p.status))) return rc;
-  if (dtype == D2C_BF16) return fwd_by_width<__nv_bfloat16, __nv_bfloat16, 1>(m, p, st);
-  if (dtype == D2C_F16) return fwd_by_width<__half, __half, 1>(m, p, st);
-  return parts == 2 ? fwd_by_width<__nv_bfloat16, float, 2>(m, p, st) : fwd_by_width<__nv_bfloat16, float, 1>(m, p, st);
+  if (staged) return parts == 2 ? fwd_by_width<__half, float, 2>(m, p, st) : fwd_by_width<__nv_bfloat16, float, 1>(m, p, st);
+  return dtype == D2C_BF16 ? fwd_by_width<__nv_bfloat16, __nv_bfloat16, 1>(m, p, st) : fwd_by_width<__half, __half, 1>(m, p, st);
 }
 
 }  // namespace attn

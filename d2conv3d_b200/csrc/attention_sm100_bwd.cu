@@ -1,5 +1,5 @@
 // Gradients of cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, up to 128 channels; fp32
-// tensors staged as bf16 (attention_sm100.cu: split_rows), in two parts up to 64 channels, in one up to 128.
+// tensors staged in 16 bits (attention_sm100.cu: split_rows), in two parts up to 64 channels, in one up to 128.
 //
 // One kernel, two uses.  A block keeps a tile of 128 rows X (X1, X2) and runs over tiles of 128 rows Y (Y1, Y2):
 //   S = X1 Y1^T,  dP = X2 Y2^T,  P = 2^(S scale log2 e - lse),  dS = P (dP - delta)
@@ -12,7 +12,7 @@
 // and on the next dP while they form P.
 //
 // fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
-// they are rounded (P by 2^14; dS so that 2 max|grad_o_i| max|v_j|, which bounds it, becomes 2^15) and the sums scaled back.
+// they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, becomes 2^14 .. 2^15) and the sums scaled back.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,7 +28,7 @@ struct BwdParams {
   float c, scale;
   int splits, blocks_x;          // tiles of X per head
   const float *lse, *delta;
-  const uint32_t* bounds;        // fp16: [B, Hkv] pairs: largest |grad_o_i|^2, |v_j|^2 (bits of a float)
+  const uint32_t* bounds;        // fp16: see largest_sizes
   void *g1, *g2;                 // keys: grad_v, grad_k; queries: g2 = grad_q
   float* part;                   // queries [splits][B, Lq, Hq][D]; keys [grad_k, grad_v][splits][B, Lk, Hkv][D]
   Args a;                        // lengths
@@ -75,6 +75,22 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   share(kKeys ? qtiles * group : (len + kRows - 1) / kRows, p.splits, split, i0, i1);
   if (kKeys && x0 >= len) i1 = i0;                // keys that are not there
   const int n = i1 - i0;
+  // powers of two: of the operands (two parts), and of dS
+  int e_q = 0, e_k = 0, e_v = 0, e_g = 0, e_ds = 0;
+  if constexpr (kHalf) {
+    const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
+    const int n_heads = p.B * p.Hkv;
+    const float bound = 2.f * p.D * __uint_as_float(q[2 * n_heads]) * __uint_as_float(q[3 * n_heads]);
+    if (bound > 0.f && bound < INFINITY) e_ds = max(-100, min(100, 14 - ilogbf(bound)));       // 2^e_ds * bound <= 2^15
+    if constexpr (kParts == 2) {
+      e_q = scale_exponent(q[0]);
+      e_k = scale_exponent(q[n_heads]);
+      e_v = scale_exponent(q[2 * n_heads]);
+      e_g = scale_exponent(q[3 * n_heads]);
+    }
+  }
+  // dS 2^e_ds = P (dP dp_mul - delta d_mul), with P scaled by 2^kUp and dP by its operands
+  const float d_mul = exp2f((float)e_ds - kUp), dp_mul = exp2f((float)(e_ds - e_v - e_g) - kUp);
   // tile i of Y: head, first row
   auto y_head = [&](int i) { return kKeys ? head * group + i / qtiles : hk; };
   auto y_row = [&](int i) { return (kKeys ? i % qtiles : i) * kRows; };
@@ -122,7 +138,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
                 const int r = lane + 32 * e;
                 const bool live = r0 + r < p.Lq;  // queries that are not there: P = 0
                 rows_of_y[s >> 1][0][r] = live ? p.lse[at + r] - kUp : INFINITY;
-                rows_of_y[s >> 1][1][r] = live ? p.delta[at + r] : 0.f;
+                rows_of_y[s >> 1][1][r] = live ? p.delta[at + r] * d_mul : 0.f;
               }
               __syncwarp();
             }
@@ -203,19 +219,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     if (!kKeys && xi < p.Lq) {
       const long long at = ((long long)b * p.Hq + head) * p.Lq + xi;
       lse = p.lse[at] - kUp;
-      delta = p.delta[at];
+      delta = p.delta[at] * d_mul;
     }
     const bool row_in = kKeys ? xi < len : true;
-    // fp16: dS leaves scaled by 2^down * 2^kUp ...
-    float ds_mul = 1.f, ds_back = 1.f;
-    if constexpr (kHalf) {
-      const uint32_t* q = p.bounds + 2 * ((long long)b * p.Hkv + hk);
-      const float bound = 2.f * sqrtf(__uint_as_float(q[0])) * sqrtf(__uint_as_float(q[1]));
-      int e = 0;                                  // 2^e * bound <= 2^15
-      if (bound > 0.f && bound < INFINITY) e = max(-100, min(100, 14 - ilogbf(bound)));
-      ds_mul = exp2f((float)e - kUp);
-      ds_back = exp2f((float)-e);
-    }
+    float c = p.c;
+    if constexpr (kParts == 2) c = ldexpf(c, -e_q - e_k);
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
       if (!warp_wait(s_full, i & 1, abort_flag)) { ok = false; break; }
@@ -240,7 +248,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            float pr = exp2_fast(fmaf(__uint_as_float(s[k][e + u]), p.c, -lv[u]));
+            float pr = exp2_fast(fmaf(__uint_as_float(s[k][e + u]), c, -lv[u]));
             if (kKeys && !row_in) pr = 0.f;
             s[k][e + u] = __float_as_uint(pr);
           }
@@ -276,8 +284,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           float v[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            v[u] = __uint_as_float(s[k][e + u]) * (__uint_as_float(d[e + u]) - dv[u]);
-            if constexpr (kHalf) v[u] *= ds_mul;
+            v[u] = __uint_as_float(s[k][e + u]) * (kHalf ? fmaf(__uint_as_float(d[e + u]), dp_mul, -dv[u]) : __uint_as_float(d[e + u]) - dv[u]);
             if (kKeys ? !row_in : 64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
           }
           w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
@@ -304,7 +311,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       const int there = kKeys ? p.Lk : p.Lq;
       const long long rows = (long long)p.B * there * heads, out = ((long long)b * there + xi) * heads + head;
       const bool first = kKeys && half == 0;
-      const float mul = first ? exp2f(-kUp) : p.scale * ds_back;
+      // grad_v: P 2^kUp and grad_o; dS and the other factor
+      const float mul = first ? exp2f(-kUp - (float)e_g) : p.scale * exp2f((float)-e_ds) * exp2f((float)-(kKeys ? e_q : e_k));
       const uint32_t acc = (first ? tA1 : tA2) + lanes;
       Out* dst = reinterpret_cast<Out*>(first ? p.g1 : p.g2) + out * p.D;
       float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
@@ -340,30 +348,6 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   }
 }
 
-// Largest squared norm of a row of x [B, L, H, D] among the valid ones, per (clip, key head): bits of a float that is not negative
-// order like the float, so that the maximum does not depend on the order of the atomics (a NaN is above all).  A warp a row.
-__global__ void __launch_bounds__(256) row_bound_kernel(Args a, const __half* x, long long sb, long long sl, long long sh, int L, int H,
-                                                        int keys, uint32_t* out) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y % H, b = blockIdx.y / H, hk = h / (H / a.Hkv);
-  const int len = keys ? key_length(a, b) : L;
-  float most = 0.f;
-  bool bad = false;
-  for (int r = blockIdx.x * 8 + warp; r < len; r += gridDim.x * 8) {
-    const __half* p = x + b * sb + (long long)r * sl + h * sh;
-    float s = 0.f;
-    for (int c = lane; c < a.D; c += 32) {
-      const float v = __half2float(p[c]);
-      s = fmaf(v, v, s);
-    }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    bad |= s != s;
-    most = fmaxf(most, s);
-  }
-  if (lane == 0 && len > 0) atomicMax(out + 2 * ((long long)b * a.Hkv + hk), bad ? 0x7fffffffu : __float_as_uint(most));
-}
-
 template <typename T, typename Out, int DP, int kParts, bool kKeys>
 int launch(const CUtensorMap (&m)[4], const BwdParams& p, cudaStream_t st) {
   const long long blocks = (long long)p.blocks_x * p.splits * (kKeys ? p.Hkv : p.Hq) * p.B;
@@ -385,26 +369,14 @@ int by_width(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStrea
 
 }  // namespace
 
-int tc_bounds(const Args& a, uint32_t* bounds, cudaStream_t st) {
-  D2C_CUDA_TRY(cudaMemsetAsync(bounds, 0, sizeof(uint32_t) * 2 * a.B * a.Hkv, st));
-  const long long hq = (long long)a.B * a.Hq, hk = (long long)a.B * a.Hkv;
-  if (hq > 65535) return D2C_ERR_TOO_LARGE;
-  auto blocks = [](int L, long long heads) {
-    return (unsigned)std::max<long long>(1, std::min<long long>((L + 7) / 8, (148 * 8 + heads - 1) / heads));
-  };
-  row_bound_kernel<<<dim3(blocks(a.Lq, hq), (unsigned)hq), 256, 0, st>>>(a, (const __half*)a.g, a.gs[0], a.gs[1], a.gs[2], a.Lq, a.Hq, 0, bounds);
-  D2C_LAUNCH_CHECK();
-  row_bound_kernel<<<dim3(blocks(a.Lk, hk), (unsigned)hk), 256, 0, st>>>(a, (const __half*)a.v, a.vs[0], a.vs[1], a.vs[2], a.Lk, a.Hkv, 1, bounds + 1);
-  D2C_LAUNCH_CHECK();
-  return D2C_OK;
-}
-
 int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys, const uint32_t* bounds, cudaStream_t st) {
   BwdParams p{};
   p.B = a.B; p.Lq = a.Lq; p.Lk = a.Lk; p.Hq = a.Hq; p.Hkv = a.Hkv; p.D = a.D;
   p.width = (a.D + 7) / 8 * 8;
   CUtensorMap q, k, v, g;
   int rc;
+  const bool staged = dtype == D2C_F32;
+  if (staged) dtype = parts == 2 ? D2C_F16 : D2C_BF16;
   if ((rc = tile_map(&q, x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
   if ((rc = tile_map(&k, x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
   if ((rc = tile_map(&v, x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
@@ -418,9 +390,8 @@ int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys
   p.part = a.part;
   p.a = a;
   if ((rc = status_pointer(&p.status))) return rc;
-  if (dtype == D2C_BF16) return by_width<__nv_bfloat16, __nv_bfloat16>(maps, p, keys, st);
-  if (dtype == D2C_F16) return by_width<__half, __half>(maps, p, keys, st);
-  return parts == 2 ? by_side<__nv_bfloat16, float, 64, 2>(maps, p, keys, st) : by_width<__nv_bfloat16, float>(maps, p, keys, st);
+  if (staged) return parts == 2 ? by_side<__half, float, 64, 2>(maps, p, keys, st) : by_width<__nv_bfloat16, float>(maps, p, keys, st);
+  return dtype == D2C_BF16 ? by_width<__nv_bfloat16, __nv_bfloat16>(maps, p, keys, st) : by_width<__half, __half>(maps, p, keys, st);
 }
 
 }  // namespace attn

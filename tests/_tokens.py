@@ -104,16 +104,22 @@ def attention_oracle(q, k, v, g, lengths, scale, p_half, product=0.0):
             o = p @ V
             # a score: D products added in fp32 (tensor cores may truncate: twice u), scaled; its exponential and the row's sum
             ds = ((2 * D + 8) * U + product) * (Q.abs() @ K.abs().T) * abs(scale)
+            # parts below fp16's normal range are off by up to 2^-25 of what they were scaled to: 2^14 for the largest element
+            low = 2.0 ** -38 if product else 0.0
+            ds = ds + low * Q.abs().max() * K.abs().max() * D * abs(scale)
             rel = 2 * ds.max(-1, keepdim=True).values + (s.abs().max() * 4 + 16) * U + (m / 64 + 64) * 2 * U
             chain = (m / 8 + 64) * 2 * U                                 # additions along the keys
             val["o"][b, :, h] = o
-            err["o"][b, :, h] = (p * (rel + 2 * p_half + product + chain)) @ V.abs() + 4 * U * o.abs()
+            p_low = 2.0 ** -25 if p_half > U else 0.0                    # a probability against the row's largest
+            err["o"][b, :, h] = (p * (rel + 2 * p_half + product + chain)) @ V.abs() + 4 * U * o.abs() + p_low * V.abs().sum(0)
             dp = G @ V.T
             delta = (G * o).sum(-1, keepdim=True)
             e_delta = (G.abs() * (err["o"][b, :, h] + half(dtype) * o.abs())).sum(-1, keepdim=True) + 2 * D * U * (G * o).abs().sum(-1, keepdim=True)
             e_dp = ((2 * D + 4) * U + product) * (G.abs() @ V.abs().T)
             d = p * (dp - delta)
             e_d = p * ((dp - delta).abs() * (rel + 2 * p_half + 4 * U) + (e_dp + e_delta) * (1 + rel + p_half))
+            if p_half > U:
+                e_d = e_d + 2.0 ** -38 * D * G.abs().max() * V.abs().max()
             rows = (Lq / 8 + 64) * 2 * U * n                             # additions along the queries
             val["gq"][b, :, h] = d @ K * scale
             err["gq"][b, :, h] = ((e_d + d.abs() * (chain + product)) @ K.abs()) * abs(scale)

@@ -22,10 +22,10 @@ def run(q, k, v, g, lengths=None, scale=None):
     return (o.detach(),) + torch.autograd.grad(o, leaves, g)
 
 
-# fp32 by math mode: (half a step of the probabilities, what the operands' rounding takes from a product).  "auto": hi + lo bf16
-# parts keep a factor to 2^-18 (half a step of the second part, 2^-9 of at most 2^-9), and lo lo, at most 2^-18, is left out.
+# fp32 by math mode: (half a step of the probabilities, what the operands' rounding takes from a product).  "auto": hi + lo fp16
+# parts keep a factor to 2^-22 (half a step of the second part, 2^-11 of at most 2^-11), and lo lo, at most 2^-22, is left out.
 # "bf16": each factor to 2^-9.
-FP32_MODES = {"fp32": (U, 0.0), "auto": (2.0 ** -18, 3 * 2.0 ** -18), "bf16": (2.0 ** -9, 2.0 ** -8 + 2.0 ** -18)}
+FP32_MODES = {"fp32": (U, 0.0), "auto": (2.0 ** -22, 3 * 2.0 ** -22), "bf16": (2.0 ** -9, 2.0 ** -8 + 2.0 ** -18)}
 
 
 def check(q, k, v, g, lengths=None, scale=None):
