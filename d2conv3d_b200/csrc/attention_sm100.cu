@@ -43,7 +43,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
               const __grid_constant__ TcParams p) {
   constexpr int kStages = kFwdStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kQ = kQTiles<DP, kParts>;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kStages + 8];
+  __shared__ uint64_t bars[2 * kStages + 9];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -54,7 +54,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
   auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
   const uint32_t q_full = bar0 + 8 * (2 * kStages), tail = q_full + 8, done = q_full + 16;
   auto s_full = [&](int t) { return q_full + 24 + 8 * t; };
-  auto p_ready = [&](int t) { return q_full + 40 + 8 * t; };
+  auto p_ready = [&](int t, int h) { return q_full + 40 + 16 * t + 8 * h; };   // a half of the keys each
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   long long id = blockIdx.x;
@@ -72,7 +72,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     ptx::mbar_init(q_full, 1);
     ptx::mbar_init(tail, 1);
     ptx::mbar_init(done, 1);
-    for (int t = 0; t < 2; ++t) { ptx::mbar_init(s_full(t), 1); ptx::mbar_init(p_ready(t), 4); }
+    for (int t = 0; t < 2; ++t) { ptx::mbar_init(s_full(t), 1); ptx::mbar_init(p_ready(t, 0), 4); ptx::mbar_init(p_ready(t, 1), 4); }
     abort_word = 0;
     ptx::fence_mbar_init();
   }
@@ -123,14 +123,16 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       for (int w = i > kStages ? i - kStages : 0; w < i; ++w) drain(full(w % kStages), (w / kStages) & 1);
     }
   } else if (warp == kFwdMmaWarp) {
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
+      const uint64_t d_q = ptx::umma_desc_kmajor_sw128(sq), d_k = ptx::umma_desc_kmajor_sw128(ring),
+                     d_v = ptx::umma_desc_mnmajor_sw128(ring, kHalfBytes, 1024);
       const uint32_t id_s = idesc_of<T>(kRows, false), id_o = idesc_of<T>((p.width + 15) & ~15, true);
       const int ksteps = (p.width + 15) >> 4;
       auto run = [&]() {
         if (!ptx::mbar_wait(q_full, 0, abort_flag) || !ptx::mbar_wait(full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
         for (int t = 0; t < nt; ++t) {
-          mma_scores<DP, kParts>(tS + 128 * t, sq + t * kTB, ring, id_s, ksteps);
+          mma_scores<DP, kParts>(tS + 128 * t, d_q + (t * kTB >> 4), d_k, id_s, ksteps);
           ptx::umma_commit(s_full(t));
         }
         ptx::umma_commit(empty(0));
@@ -139,12 +141,14 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           const bool more = j + 1 < n;
           if (!ptx::mbar_wait(full(sv), (iv / kStages) & 1, abort_flag)) return;
           for (int t = 0; t < nt; ++t) {
-            if (!ptx::mbar_wait(p_ready(t), j & 1, abort_flag)) return;
-            ptx::tc_fence_after();
-            mma_weigh<DP, kParts>(tO + DP * t, tS + 128 * t, 0, 64, ring + sv * kTB, id_o, j > 0);
+            for (int h = 0; h < 2; ++h) {         // the first half of the keys while the second's p is formed
+              if (!ptx::mbar_wait(p_ready(t, h), j & 1, abort_flag)) return;
+              ptx::tc_fence_after();
+              mma_weigh<DP, kParts>(tO + DP * t, tS + 128 * t + 32 * h, 64, d_v + (sv * kTB >> 4) + 512 * h, id_o, j > 0 || h > 0);
+            }
             if (more) {
               if (t == 0 && !ptx::mbar_wait(full(sk), (ik / kStages) & 1, abort_flag)) return;
-              mma_scores<DP, kParts>(tS + 128 * t, sq + t * kTB, ring + sk * kTB, id_s, ksteps);
+              mma_scores<DP, kParts>(tS + 128 * t, d_q + (t * kTB >> 4), d_k + (sk * kTB >> 4), id_s, ksteps);
             }
             ptx::umma_commit(s_full(t));          // after the last tile: O_t is complete
           }
@@ -175,23 +179,27 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     for (int j = 0; ok && j < n; ++j) {
       if (!warp_wait(s_full(t), j & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
+      // scores, 32 columns at a time: the next are on their way while the maximum of these is taken
       uint32_t s[4][32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ptx::tmem_ld_32x32(s_at + 32 * k, s[k]);
-      ptx::tmem_ld_wait();
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       const int valid = len - (j0 + j) * kRows;
-      if (valid < kRows) {
+      ptx::tmem_ld_32x32(s_at, s[0]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        ptx::tmem_ld_wait();
+        if (k < 3) ptx::tmem_ld_32x32(s_at + 32 * (k + 1), s[k + 1]);
+        if (valid < kRows) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * k + e >= valid) s[k][e] = 0xff800000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mx4[i] = fmaxf(fmaxf(mx4[i], __uint_as_float(s[k][e + 2 * i])), __uint_as_float(s[k][e + 2 * i + 1]));
       }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(s[k][e]));
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx *= c;
       if (j == 0) {
         m = mx == -INFINITY ? 0.f : mx;
@@ -224,12 +232,12 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         }
         tmem_st_32x32(s_at + 32 * h, w);
         if constexpr (kParts == 2) tmem_st_32x32(s_at + 64 + 32 * h, rest);
+        tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready(t, h));
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(p_ready(t));
     }
     if (ok && n > 0) {
       ok = warp_wait(s_full(t), n & 1, abort_flag);

@@ -163,21 +163,24 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           for (int w = i > kSt ? i - kSt : 0; w < i; ++w) drain(full(w % kSt), (w / kSt) & 1);
         }
       }
-    } else if (warp == kMmaWarp && lane == 0 && n > 0) {
+    } else if (warp == kMmaWarp && n > 0 && elect_one()) {
+      const uint64_t d_x = ptx::umma_desc_kmajor_sw128(sx), d_y = ptx::umma_desc_kmajor_sw128(ring),
+                     d_yt = ptx::umma_desc_mnmajor_sw128(ring, kHalfBytes, 1024);
       const uint32_t id_s = idesc_of<T>(kRows, false), id_a = idesc_of<T>((p.width + 15) & ~15, true);
       const int ksteps = (p.width + 15) >> 4;
-      auto slot = [&](int i) { return ring + (i % kSt) * kTB; };
+      auto slot = [&](int i) { return (uint32_t)((i % kSt) * kTB) >> 4; };
       auto there = [&](int i) { return ptx::mbar_wait(full(i % kSt), (i / kSt) & 1, abort_flag); };
       auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {   // each half of the columns has its parts at its own start
-        mma_weigh<DP, kParts>(acc, w, 32, 32, y, id_a, more);
+        mma_weigh<DP, kParts>(acc, w, 32, d_yt + y, id_a, more);
+        mma_weigh<DP, kParts>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
       };
       auto run = [&]() {
         if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
         ptx::tc_fence_after();
-        mma_scores<DP, kParts>(tS, sx, slot(0), id_s, ksteps);
+        mma_scores<DP, kParts>(tS, d_x, d_y + slot(0), id_s, ksteps);
         ptx::umma_commit(s_full);
         if (!there(1)) return;
-        mma_scores<DP, kParts>(tD, sx + kTB, slot(1), id_s, ksteps);
+        mma_scores<DP, kParts>(tD, d_x + (kTB >> 4), d_y + slot(1), id_s, ksteps);
         ptx::umma_commit(dp_full);
         if (!kKeys) ptx::umma_commit(empty(1));
         for (int i = 0; i < n; ++i) {
@@ -191,7 +194,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           if (more) {
             if (!there(y1 + 2)) return;
-            mma_scores<DP, kParts>(tS, sx, slot(y1 + 2), id_s, ksteps);
+            mma_scores<DP, kParts>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
           }
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
@@ -200,7 +203,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           ptx::umma_commit(empty(y1 % kSt));
           if (more) {
             if (!there(y2 + 2)) return;
-            mma_scores<DP, kParts>(tD, sx + kTB, slot(y2 + 2), id_s, ksteps);
+            mma_scores<DP, kParts>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
             if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
           }
