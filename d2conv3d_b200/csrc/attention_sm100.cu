@@ -216,17 +216,19 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           tmem_st_32x32(o_at + c0, o);
         }
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      F2 sum[2] = {0ull, 0ull};
+      const F2 c2 = f2(c, c), m2 = f2(-m, -m);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t w[32], rest[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int i0 = 64 * h + 2 * e;
-          const float x = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][i0 & 31]), c, -m));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[i0 >> 5][(i0 & 31) + 1]), c, -m));
-          sum[e & 1] += x;
-          sum[2 + (e & 1)] += y;
+          float x, y;
+          f2_split(fma2(f2(__uint_as_float(s[i0 >> 5][i0 & 31]), __uint_as_float(s[i0 >> 5][(i0 & 31) + 1])), c2, m2), x, y);
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          sum[e & 1] = add2(sum[e & 1], f2(x, y));
           w[e] = pack2<T>(x, y);
           if constexpr (kParts == 2) rest[e] = pack2_rest(x, y, w[e]);
         }
@@ -237,7 +239,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_ready(t, h));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float sa, sb;
+      f2_split(add2(sum[0], sum[1]), sa, sb);
+      l += sa + sb;
     }
     if (ok && n > 0) {
       ok = warp_wait(s_full(t), n & 1, abort_flag);

@@ -227,6 +227,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     const bool row_in = kKeys ? xi < len : true;
     float c = p.c;
     if constexpr (kParts == 2) c = ldexpf(c, -e_q - e_k);
+    const F2 c2 = f2(c, c);
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
       if (!warp_wait(s_full, i & 1, abort_flag)) { ok = false; break; }
@@ -241,6 +242,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         if (lane == 0) ptx::mbar_arrive(p_ready);
       }
       const int valid = kKeys ? kRows : len - y_row(i0 + i);   // columns from there on are masked
+      const bool ragged = valid < kRows;
       const float* ly = kKeys ? &rows_of_y[(2 * i % kSt) >> 1][0][64 * half] : nullptr;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -248,12 +250,14 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (int e = 0; e < 32; e += 4) {
           float4 l4 = make_float4(lse, lse, lse, lse);
           if constexpr (kKeys) l4 = *reinterpret_cast<const float4*>(ly + 32 * k + e);
-          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+          const F2 lv[2] = {f2(-l4.x, -l4.y), f2(-l4.z, -l4.w)};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            float pr = exp2_fast(fmaf(__uint_as_float(s[k][e + u]), c, -lv[u]));
-            if (kKeys && !row_in) pr = 0.f;
-            s[k][e + u] = __float_as_uint(pr);
+          for (int u = 0; u < 4; u += 2) {
+            float x, y;
+            f2_split(fma2(f2(__uint_as_float(s[k][e + u]), __uint_as_float(s[k][e + u + 1])), c2, lv[u / 2]), x, y);
+            const bool out = kKeys && !row_in;
+            s[k][e + u] = out ? 0u : __float_as_uint(exp2_fast(x));
+            s[k][e + u + 1] = out ? 0u : __float_as_uint(exp2_fast(y));
           }
         }
       if constexpr (kKeys) {
@@ -283,12 +287,19 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (int e = 0; e < 32; e += 4) {
           float4 d4 = make_float4(delta, delta, delta, delta);
           if constexpr (kKeys) d4 = *reinterpret_cast<const float4*>(ly + kRows + 32 * k + e);
-          const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+          const F2 dv[2] = {f2(-d4.x, -d4.y), f2(-d4.z, -d4.w)};
           float v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            v[u] = __uint_as_float(s[k][e + u]) * (kHalf ? fmaf(__uint_as_float(d[e + u]), dp_mul, -dv[u]) : __uint_as_float(d[e + u]) - dv[u]);
-            if (kKeys ? !row_in : 64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
+          for (int u = 0; u < 4; u += 2) {
+            const F2 dp = f2(__uint_as_float(d[e + u]), __uint_as_float(d[e + u + 1]));
+            const F2 t = mul2(f2(__uint_as_float(s[k][e + u]), __uint_as_float(s[k][e + u + 1])),
+                              kHalf ? fma2(dp, f2(dp_mul, dp_mul), dv[u / 2]) : add2(dp, dv[u / 2]));
+            f2_split(t, v[u], v[u + 1]);
+          }
+          if (kKeys ? !row_in : ragged) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (kKeys || 64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
           }
           w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
           w[16 * k + e / 2 + 1] = pack2<T>(v[2], v[3]);

@@ -154,6 +154,7 @@ __device__ __forceinline__ void store8(Out* dst, const float (&f)[8], int n, boo
       if (i < n) dst[i] = from_f32<Out>(f[i]);
   }
 }
+// (A polynomial on the FMA pipe for a share of the values made no kernel faster: they wait for one another, not for this pipe.)
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -164,6 +165,30 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // (8 * 208 + 4 * 80 <= 12 * 168).  Executed by every warp of a group of four.
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+
+// Pairs of floats: one instruction for two operations.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 // Called by all threads at a kernel's end: reports a wait that gave up to the host.
 __device__ __forceinline__ void report(int* status, volatile int* abort_flag) {
