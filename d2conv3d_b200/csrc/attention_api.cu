@@ -79,12 +79,14 @@ int fewest_shares(int parts, int steps, long long rows, int dim) {
   return (int)std::min<long long>(ceil_div(steps, kChainTiles), std::max(1LL, (2LL << 30) / (4 * rows * dim)));
 }
 
-Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, int steps_rows, int sms) {
+// `slots` blocks at a time on the tensor cores.
+Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, int steps_rows, int slots,
+               int sms) {
   const bool tensor = parts > 0;
   const int tile = tensor ? 128 : kTile;
   const int steps = ceil_div(steps_rows, tile);
   return {tensor ? Path::tensor : Path::exact,
-          shares((long long)ceil_div(rows_x, tile * per_block) * heads_x * d.batch, steps, tensor ? sms : 2 * sms, tensor ? 3.0 : 1.0,
+          shares((long long)ceil_div(rows_x, tile * per_block) * heads_x * d.batch, steps, tensor ? slots : 2 * sms, tensor ? 3.0 : 1.0,
                  join_steps(rows_out, d.dim), fewest_shares(parts, steps, rows_out, d.dim)),
           parts};
 }
@@ -98,14 +100,15 @@ Plan plan_fwd(const d2c_attention_desc& d, int mode, bool aligned, int sms) {
   }
   const int parts = tensor_parts(d, mode, aligned, false);
   const bool two_tiles = parts > 0 && !(parts == 2 && d.dim > 64);
-  return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), two_tiles ? 2 : 1, d.keys, sms);
+  return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), two_tiles ? 2 : 1, d.keys, sms, sms);
 }
 // A gradient kernel's block has a tile of one side and runs over the other.
 Plan plan_bwd(const d2c_attention_desc& d, int mode, bool keys, bool aligned, int sms) {
   const int parts = tensor_parts(d, mode, aligned, true);
-  if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, sms);
+  const int slots = parts == 1 && d.dim <= 64 ? 2 * sms : sms;
+  if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, slots, sms);
   const int tile = parts ? 128 : kTile;
-  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), sms);
+  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), slots, sms);
 }
 
 size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 4 * d.batch * d.kv_heads, 256); }

@@ -445,13 +445,13 @@ int status_pointer(int** out) {
 }
 
 // [clips, tokens, heads, D] 16-bit; a dimension of one element has no stride.
-int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips) {
+int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips, int rows) {
   EncodeTiled f;
   if (const int rc = encoder(&f)) return rc;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)clips};
   auto bytes = [&](long long st, int n) { return (cuuint64_t)(n == 1 ? 256 : 2 * st); };
   const cuuint64_t strides[3] = {bytes(o.s[2], heads), bytes(o.s[1], tokens), bytes(o.s[0], clips)};
-  const cuuint32_t box[4] = {64, 1, kRows, 1}, ones[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, ones[4] = {1, 1, 1, 1};
   const CUresult rc = f(map, dtype == D2C_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                         const_cast<void*>(o.p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -7,9 +7,13 @@
 //   keys:     X = (k, v),      Y = (q, grad_o):   grad_v += P Y2, grad_k += dS Y1      (S, P, dS are transposed; over all heads
 //                                                                                       that share the keys)
 // so that every gradient has one writer: no atomics, the same bits in every call, for 7 products a score instead of 5.  S, dP and
-// the accumulators fill tensor memory (4 x 128 columns); P and dS go back over S and dP as 16-bit A operands.  8 warps, a thread a
-// row and half of the columns.  The order of the issued products lets the tensor cores work on the next S while the warps form dS,
-// and on the next dP while they form P.
+// the accumulators stay in tensor memory; P and dS go back over S and dP as 16-bit A operands.  The order of the issued products lets
+// the tensor cores work on the next S while the warps form dS, and on the next dP while they form P.
+//
+// A tile's products, exponentials and gradients wait for one another: what a SM does at a time is what it has of independent tiles.  Up
+// to 64 channels Y tiles have 64 rows (kY), so that tensor memory (64 + 64 + 64 + 64 columns) and shared memory hold two blocks a SM, of
+// 4 working warps, a thread a row.  Above, and with operands in two parts, Y tiles have 128 rows and the one block has 8 working warps, a
+// thread a row and half of the columns.
 //
 // fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
 // they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, becomes 2^14 .. 2^15) and the sums scaled back.
@@ -35,23 +39,30 @@ struct BwdParams {
   int* status;
 };
 
-constexpr int kThreads = 384;                     // 8 working warps; MMA issuer, loader, two idle (see registers_up)
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+template <int DP, int kParts>
+constexpr int kYRows = DP * kParts == 64 ? 64 : 128;
+template <int DP, int kParts>
+constexpr int kThreads = kYRows<DP, kParts> == 64 ? 256 : 384;       // working warps; MMA issuer, loader, two idle (see registers_up)
 template <int DP, int kParts>
 constexpr int kStages = DP * kParts == 64 ? 8 : 4;
 template <int DP, int kParts>
-constexpr int kSmem = kTileBytes<DP> * kParts * (2 + kStages<DP, kParts>) + 1024;
+constexpr int kYBytes = kYRows<DP, kParts> * DP * 2 * kParts;
+template <int DP, int kParts>
+constexpr int kSmem = 2 * kTileBytes<DP> * kParts + kStages<DP, kParts> * kYBytes<DP, kParts> + 1024;
 
 template <typename T, typename Out, int DP, int kParts, bool kKeys>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<DP, kParts>, kYRows<DP, kParts> == 64 ? 2 : 1)
 bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2, const __grid_constant__ CUtensorMap my1,
               const __grid_constant__ CUtensorMap my2, const __grid_constant__ BwdParams p) {
-  constexpr int kSt = kStages<DP, kParts>, kTB = kTileBytes<DP> * kParts;
+  constexpr int kY = kYRows<DP, kParts>, kWork = kY / 16;        // rows of a Y tile, working warps
+  constexpr int kSt = kStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kYB = kYBytes<DP, kParts>;
+  constexpr int kMmaWarp = kWork, kLoadWarp = kWork + 1, kCols = kY == 64 ? 256 : 512;
+  static_assert(kY == 128 || DP == 64);
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kSt + 8];
-  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][2][kRows];     // lse - kUp, delta of the queries of a Y tile
+  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][2][kY];     // lse - kUp, delta of the queries of a Y tile
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -70,9 +81,9 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   const int group = p.Hq / p.Hkv, hk = kKeys ? head : head / group;
   const int x0 = xb * kRows;
   const int len = key_length(p.a, b);
-  const int qtiles = (p.Lq + kRows - 1) / kRows;
+  const int qtiles = (p.Lq + kY - 1) / kY;
   int i0, i1;
-  share(kKeys ? qtiles * group : (len + kRows - 1) / kRows, p.splits, split, i0, i1);
+  share(kKeys ? qtiles * group : (len + kY - 1) / kY, p.splits, split, i0, i1);
   if (kKeys && x0 >= len) i1 = i0;                // keys that are not there
   const int n = i1 - i0;
   // powers of two: of the operands (two parts), and of dS
@@ -93,7 +104,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   const float d_mul = exp2f((float)e_ds - kUp), dp_mul = exp2f((float)(e_ds - e_v - e_g) - kUp);
   // tile i of Y: head, first row
   auto y_head = [&](int i) { return kKeys ? head * group + i / qtiles : hk; };
-  auto y_row = [&](int i) { return (kKeys ? i % qtiles : i) * kRows; };
+  auto y_row = [&](int i) { return (kKeys ? i % qtiles : i) * kY; };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) { ptx::mbar_init(full(i), 1); ptx::mbar_init(empty(i), 1); }
@@ -102,22 +113,23 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     ptx::mbar_init(done, 1);
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(dp_full, 1);
-    ptx::mbar_init(p_ready, 8);
-    ptx::mbar_init(ds_ready, 8);
+    ptx::mbar_init(p_ready, kWork);
+    ptx::mbar_init(ds_ready, kWork);
     abort_word = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kMmaWarp) {
-    ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), kCols);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = tmem_slot, tS = tmem, tD = tmem + 128, tA1 = tmem + 256, tA2 = tmem + 384;
+  const uint32_t tmem = tmem_slot, tS = tmem, tD = tmem + kY, tA1 = tmem + 2 * kY, tA2 = tA1 + (kY == 64 ? 64 : 128);
 
-  if (warp >= 8) {
-    registers_down();
+  if (warp >= kWork) {
+    if constexpr (kY == 64) registers_down_4();
+    else registers_down();
     if (warp == kLoadWarp) {
       int i = 0;                                  // Y tiles asked for: Y1 Y2 Y1 Y2 ...
       if (n > 0) {
@@ -134,7 +146,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             if (!second) {
               const long long at = ((long long)b * p.Hq + h) * p.Lq + r0;
 #pragma unroll
-              for (int e = 0; e < kRows / 32; ++e) {
+              for (int e = 0; e < kY / 32; ++e) {
                 const int r = lane + 32 * e;
                 const bool live = r0 + r < p.Lq;  // queries that are not there: P = 0
                 rows_of_y[s >> 1][0][r] = live ? p.lse[at + r] - kUp : INFINITY;
@@ -144,15 +156,15 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             }
           }
           // keys behind the clip's length may hold anything: dS is 0 there, and 0 * NaN is NaN
-          const bool patch = !kKeys && !second && len - r0 < kRows && len < p.Lk;
-          const uint32_t bar = patch ? tail : full(s), dst = ring + s * kTB;
+          const bool patch = !kKeys && !second && len - r0 < kY && len < p.Lk;
+          const uint32_t bar = patch ? tail : full(s), dst = ring + s * kYB;
           if (lane == 0) {
-            ptx::mbar_arrive_expect_tx(bar, kTB);
-            tma_tile<DP, kParts>(dst, second ? &my2 : &my1, h, r0, b, p.B, bar);
+            ptx::mbar_arrive_expect_tx(bar, kYB);
+            tma_tile<DP, kParts, kY>(dst, second ? &my2 : &my1, h, r0, b, p.B, bar);
           }
           if (patch) {                            // the last tile: once per block
             drain(tail, 0);
-            clear_rows<DP, kParts>(dst, len - r0);
+            clear_rows<DP, kParts, kY>(dst, len - r0);
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(full(s));
@@ -165,22 +177,22 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       }
     } else if (warp == kMmaWarp && n > 0 && elect_one()) {
       const uint64_t d_x = ptx::umma_desc_kmajor_sw128(sx), d_y = ptx::umma_desc_kmajor_sw128(ring),
-                     d_yt = ptx::umma_desc_mnmajor_sw128(ring, kHalfBytes, 1024);
-      const uint32_t id_s = idesc_of<T>(kRows, false), id_a = idesc_of<T>((p.width + 15) & ~15, true);
+                     d_yt = ptx::umma_desc_mnmajor_sw128(ring, kY * 128, 1024);
+      const uint32_t id_s = idesc_of<T>(kY, false), id_a = idesc_of<T>((p.width + 15) & ~15, true);
       const int ksteps = (p.width + 15) >> 4;
-      auto slot = [&](int i) { return (uint32_t)((i % kSt) * kTB) >> 4; };
+      auto slot = [&](int i) { return (uint32_t)((i % kSt) * kYB) >> 4; };
       auto there = [&](int i) { return ptx::mbar_wait(full(i % kSt), (i / kSt) & 1, abort_flag); };
       auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {   // each half of the columns has its parts at its own start
-        mma_weigh<DP, kParts>(acc, w, 32, d_yt + y, id_a, more);
-        mma_weigh<DP, kParts>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
+        mma_weigh<DP, kParts, kY>(acc, w, 32, d_yt + y, id_a, more);
+        if constexpr (kY == 128) mma_weigh<DP, kParts, kY>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
       };
       auto run = [&]() {
         if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
         ptx::tc_fence_after();
-        mma_scores<DP, kParts>(tS, d_x, d_y + slot(0), id_s, ksteps);
+        mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(0), id_s, ksteps);
         ptx::umma_commit(s_full);
         if (!there(1)) return;
-        mma_scores<DP, kParts>(tD, d_x + (kTB >> 4), d_y + slot(1), id_s, ksteps);
+        mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(1), id_s, ksteps);
         ptx::umma_commit(dp_full);
         if (!kKeys) ptx::umma_commit(empty(1));
         for (int i = 0; i < n; ++i) {
@@ -194,7 +206,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           if (more) {
             if (!there(y1 + 2)) return;
-            mma_scores<DP, kParts>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
+            mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
           }
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
@@ -203,7 +215,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           ptx::umma_commit(empty(y1 % kSt));
           if (more) {
             if (!there(y2 + 2)) return;
-            mma_scores<DP, kParts>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
+            mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
             if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
           }
@@ -214,7 +226,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       drain(done, 0);
     }
   } else {
-    registers_up();
+    if constexpr (kY == 64) registers_up_4();
+    else registers_up();
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, xi = x0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tS + 64 * half + lanes, d_at = tD + 64 * half + lanes;
@@ -241,8 +254,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_ready);
       }
-      const int valid = kKeys ? kRows : len - y_row(i0 + i);   // columns from there on are masked
-      const bool ragged = valid < kRows;
+      const int valid = kKeys ? kY : len - y_row(i0 + i);   // columns from there on are masked
+      const bool ragged = valid < kY;
       const float* ly = kKeys ? &rows_of_y[(2 * i % kSt) >> 1][0][64 * half] : nullptr;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -286,7 +299,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           float4 d4 = make_float4(delta, delta, delta, delta);
-          if constexpr (kKeys) d4 = *reinterpret_cast<const float4*>(ly + kRows + 32 * k + e);
+          if constexpr (kKeys) d4 = *reinterpret_cast<const float4*>(ly + kY + 32 * k + e);
           const F2 dv[2] = {f2(-d4.x, -d4.y), f2(-d4.z, -d4.w)};
           float v[4];
 #pragma unroll
@@ -321,35 +334,43 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       ptx::tc_fence_after();
     }
     if (ok) {
-      // keys: the first four warps write grad_v, the others grad_k; queries: a half of the channels each
+      // keys: grad_v and grad_k, by four warps each or one after the other; queries: all channels, or half of them
       const int there = kKeys ? p.Lk : p.Lq;
       const long long rows = (long long)p.B * there * heads, out = ((long long)b * there + xi) * heads + head;
-      const bool first = kKeys && half == 0;
-      // grad_v: P 2^kUp and grad_o; dS and the other factor
-      const float mul = first ? exp2f(-kUp - (float)e_g) : p.scale * exp2f((float)-e_ds) * exp2f((float)-(kKeys ? e_q : e_k));
-      const uint32_t acc = (first ? tA1 : tA2) + lanes;
-      Out* dst = reinterpret_cast<Out*>(first ? p.g1 : p.g2) + out * p.D;
-      float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
-      const int c_end = kKeys ? p.D : min(p.D, (half + 1) * (DP / 2));
-      for (int c0 = kKeys ? 0 : half * (DP / 2); c0 < c_end; c0 += 32) {
-        uint32_t r[32];
-        if (n > 0) {
-          ptx::tmem_ld_32x32(acc + c0, r);
-          ptx::tmem_ld_wait();
-        } else {
+      auto write = [&](bool first, int c0, int c_end) {
+        // grad_v: P 2^kUp and grad_o; dS and the other factor
+        const float mul = first ? exp2f(-kUp - (float)e_g) : p.scale * exp2f((float)-e_ds) * exp2f((float)-(kKeys ? e_q : e_k));
+        const uint32_t acc = (first ? tA1 : tA2) + lanes;
+        Out* dst = reinterpret_cast<Out*>(first ? p.g1 : p.g2) + out * p.D;
+        float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
+        for (; c0 < c_end; c0 += 32) {
+          uint32_t r[32];
+          if (n > 0) {
+            ptx::tmem_ld_32x32(acc + c0, r);
+            ptx::tmem_ld_wait();
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = 0u;
+            for (int e = 0; e < 32; ++e) r[e] = 0u;
+          }
+          if (xi >= there) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (c0 + e >= c_end) break;
+            float f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(r[e + u]) * mul;
+            if (part) store8(part + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
+            else store8(dst + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
+          }
         }
-        if (xi >= there) continue;
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (c0 + e >= c_end) break;
-          float f[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(r[e + u]) * mul;
-          if (part) store8(part + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
-          else store8(dst + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
-        }
+      };
+      if (kY == 64) {
+        if (kKeys) write(true, 0, p.D);
+        write(false, 0, p.D);
+      } else if (kKeys) {
+        write(half == 0, 0, p.D);
+      } else {
+        write(false, half * (DP / 2), min(p.D, (half + 1) * (DP / 2)));
       }
     }
     ptx::tc_fence_before();
@@ -358,7 +379,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   report(p.status, abort_flag);
   if (warp == kMmaWarp) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, 512);
+    ptx::tmem_dealloc(tmem, kCols);
   }
 }
 
@@ -368,7 +389,7 @@ int launch(const CUtensorMap (&m)[4], const BwdParams& p, cudaStream_t st) {
   if (blocks > 0x7fffffffLL) return D2C_ERR_TOO_LARGE;
   constexpr int smem = kSmem<DP, kParts>;
   if (const int rc = allow_dynamic_smem<bwd_tc_kernel<T, Out, DP, kParts, kKeys>>(smem)) return rc;
-  bwd_tc_kernel<T, Out, DP, kParts, kKeys><<<(unsigned)blocks, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], p);
+  bwd_tc_kernel<T, Out, DP, kParts, kKeys><<<(unsigned)blocks, kThreads<DP, kParts>, smem, st>>>(m[0], m[1], m[2], m[3], p);
   D2C_LAUNCH_CHECK();
   return D2C_OK;
 }
@@ -391,10 +412,12 @@ int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys
   int rc;
   const bool staged = dtype == D2C_F32;
   if (staged) dtype = parts == 2 ? D2C_F16 : D2C_BF16;
-  if ((rc = tile_map(&q, x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
-  if ((rc = tile_map(&k, x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
-  if ((rc = tile_map(&v, x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts))) return rc;
-  if ((rc = tile_map(&g, x[3], dtype, p.width, a.Hq, a.Lq, a.B * parts))) return rc;
+  const int y_rows = parts == 1 && p.width <= 64 ? 64 : 128;            // kYRows
+  const int q_rows = keys ? y_rows : kRows, k_rows = keys ? kRows : y_rows;
+  if ((rc = tile_map(&q, x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts, q_rows))) return rc;
+  if ((rc = tile_map(&k, x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts, k_rows))) return rc;
+  if ((rc = tile_map(&v, x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts, k_rows))) return rc;
+  if ((rc = tile_map(&g, x[3], dtype, p.width, a.Hq, a.Lq, a.B * parts, q_rows))) return rc;
   const CUtensorMap maps[4] = {keys ? k : q, keys ? v : g, keys ? q : k, keys ? g : v};
   p.c = a.scale * kLog2e; p.scale = a.scale;
   p.splits = a.splits;

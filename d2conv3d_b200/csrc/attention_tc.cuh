@@ -25,28 +25,28 @@ constexpr int kTileBytes = kHalfBytes * (DP / 64);
 // whose products hi hi + lo hi + hi lo keep 22 bits of each factor, with 2^e from the largest element of the clip and key head, so that
 // neither type's range matters; or in one, bf16.  The parts are the outer half of a tensor map's clips.
 //
-// One box of 64 channels x 1 head x 128 tokens x 1 clip; what lies outside the tensor arrives as zeros.  x is 0 or 64.
+// One box of 64 channels x 1 head x 128 (R) tokens x 1 clip; what lies outside the tensor arrives as zeros.  x is 0 or 64.
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, int clip, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(token), "r"(clip), "r"(bar)
                : "memory");
 }
-template <int DP, int kParts>
+template <int DP, int kParts, int R = kRows>
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int head, int token, int clip, int clips, uint32_t bar) {
 #pragma unroll
   for (int part = 0; part < kParts; ++part)
 #pragma unroll
     for (int h = 0; h < DP / 64; ++h)
-      tma_box(dst + part * kTileBytes<DP> + h * kHalfBytes, map, h * 64, head, token, part * clips + clip, bar);
+      tma_box(dst + (part * DP / 64 + h) * R * 128, map, h * 64, head, token, part * clips + clip, bar);
 }
 
-// Zeroes rows [from, 128) of a tile (one warp).
-template <int DP, int kParts>
+// Zeroes rows [from, R) of a tile of R rows (one warp).
+template <int DP, int kParts, int R = kRows>
 __device__ __forceinline__ void clear_rows(uint32_t tile, int from) {
   const int lane = threadIdx.x & 31;
-  for (int i = from * 8 + lane; i < kRows * 8; i += 32) {        // 16-byte pieces: the swizzle stays inside a row
+  for (int i = from * 8 + lane; i < R * 8; i += 32) {            // 16-byte pieces: the swizzle stays inside a row
 #pragma unroll
-    for (int h = 0; h < kParts * DP / 64; ++h) ptx::sts_v4(tile + h * kHalfBytes + i * 16, make_uint4(0u, 0u, 0u, 0u));
+    for (int h = 0; h < kParts * DP / 64; ++h) ptx::sts_v4(tile + h * R * 128 + i * 16, make_uint4(0u, 0u, 0u, 0u));
   }
 }
 
@@ -92,26 +92,27 @@ __device__ __forceinline__ bool elect_one() {
 // Operand descriptors are formed once per buffer; tiles, halves and steps are constant distances (in 16 bytes) on the address field:
 // with a descriptor built for each product in a rolled loop, the products issued 200 clocks apart instead of their 64.
 //
-// D (128 x 128) = X Y^T over the channels, both K-major (descriptors of the first part's first step); ksteps = channels / 16 rounded up
+// D (128 x RY) = X Y^T over the channels, both K-major (descriptors of the first part's first step); ksteps = channels / 16 rounded up
 // (zero-filled above D).
-template <int DP, int kParts>
+template <int DP, int kParts, int RY = kRows>
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint64_t x, uint64_t y, uint32_t idesc, int ksteps) {
 #pragma unroll
   for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
-    const uint32_t xp = pass == 1 ? kTileBytes<DP> >> 4 : 0, yp = pass == 2 ? kTileBytes<DP> >> 4 : 0;
+    const uint32_t xp = pass == 1 ? kTileBytes<DP> >> 4 : 0, yp = pass == 2 ? RY * DP * 2 >> 4 : 0;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-      const uint32_t at = (uint32_t)((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-      if (k < ksteps) ptx::umma_bf16(d_tmem, x + (xp + at), y + (yp + at), idesc, pass > 0 || k > 0);
+      const uint32_t in = (k & 3) * 2, h = k >> 2;
+      if (k < ksteps)
+        ptx::umma_bf16(d_tmem, x + (xp + in + h * (kHalfBytes >> 4)), y + (yp + in + h * (RY * 128 >> 4)), idesc, pass > 0 || k > 0);
     }
   }
 }
 // D (128 x N) (+)= A Y, A 128 x 64 in tensor memory (32 columns; its lo part `lo` columns further), 64 rows of Y, MN-major, the reduction.
-template <int DP, int kParts>
+template <int DP, int kParts, int RY = kRows>
 __device__ __forceinline__ void mma_weigh(uint32_t d_tmem, uint32_t a_tmem, int lo, uint64_t y, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
-    const uint32_t ap = a_tmem + (pass == 1 ? lo : 0), yp = pass == 2 ? kTileBytes<DP> >> 4 : 0;
+    const uint32_t ap = a_tmem + (pass == 1 ? lo : 0), yp = pass == 2 ? RY * DP * 2 >> 4 : 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) umma_ts(d_tmem, ap + 8 * k, y + (yp + 128 * k), idesc, accumulate || pass > 0 || k > 0);
   }
@@ -165,6 +166,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // (8 * 208 + 4 * 80 <= 12 * 168).  Executed by every warp of a group of four.
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+// The same for a block of 8 warps launched with 128 registers a thread (two blocks a SM): 4 * 184 + 4 * 72 = 8 * 128.
+__device__ __forceinline__ void registers_up_4() { asm volatile("setmaxnreg.inc.sync.aligned.u32 184;"); }
+__device__ __forceinline__ void registers_down_4() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
 // Pairs of floats: one instruction for two operations.
 using F2 = unsigned long long;
@@ -212,7 +216,7 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
 
 // attention_sm100.cu: host helpers
 int status_pointer(int** out);
-int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips);
+int tile_map(CUtensorMap* map, const Operand& o, int dtype, int D, int heads, int tokens, int clips, int rows = kRows);
 
 }  // namespace attn
 }  // namespace d2c
