@@ -139,7 +139,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         for (int j = 0; j < n; ++j) {
           const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % kStages, sk = ik % kStages;
           const bool more = j + 1 < n;
-          if (!ptx::mbar_wait(full(sv), (iv / kStages) & 1, abort_flag)) return;
+          if (!ptx::mbar_wait(full(sv), (iv / kStages) & 1, abort_flag)) return;      // what is there long before p
+          if (more && !ptx::mbar_wait(full(sk), (ik / kStages) & 1, abort_flag)) return;
           for (int t = 0; t < nt; ++t) {
             for (int h = 0; h < 2; ++h) {         // the first half of the keys while the second's p is formed
               if (!ptx::mbar_wait(p_ready(t, h), j & 1, abort_flag)) return;
@@ -147,7 +148,6 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
               mma_weigh<DP, kParts>(tO + DP * t, tS + 128 * t + 32 * h, 64, d_v + (sv * kTB >> 4) + 512 * h, id_o, j > 0 || h > 0);
             }
             if (more) {
-              if (t == 0 && !ptx::mbar_wait(full(sk), (ik / kStages) & 1, abort_flag)) return;
               mma_scores<DP, kParts>(tS + 128 * t, d_q + (t * kTB >> 4), d_k + (sk * kTB >> 4), id_s, ksteps);
             }
             ptx::umma_commit(s_full(t));          // after the last tile: O_t is complete

@@ -198,27 +198,24 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (int i = 0; i < n; ++i) {
           const int y1 = 2 * i, y2 = y1 + 1;
           const bool more = i + 1 < n;
+          if (more && (!there(y1 + 2) || !there(y2 + 2))) return;         // what is there long before P
           if (!ptx::mbar_wait(p_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
-          if constexpr (kKeys) {
-            weigh(tA1, tS, slot(y2), i > 0);
-            ptx::umma_commit(empty(y2 % kSt));
-          }
+          if constexpr (kKeys) weigh(tA1, tS, slot(y2), i > 0);
           if (more) {
-            if (!there(y1 + 2)) return;
             mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
           }
+          if constexpr (kKeys) ptx::umma_commit(empty(y2 % kSt));
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
           weigh(tA2, tD, slot(y1), i > 0);
-          ptx::umma_commit(empty(y1 % kSt));
           if (more) {
-            if (!there(y2 + 2)) return;
             mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
             if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
           }
+          ptx::umma_commit(empty(y1 % kSt));
         }
       };
       run();
@@ -237,7 +234,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       lse = p.lse[at] - kUp;
       delta = p.delta[at] * d_mul;
     }
-    const bool row_in = kKeys ? xi < len : true;
+    const bool row_in = kKeys ? xi < len : true, x_ragged = kKeys && x0 + kRows > len;
+    constexpr bool kZeroEach = kKeys && kParts == 2;   // keys that are not there value by value: at the end, both parts spill
     float c = p.c;
     if constexpr (kParts == 2) c = ldexpf(c, -e_q - e_k);
     const F2 c2 = f2(c, c);
@@ -268,7 +266,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           for (int u = 0; u < 4; u += 2) {
             float x, y;
             f2_split(fma2(f2(__uint_as_float(s[k][e + u]), __uint_as_float(s[k][e + u + 1])), c2, lv[u / 2]), x, y);
-            const bool out = kKeys && !row_in;
+            const bool out = kZeroEach && !row_in;
             s[k][e + u] = out ? 0u : __float_as_uint(exp2_fast(x));
             s[k][e + u + 1] = out ? 0u : __float_as_uint(exp2_fast(y));
           }
@@ -280,6 +278,10 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           const float x = __uint_as_float(s[e >> 4][2 * e & 31]), y = __uint_as_float(s[e >> 4][(2 * e & 31) + 1]);
           w[e] = pack2<T>(x, y);
           if constexpr (kParts == 2) rest[e] = pack2_rest(x, y, w[e]);
+        }
+        if (!kZeroEach && x_ragged && !row_in) {  // keys that are not there: whatever S is
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w[e] = 0u;
         }
         tmem_st_32x32(s_at, w);
         if constexpr (kParts == 2) tmem_st_32x32(s_at + 32, rest);
@@ -309,10 +311,15 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
                               kHalf ? fma2(dp, f2(dp_mul, dp_mul), dv[u / 2]) : add2(dp, dv[u / 2]));
             f2_split(t, v[u], v[u + 1]);
           }
-          if (kKeys ? !row_in : ragged) {
+          if constexpr (kZeroEach) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              if (kKeys || 64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
+              if (!row_in) v[u] = 0.f;
+          }
+          if (!kKeys && ragged) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (64 * half + 32 * k + e + u >= valid) v[u] = 0.f;
           }
           w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
           w[16 * k + e / 2 + 1] = pack2<T>(v[2], v[3]);
@@ -321,6 +328,10 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             rest[16 * k + e / 2 + 1] = pack2_rest(v[2], v[3], w[16 * k + e / 2 + 1]);
           }
         }
+      }
+      if (kKeys && !kZeroEach && x_ragged && !row_in) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = 0u;
       }
       tmem_st_32x32(d_at, w);
       if constexpr (kParts == 2) tmem_st_32x32(d_at + 32, rest);
