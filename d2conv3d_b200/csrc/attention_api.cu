@@ -96,7 +96,7 @@ Plan plan_fwd(const d2c_attention_desc& d, int mode, bool aligned, int sms) {
   const long long rows = (long long)d.q_heads / d.kv_heads * d.queries;
   if (rows <= 16 && few_fits(d) && aligned) {
     const long long blocks = (long long)ceil_div(rows, kFewRows) * d.kv_heads * d.batch;
-    return {Path::few, std::max(1, std::min({ceil_div(4LL * sms, blocks), ceil_div(d.keys, 128), 128})), 0};
+    return {Path::few, std::max(1, std::min({ceil_div(2LL * sms, blocks), ceil_div(d.keys, 256), 128})), 0};
   }
   const int parts = tensor_parts(d, mode, aligned, false);
   const bool two_tiles = parts > 0 && !(parts == 2 && d.dim > 64);

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kv_kernel(Args a) {
 // R query rows (heads that share keys, times queries) against a share of the keys, which are read once.  LPK lanes hold a key's
 // channels, 16 bytes each; every such group of lanes runs a softmax of its own over every (32 / LPK * 4)-th key, four keys at a
 // time so that eight 16-byte loads are in flight; the groups meet in shared memory.  Bound by HBM where the GPU is filled.
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 256;
 template <typename T, int LPK, int R>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
   constexpr int V = 16 / (int)sizeof(T), kGroups = kFewThreads / LPK, kU = 4;
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Args a) {
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float shift = m == -INFINITY ? 0.f : m;
   float acc[4] = {}, sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = first; s < a.splits; s += W) {
     const float f = exp2f(a.part_lse[s * rows + row] - shift);
     const float* p = a.part + (s * rows + row) * a.D;

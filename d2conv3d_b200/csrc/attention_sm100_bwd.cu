@@ -198,24 +198,27 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (int i = 0; i < n; ++i) {
           const int y1 = 2 * i, y2 = y1 + 1;
           const bool more = i + 1 < n;
-          if (more && (!there(y1 + 2) || !there(y2 + 2))) return;         // what is there long before P
+          if (more && !there(y1 + 2)) return;     // what is there long before P
           if (!ptx::mbar_wait(p_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
-          if constexpr (kKeys) weigh(tA1, tS, slot(y2), i > 0);
+          if constexpr (kKeys) {
+            weigh(tA1, tS, slot(y2), i > 0);
+            ptx::umma_commit(empty(y2 % kSt));    // before the next S: a short ring waits for this tile's place
+          }
           if (more) {
             mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
           }
-          if constexpr (kKeys) ptx::umma_commit(empty(y2 % kSt));
+          if (more && !there(y2 + 2)) return;
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
           weigh(tA2, tD, slot(y1), i > 0);
+          ptx::umma_commit(empty(y1 % kSt));
           if (more) {
             mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
             if (!kKeys) ptx::umma_commit(empty((y2 + 2) % kSt));
           }
-          ptx::umma_commit(empty(y1 % kSt));
         }
       };
       run();

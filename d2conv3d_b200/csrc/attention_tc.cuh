@@ -170,30 +170,6 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 __device__ __forceinline__ void registers_up_4() { asm volatile("setmaxnreg.inc.sync.aligned.u32 184;"); }
 __device__ __forceinline__ void registers_down_4() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
-// Pairs of floats: one instruction for two operations.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_split(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // Called by all threads at a kernel's end: reports a wait that gave up to the host.
 __device__ __forceinline__ void report(int* status, volatile int* abort_flag) {
   if (threadIdx.x == 0 && *abort_flag && status) {

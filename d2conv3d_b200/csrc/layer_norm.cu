@@ -309,6 +309,15 @@ struct Cell {
       return i ? __high2float(h) : __low2float(h);
     }
   }
+  // both positions (VV = 2)
+  __device__ __forceinline__ F2 get2() const {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return f2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u));
+    } else {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+      return f2(h.x, h.y);
+    }
+  }
   // v[0], v[1] rounded
   __device__ __forceinline__ void set(const float (&v)[VV]) {
     if constexpr (!kPair) {
@@ -366,6 +375,28 @@ struct RowPiece {
 // A tile is LV * VV neighbouring positions with all their channels: LV threads, of VV positions each, by groups of EPT
 // neighbouring channels.  A warp's access to one channel is a contiguous run of positions; a thread's channels of a position
 // are contiguous in a token row and move as 32-byte accesses, one full sector each, without a detour through shared memory.
+// Arithmetic goes by pairs of values (one instruction for two): the two positions of a channel (VV = 2), or two channels.
+template <typename T, int EPT, int VV>
+__device__ __forceinline__ F2 pair_of(const Cell<T, VV> (&v)[EPT], int i) {
+  if constexpr (VV == 2) return v[i].get2();
+  else return f2(v[2 * i].get(0), v[2 * i + 1].get(0));
+}
+template <int VV>
+__device__ __forceinline__ F2 param_pair(const float (&w)[4], int i) {     // i-th pair of four channels (VV = 2: of 4 pairs, else of 2)
+  if constexpr (VV == 2) return f2(w[i], w[i]);
+  else return f2(w[2 * i], w[2 * i + 1]);
+}
+// One value a position of the thread from a pair's two halves.
+template <int VV>
+__device__ __forceinline__ void per_position(F2 v, float (&out)[VV]) {
+  float a, b;
+  f2_split(v, a, b);
+  if constexpr (VV == 2) { out[0] = a; out[1] = b; }
+  else out[0] = a + b;
+}
+template <int VV>
+__device__ __forceinline__ F2 both(const float (&v)[VV]) { return f2(v[0], v[VV - 1]); }
+
 // EPT channels of a thread's positions, `stride` apart; what is not there is zero.
 template <typename T, int EPT, int VV>
 __device__ __forceinline__ void load_cells(Cell<T, VV> (&v)[EPT], const T* p, long long stride, bool live, bool whole, int n) {
@@ -414,19 +445,36 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
     if constexpr (!kBackward) {
       // mean and sum of squares around it, of each thread's channels; merged: the squares of the means' distances come in too
       const float inv = n ? 1.f / (float)n : 0.f;
+      constexpr int kPairs = EPT * VV / 2;
+      F2 total = 0ull;
 #pragma unroll
-      for (int i = 0; i < VV; ++i) {
-        float m = 0.f, q = 0.f;
+      for (int i = 0; i < kPairs; ++i) total = add2(total, pair_of<T, EPT, VV>(xv, i));
+      float m[VV], q[VV];
+      per_position<VV>(total, m);
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) m += xv[e].get(i);
-        m *= inv;
+      for (int i = 0; i < VV; ++i) m[i] *= inv;
+      if (whole) {
+        F2 sq = 0ull;
+        const F2 off = f2(-m[0], -m[VV - 1]);
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) {
-          const float d = xv[e].get(i) - m;
-          if (whole || e < n) q = fmaf(d, d, q);
+        for (int i = 0; i < kPairs; ++i) {
+          const F2 d = add2(pair_of<T, EPT, VV>(xv, i), off);
+          sq = fma2(d, d, sq);
         }
-        slot[grp * kTile + lv * VV + i] = make_float2(m, q);
+        per_position<VV>(sq, q);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VV; ++i) {
+          q[i] = 0.f;
+#pragma unroll
+          for (int e = 0; e < EPT; ++e) {
+            const float d = xv[e].get(i) - m[i];
+            if (e < n) q[i] = fmaf(d, d, q[i]);
+          }
+        }
       }
+#pragma unroll
+      for (int i = 0; i < VV; ++i) slot[grp * kTile + lv * VV + i] = make_float2(m[i], q[i]);
       __syncthreads();
       float mean[VV], rstd[VV];
 #pragma unroll
@@ -446,26 +494,37 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
         if (live && a.stats && grp == 0) a.stats[b * a.V + p + i] = make_float2(m, rstd[i]);
       }
       if (live) {
+        const F2 off = f2(-mean[0], -mean[VV - 1]), mul = both<VV>(rstd);
+        constexpr int kStep = 4 * VV / 2;                                 // pairs of four channels
         if constexpr (kTokens) {
 #pragma unroll
           for (int e0 = 0; e0 < EPT; e0 += kW) {
-            float w[kW], bb[kW];
-            params_at<kW>(wb + c0 + e0, w);
-            params_at<kW>(wb + cpad + c0 + e0, bb);
+            float f[VV][kW];
+#pragma unroll
+            for (int e1 = 0; e1 < kW; e1 += 4) {
+              float w[4], bb[4];
+              params_at<4>(wb + c0 + e0 + e1, w);
+              params_at<4>(wb + cpad + c0 + e0 + e1, bb);
+#pragma unroll
+              for (int k = 0; k < kStep; ++k) {
+                const F2 h = mul2(add2(pair_of<T, EPT, VV>(xv, (e0 + e1) * VV / 2 + k), off), mul);
+                const F2 y2 = fma2(h, param_pair<VV>(w, k), param_pair<VV>(bb, k));
+                if constexpr (VV == 2) f2_split(y2, f[0][e1 + k], f[VV - 1][e1 + k]);
+                else f2_split(y2, f[0][e1 + 2 * k], f[0][e1 + 2 * k + 1]);
+              }
+            }
 #pragma unroll
             for (int i = 0; i < VV; ++i) {
               T* y = reinterpret_cast<T*>(a.y) + tok + (long long)i * C + e0;
               RowPiece<T, kW> o;
 #pragma unroll
               for (int k = 0; k < RowPiece<T, kW>::kWords; ++k) {
-                float f[4 / sizeof(T)];
+                constexpr int kPer = 4 / (int)sizeof(T);
+                float pair[kPer];
 #pragma unroll
-                for (int j = 0; j < 4 / (int)sizeof(T); ++j) {
-                  const int e = k * (4 / (int)sizeof(T)) + j;
-                  f[j] = fmaf((xv[e0 + e].get(i) - mean[i]) * rstd[i], w[e], bb[e]);
-                }
-                Cell<T, 4 / sizeof(T)> c;
-                c.set(f);
+                for (int j = 0; j < kPer; ++j) pair[j] = f[i][k * kPer + j];
+                Cell<T, kPer> c;
+                c.set(pair);
                 o.w[k] = *reinterpret_cast<const uint32_t*>(&c.raw);
               }
               if (!a.vec_tokens) o.store(y, n - e0);
@@ -476,16 +535,20 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
           T* y = reinterpret_cast<T*>(a.y) + vol;
 #pragma unroll
           for (int e0 = 0; e0 < EPT; e0 += 4) {
-            float w[4], bb[4];
+            float w[4], bb[4], f[4][VV];
             params_at<4>(wb + c0 + e0, w);
             params_at<4>(wb + cpad + c0 + e0, bb);
 #pragma unroll
-            for (int k = 0; k < 4; ++k, y += a.V) {
-              float f[VV];
+            for (int k = 0; k < kStep; ++k) {
+              const F2 h = mul2(add2(pair_of<T, EPT, VV>(xv, e0 * VV / 2 + k), off), mul);
+              const F2 y2 = fma2(h, param_pair<VV>(w, k), param_pair<VV>(bb, k));
+              if constexpr (VV == 2) f2_split(y2, f[k][0], f[k][VV - 1]);
+              else f2_split(y2, f[2 * k][0], f[2 * k + 1][0]);
+            }
 #pragma unroll
-              for (int i = 0; i < VV; ++i) f[i] = fmaf((xv[e0 + k].get(i) - mean[i]) * rstd[i], w[k], bb[k]);
+            for (int k = 0; k < 4; ++k, y += a.V) {
               Cell<T, VV> o;
-              o.set(f);
+              o.set(f[k]);
               if (whole || e0 + k < n) o.store(y);
             }
           }
@@ -520,35 +583,49 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
         const T* g = reinterpret_cast<const T*>(a.g) + vol;
         load_cells<T, EPT, VV>(gv, g, a.V, live, whole, n);
       }
-      float2 st[VV];
+      float mean[VV], rstd[VV];
 #pragma unroll
       for (int i = 0; i < VV; ++i) {
-        st[i] = live ? a.stats[b * a.V + p + i] : make_float2(0.f, 0.f);
-        float s1 = 0.f, s2 = 0.f;
+        const float2 st = live ? a.stats[b * a.V + p + i] : make_float2(0.f, 0.f);
+        mean[i] = st.x;
+        rstd[i] = st.y;
+      }
+      const F2 off = f2(-mean[0], -mean[VV - 1]), mul = both<VV>(rstd);
+      constexpr int kStep = 4 * VV / 2;                                   // pairs of four channels
+      {
+        F2 s1 = 0ull, s2 = 0ull;
 #pragma unroll
         for (int e0 = 0; e0 < EPT; e0 += 4) {
           float w[4];
           params_at<4>(wb + c0 + e0, w);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {                                   // channels that are not there: g = w = 0
-            const float gw = gv[e0 + k].get(i) * w[k];
-            s1 += gw;
-            s2 = fmaf(gw, (xv[e0 + k].get(i) - st[i].x) * st[i].y, s2);
+          for (int k = 0; k < kStep; ++k) {                               // channels that are not there: g = w = 0
+            const int i = e0 * VV / 2 + k;
+            const F2 gw = mul2(pair_of<T, EPT, VV>(gv, i), param_pair<VV>(w, k));
+            s1 = add2(s1, gw);
+            s2 = fma2(gw, mul2(add2(pair_of<T, EPT, VV>(xv, i), off), mul), s2);
           }
         }
-        slot[grp * kTile + lv * VV + i] = make_float2(s1, s2);
+        float t1[VV], t2[VV];
+        per_position<VV>(s1, t1);
+        per_position<VV>(s2, t2);
+#pragma unroll
+        for (int i = 0; i < VV; ++i) slot[grp * kTile + lv * VV + i] = make_float2(t1[i], t2[i]);
       }
       if (a.partial) {
         float v[EPT];
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
 #pragma unroll
-          for (int e = 0; e < EPT; ++e) {
-            v[e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < VV; ++i) {
-              const float gg = gv[e].get(i);
-              v[e] += part ? gg : gg * ((xv[e].get(i) - st[i].x) * st[i].y);
+          for (int i = 0; i < EPT * VV / 2; ++i) {
+            const F2 g2 = pair_of<T, EPT, VV>(gv, i);
+            const F2 t = part ? g2 : mul2(g2, mul2(add2(pair_of<T, EPT, VV>(xv, i), off), mul));
+            if constexpr (VV == 2) {
+              float sum[1];
+              per_position<1>(t, sum);
+              v[i] = sum[0];
+            } else {
+              f2_split(t, v[2 * i], v[2 * i + 1]);
             }
           }
           spread_sum<EPT, LV>(v);
@@ -567,24 +644,27 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
             s1 += s.x;
             s2 += s.y;
           }
-          m1[i] = s1 / (float)C;
-          m2[i] = s2 / (float)C;
+          m1[i] = -s1 / (float)C;
+          m2[i] = -s2 / (float)C;
         }
+        const F2 n1 = both<VV>(m1), n2 = both<VV>(m2);
         T* gx = reinterpret_cast<T*>(a.y) + vol;
 #pragma unroll
         for (int e0 = 0; e0 < EPT; e0 += 4) {
-          float w[4];
+          float w[4], f[4][VV];
           params_at<4>(wb + c0 + e0, w);
 #pragma unroll
-          for (int k = 0; k < 4; ++k, gx += a.V) {
-            float f[VV];
+          for (int k = 0; k < kStep; ++k) {
+            const int i = e0 * VV / 2 + k;
+            const F2 h = mul2(add2(pair_of<T, EPT, VV>(xv, i), off), mul);
+            const F2 r = mul2(fma2(h, n2, fma2(pair_of<T, EPT, VV>(gv, i), param_pair<VV>(w, k), n1)), mul);
+            if constexpr (VV == 2) f2_split(r, f[k][0], f[k][VV - 1]);
+            else f2_split(r, f[2 * k][0], f[2 * k + 1][0]);
+          }
 #pragma unroll
-            for (int i = 0; i < VV; ++i) {
-              const float h = (xv[e0 + k].get(i) - st[i].x) * st[i].y;
-              f[i] = st[i].y * (fmaf(gv[e0 + k].get(i), w[k], -m1[i]) - h * m2[i]);
-            }
+          for (int k = 0; k < 4; ++k, gx += a.V) {
             Cell<T, VV> o;
-            o.set(f);
+            o.set(f[k]);
             if (live && (whole || e0 + k < n)) o.store(gx);
           }
         }
