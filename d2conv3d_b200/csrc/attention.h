@@ -46,7 +46,7 @@ int exact_bwd_q(int dtype, const Args& a, cudaStream_t st);
 int exact_bwd_kv(int dtype, const Args& a, cudaStream_t st);
 int combine(int dtype, const Args& a, cudaStream_t st);          // partial outputs -> o, lse
 int delta_rows(int dtype, const Args& a, cudaStream_t st);
-int sum_parts(int dtype, const float* part, int splits, long long n, void* out, cudaStream_t st);
+int sum_parts(int dtype, const float* part, int splits, long long n, void* out0, void* out1, cudaStream_t st);   // out1: NULL, or a second sum
 
 // ---- tensor cores: operands with positive strides and 16-byte rows, scale > 0
 struct Operand {

@@ -226,13 +226,11 @@ int run_bwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int 
   a.splits = pk.splits;
   if ((rc = tensor ? tc_bwd(d.dtype, a, x, pk.parts, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
   if (a.splits > 1) {
-    const long long n = kv_rows(d) * d.dim;
-    if ((rc = sum_parts(d.dtype, a.part, a.splits, n, a.gk, st))) return rc;
-    if ((rc = sum_parts(d.dtype, a.part + a.splits * n, a.splits, n, a.gv, st))) return rc;
+    if ((rc = sum_parts(d.dtype, a.part, a.splits, kv_rows(d) * d.dim, a.gk, a.gv, st))) return rc;
   }
   a.splits = pq.splits;
   if ((rc = tensor ? tc_bwd(d.dtype, a, x, pq.parts, false, bounds, st) : exact_bwd_q(d.dtype, a, st))) return rc;
-  if (a.splits > 1) return sum_parts(d.dtype, a.part, a.splits, q_rows(d) * d.dim, a.gq, st);
+  if (a.splits > 1) return sum_parts(d.dtype, a.part, a.splits, q_rows(d) * d.dim, a.gq, nullptr, st);
   return D2C_OK;
 }
 

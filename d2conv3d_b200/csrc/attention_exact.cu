@@ -540,8 +540,13 @@ __global__ void __launch_bounds__(256) delta_kernel(Args a) {
   if (lane == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + qi] = s;
 }
 
+// out[y] = sum of `splits` parts of n values each, part[y]'s one behind the other; y = blockIdx.y.  Launched beside the kernel that
+// writes the parts.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int splits, long long n, T* out) {
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int splits, long long n, T* out0, T* out1) {
+  wait_for_kernels_before();
+  T* out = blockIdx.y ? out1 : out0;
+  part += (long long)blockIdx.y * splits * n;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     float s = 0.f;
 #pragma unroll 4
@@ -663,15 +668,19 @@ int delta_rows(int dtype, const Args& a, cudaStream_t st) {
   return D2C_OK;
 }
 
-int sum_parts(int dtype, const float* part, int splits, long long n, void* out, cudaStream_t st) {
+template <typename T>
+static int sum_parts_typed(const float* part, int splits, long long n, void* out0, void* out1, cudaStream_t st) {
   const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 148 * 8);
-  switch (dtype) {
-    case D2C_F32: sum_parts_kernel<float><<<grid, 256, 0, st>>>(part, splits, n, (float*)out); break;
-    case D2C_F16: sum_parts_kernel<__half><<<grid, 256, 0, st>>>(part, splits, n, (__half*)out); break;
-    default: sum_parts_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(part, splits, n, (__nv_bfloat16*)out); break;
-  }
+  D2C_CUDA_TRY(launch_beside(sum_parts_kernel<T>, dim3(grid, out1 ? 2 : 1), dim3(256), 0, st, part, splits, n, (T*)out0, (T*)out1));
   D2C_LAUNCH_CHECK();
   return D2C_OK;
+}
+int sum_parts(int dtype, const float* part, int splits, long long n, void* out0, void* out1, cudaStream_t st) {
+  switch (dtype) {
+    case D2C_F32: return sum_parts_typed<float>(part, splits, n, out0, out1, st);
+    case D2C_F16: return sum_parts_typed<__half>(part, splits, n, out0, out1, st);
+    default: return sum_parts_typed<__nv_bfloat16>(part, splits, n, out0, out1, st);
+  }
 }
 
 }  // namespace attn

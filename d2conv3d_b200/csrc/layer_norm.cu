@@ -27,7 +27,7 @@ struct NormArgs {
   float* partial;              // [blocks][2][C]: sums for grad_w, grad_b of one block; NULL if neither is asked for
   float eps;
   int param_f32;               // w and b are fp32 (otherwise of x's type)
-  int vec_tokens;              // token rows can be moved 32 bytes (fewer where a thread holds fewer) at a time
+  int vec_tokens;              // token rows are whole vectors, of 32 bytes (fewer where a thread holds fewer)
 };
 
 template <typename T>
@@ -59,6 +59,34 @@ __device__ __forceinline__ void params_at(const float* p, float (&f)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = p[e];
   }
+}
+
+// VEC neighbouring values as pairs (one instruction for two operations), where there are pairs.
+template <typename T, int VEC>
+__device__ __forceinline__ F2 value_pair(const Vec<T, VEC>& v, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return f2(v.v[2 * i], v.v[2 * i + 1]);
+  } else {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[i];
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      return f2(h.x, h.y);
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void set_pair(Vec<T, VEC>& v, int i, F2 f) {
+  float a, b;
+  f2_split(f, a, b);
+  v.v[2 * i] = from_f32<T>(a);
+  v.v[2 * i + 1] = from_f32<T>(b);
+}
+__device__ __forceinline__ float both_halves(F2 f) {
+  float a, b;
+  f2_split(f, a, b);
+  return a + b;
 }
 
 // ---- token rows -------------------------------------------------------------------------------------------
@@ -109,28 +137,42 @@ __global__ void __launch_bounds__(256) norm_rows_fwd_kernel(NormArgs a) {
     for (int k = 0; k < kChunks; ++k) v[k] = next[k];
     ask(row + step, next);
     float s = 0.f, q = 0.f;
+    F2 acc = 0ull;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (live && c < C) {
+        if constexpr (VEC > 1) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s += to_f32(v[k].v[e]);
+          for (int i = 0; i < VEC / 2; ++i) acc = add2(acc, value_pair<T, VEC>(v[k], i));
+        } else {
+          s += to_f32(v[k].v[0]);
+        }
       }
     }
+    s += both_halves(acc);
     row_sum<TPR>(s, q, red);
     const float mean = s / (float)C;
+    const F2 off = f2(-mean, -mean);
     s = q = 0.f;
+    acc = 0ull;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
       if (live && c < C) {
+        if constexpr (VEC > 1) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = to_f32(v[k].v[e]) - mean;
+          for (int i = 0; i < VEC / 2; ++i) {
+            const F2 d = add2(value_pair<T, VEC>(v[k], i), off);
+            acc = fma2(d, d, acc);
+          }
+        } else {
+          const float d = to_f32(v[k].v[0]) - mean;
           q = fmaf(d, d, q);
         }
       }
     }
+    q += both_halves(acc);
     row_sum<TPR>(s, q, red);
     const float rstd = 1.f / sqrtf(q / (float)C + a.eps);
     if (!live) continue;                   // no barrier follows in a block of several rows; a block of one row is all live
@@ -144,8 +186,13 @@ __global__ void __launch_bounds__(256) norm_rows_fwd_kernel(NormArgs a) {
         params_at<VEC>(wb + c, w);
         params_at<VEC>(wb + cpad + c, b);
         Vec<T, VEC> o;
+        if constexpr (VEC > 1) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(fmaf((to_f32(v[k].v[e]) - mean) * rstd, w[e], b[e]));
+          for (int i = 0; i < VEC / 2; ++i)
+            set_pair<T, VEC>(o, i, fma2(mul2(add2(value_pair<T, VEC>(v[k], i), off), f2(rstd, rstd)), f2(w[2 * i], w[2 * i + 1]), f2(b[2 * i], b[2 * i + 1])));
+        } else {
+          o.v[0] = from_f32<T>(fmaf((to_f32(v[k].v[0]) - mean) * rstd, w[0], b[0]));
+        }
         store_vec<T, VEC>(y + c, o);
       }
     }
@@ -161,9 +208,10 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
   extern __shared__ __align__(16) float sums[];   // [kRows][C] at the end, w before
   const int t = threadIdx.x % TPR, C = a.C;
   const long long rows = a.V * a.batch, step = (long long)gridDim.x * kRows;
-  float aw[EPT], ab[EPT];
+  constexpr int kPair = VEC > 1 ? 2 : 1;   // sums of one channel, or of two in one register pair
+  F2 aw[EPT / kPair], ab[EPT / kPair];
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) aw[i] = ab[i] = 0.f;
+  for (int i = 0; i < EPT / kPair; ++i) aw[i] = ab[i] = 0ull;
   constexpr bool kAhead = EPT <= 16;       // the next rows are asked for before these are worked on, where registers allow
   Vec<T, VEC> xv[kChunks], gv[kChunks], xn[kAhead ? kChunks : 1], gn[kAhead ? kChunks : 1];
   float2 st, stn = make_float2(0.f, 0.f);
@@ -193,7 +241,9 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
     } else {
       ask(row, xv, gv, st);
     }
-    float s1 = 0.f, s2 = 0.f;
+    float s1, s2;
+    F2 p1 = 0ull, p2 = 0ull;
+    const F2 off = f2(-st.x, -st.x), mul = f2(st.y, st.y);
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = (k * TPR + t) * VEC;
@@ -201,16 +251,28 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
         float w[VEC];
         params_at<VEC>(sums + c, w);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = (to_f32(xv[k].v[e]) - st.x) * st.y, gg = to_f32(gv[k].v[e]);
-          const float gw = gg * w[e];
-          s1 += gw;
-          s2 = fmaf(gw, h, s2);
-          aw[k * VEC + e] = fmaf(gg, h, aw[k * VEC + e]);
-          ab[k * VEC + e] += gg;
+        for (int i = 0; i < VEC / kPair; ++i) {
+          const int at = k * (VEC / kPair) + i;
+          F2 x, gg, ww;
+          if constexpr (VEC > 1) {
+            x = value_pair<T, VEC>(xv[k], i);
+            gg = value_pair<T, VEC>(gv[k], i);
+            ww = f2(w[2 * i], w[2 * i + 1]);
+          } else {
+            x = f2(to_f32(xv[k].v[0]), st.x);
+            gg = f2(to_f32(gv[k].v[0]), 0.f);
+            ww = f2(w[0], 0.f);
+          }
+          const F2 h = mul2(add2(x, off), mul), gw = mul2(gg, ww);
+          p1 = add2(p1, gw);
+          p2 = fma2(gw, h, p2);
+          aw[at] = fma2(gg, h, aw[at]);
+          ab[at] = add2(ab[at], gg);
         }
       }
     }
+    s1 = both_halves(p1);
+    s2 = both_halves(p2);
     row_sum<TPR>(s1, s2, red);
     if (!live || !a.y) continue;           // see the forward
     s1 /= (float)C;
@@ -223,16 +285,27 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
         float w[VEC];
         params_at<VEC>(sums + c, w);
         Vec<T, VEC> o;
+        if constexpr (VEC > 1) {
+          const F2 n1 = f2(-s1, -s1), n2 = f2(-s2, -s2);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = (to_f32(xv[k].v[e]) - st.x) * st.y;
-          o.v[e] = from_f32<T>(st.y * (to_f32(gv[k].v[e]) * w[e] - s1 - h * s2));
+          for (int i = 0; i < VEC / 2; ++i) {
+            const F2 h = mul2(add2(value_pair<T, VEC>(xv[k], i), off), mul);
+            set_pair<T, VEC>(o, i, mul2(fma2(h, n2, fma2(value_pair<T, VEC>(gv[k], i), f2(w[2 * i], w[2 * i + 1]), n1)), mul));
+          }
+        } else {
+          const float h = (to_f32(xv[k].v[0]) - st.x) * st.y;
+          o.v[0] = from_f32<T>(st.y * (to_f32(gv[k].v[0]) * w[0] - s1 - h * s2));
         }
         store_vec<T, VEC>(gx + c, o);
       }
     }
   }
   if (!a.partial) return;
+  auto sum_of = [&](int part, int i) {
+    float u, v;
+    f2_split(part ? ab[i / kPair] : aw[i / kPair], u, v);
+    return kPair == 1 || i % 2 == 0 ? u : v;
+  };
   float* out = a.partial + (long long)blockIdx.x * 2 * C;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
@@ -240,14 +313,14 @@ __global__ void __launch_bounds__(256) norm_rows_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
         const int c = ((i / VEC) * TPR + t) * VEC + i % VEC;
-        if (c < C) out[part * C + c] = part ? ab[i] : aw[i];
+        if (c < C) out[part * C + c] = sum_of(part, i);
       }
     } else {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
         const int c = ((i / VEC) * TPR + t) * VEC + i % VEC;
-        if (c < C) sums[(threadIdx.x / TPR) * C + c] = part ? ab[i] : aw[i];
+        if (c < C) sums[(threadIdx.x / TPR) * C + c] = sum_of(part, i);
       }
       __syncthreads();
       for (int c = threadIdx.x; c < C; c += 256) {
@@ -336,10 +409,16 @@ template <typename T, int kW>
 struct RowPiece {
   static constexpr int kWords = kW * (int)sizeof(T) / 4;
   uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* p) {
-    const Vec<uint32_t, kWords> v = load_vec<uint32_t, kWords>(reinterpret_cast<const uint32_t*>(p));
+  __device__ __forceinline__ void get(const uint8_t* p) {             // from shared memory
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = v.v[i];
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+      w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   }
   __device__ __forceinline__ void load(const T* p, int n) {          // the first n channels, element by element
 #pragma unroll
@@ -351,12 +430,6 @@ struct RowPiece {
         w[i] = (2 * i < n ? q[2 * i] : 0u) | ((uint32_t)(2 * i + 1 < n ? q[2 * i + 1] : 0u) << 16);
       }
     }
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    Vec<uint32_t, kWords> v;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) v.v[i] = w[i];
-    store_vec<uint32_t, kWords>(reinterpret_cast<uint32_t*>(p), v);
   }
   __device__ __forceinline__ void store(T* p, int n) const {
 #pragma unroll
@@ -373,8 +446,9 @@ struct RowPiece {
 };
 
 // A tile is LV * VV neighbouring positions with all their channels: LV threads, of VV positions each, by groups of EPT
-// neighbouring channels.  A warp's access to one channel is a contiguous run of positions; a thread's channels of a position
-// are contiguous in a token row and move as 32-byte accesses, one full sector each, without a detour through shared memory.
+// neighbouring channels.  A warp's access to one channel is a contiguous run of positions.  Token rows pass through shared memory, where a
+// warp moves whole rows (each lane its own 32 bytes of a row, straight from registers: 46 instead of 31 us for 25920 rows of 1024 in
+// bf16); rows whose channels are not whole vectors move element by element.
 // Arithmetic goes by pairs of values (one instruction for two): the two positions of a channel (VV = 2), or two channels.
 template <typename T, int EPT, int VV>
 __device__ __forceinline__ F2 pair_of(const Cell<T, VV> (&v)[EPT], int i) {
@@ -419,6 +493,8 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
   float* wb = shared;                                                     // [2][C rounded up to whole groups]
   const int cpad = groups * EPT;
   float2* red = reinterpret_cast<float2*>(wb + 2 * cpad);                 // [2][groups][LV * VV]
+  uint8_t* rows = reinterpret_cast<uint8_t*>(red + 2 * groups * LV * VV); // token rows of a tile, 16 bytes apart from a whole power of two
+  const int pitch = C * (int)sizeof(T) + 16;
   stage_params<T>(a, wb, kBackward ? nullptr : wb + cpad, cpad);
   const int lv = threadIdx.x % LV, grp = threadIdx.x / LV, c0 = grp * EPT;
   const int n = min(max(C - c0, 0), EPT);                                 // channels that this thread has
@@ -430,8 +506,22 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
   // tile -> clip, place in it: divided once, then stepped
   const long long step_b = gridDim.x / tiles_b, step_t = gridDim.x % tiles_b;
   long long b = blockIdx.x / tiles_b, tb = blockIdx.x % tiles_b;
-  const int parts = (C + EPT - 1) / EPT, last = C - (parts - 1) * EPT;    // groups that have channels; of the last one
   const bool whole = n == EPT;
+  // groups of a warp meet in shuffles, warps in shared memory: 32 groups read one after the other took longer than the tile's loads
+  constexpr int kSteps = LV == 32 ? 0 : (LV == 16 ? 1 : 2), kOfWarp = 32 / LV * EPT;      // steps; channels of a warp
+  const int warps = (C + kOfWarp - 1) / kOfWarp, warp = threadIdx.x >> 5;                 // warps that have channels
+  float toward[kSteps + 1], apart[kSteps + 1];                            // of two groups' means: n_b / (n_a + n_b), n_a n_b / (n_a + n_b)
+  {
+    int na = n;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int nb = __shfl_xor_sync(0xffffffffu, na, LV << k);
+      const float inv = na + nb ? 1.f / (float)(na + nb) : 0.f;
+      toward[k] = (float)nb * inv;
+      apart[k] = (float)na * (float)nb * inv;
+      na += nb;
+    }
+  }
   int turn = 0;
   for (long long tile = blockIdx.x; tile < tiles;
        tile += gridDim.x, turn ^= 1, b += step_b, tb += step_t, b += tb >= tiles_b, tb -= tb >= tiles_b ? tiles_b : 0) {
@@ -439,6 +529,17 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
     const bool live = p < a.V;             // VV > 1 only where it divides V
     const long long vol = (b * C + c0) * a.V + p, tok = (b * a.V + p) * C + c0;
     const T* x = reinterpret_cast<const T*>(a.x) + vol;
+    if constexpr (kTokens && kBackward) {
+      if (a.vec_tokens) {                                                 // asked for before x
+        const T* g = reinterpret_cast<const T*>(a.g) + (b * a.V + tb * kTile) * C;
+        const int there = (int)min((long long)kTile, a.V - tb * kTile);
+        for (int r = threadIdx.x >> 5; r < there; r += blockDim.x >> 5)
+          for (int c = threadIdx.x & 31; c < pitch / 16 - 1; c += 32)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(rows + r * pitch + c * 16)),
+                         "l"(reinterpret_cast<const uint4*>(g + (long long)r * C) + c)
+                         : "memory");
+      }
+    }
     Cell<T, VV> xv[EPT];
     load_cells<T, EPT, VV>(xv, x, a.V, live, whole, n);
     float2* slot = red + turn * groups * kTile;    // the other half is still read by threads that are behind
@@ -474,21 +575,31 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
         }
       }
 #pragma unroll
-      for (int i = 0; i < VV; ++i) slot[grp * kTile + lv * VV + i] = make_float2(m[i], q[i]);
+      for (int i = 0; i < VV; ++i) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const float d = __shfl_xor_sync(0xffffffffu, m[i], LV << k) - m[i], oq = __shfl_xor_sync(0xffffffffu, q[i], LV << k);
+          m[i] = fmaf(d, toward[k], m[i]);
+          q[i] = fmaf(d * d, apart[k], q[i] + oq);
+        }
+        if ((threadIdx.x & 31) < LV) slot[warp * kTile + lv * VV + i] = make_float2(m[i], q[i]);
+      }
       __syncthreads();
       float mean[VV], rstd[VV];
 #pragma unroll
       for (int i = 0; i < VV; ++i) {
         float m = 0.f, q = 0.f;
-        for (int k = 0; k < parts - 1; ++k) m += slot[k * kTile + lv * VV + i].x;
-        const float2 end = slot[(parts - 1) * kTile + lv * VV + i];
-        m = (m * (float)EPT + end.x * (float)last) / (float)C;
-        for (int k = 0; k < parts - 1; ++k) {
-          const float2 s = slot[k * kTile + lv * VV + i];
+        const float2* all = slot + lv * VV + i;
+        auto count = [&](int w) { return (float)min(C - w * kOfWarp, kOfWarp); };
+#pragma unroll 4
+        for (int w = 0; w < warps; ++w) m = fmaf(all[w * kTile].x, count(w), m);
+        m /= (float)C;
+#pragma unroll 4
+        for (int w = 0; w < warps; ++w) {
+          const float2 s = all[w * kTile];
           const float d = s.x - m;
-          q = fmaf(d * (float)EPT, d, q) + s.y;
+          q = fmaf(d * count(w), d, q) + s.y;
         }
-        q = fmaf((end.x - m) * (float)last, end.x - m, q) + end.y;
         mean[i] = m;
         rstd[i] = 1.f / sqrtf(q / (float)C + a.eps);
         if (live && a.stats && grp == 0) a.stats[b * a.V + p + i] = make_float2(m, rstd[i]);
@@ -528,7 +639,7 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
                 o.w[k] = *reinterpret_cast<const uint32_t*>(&c.raw);
               }
               if (!a.vec_tokens) o.store(y, n - e0);
-              else if (e0 < n) o.store(y);
+              else if (e0 < n) o.put(rows + (lv * VV + i) * pitch + (c0 + e0) * (int)sizeof(T));
             }
           }
         } else {
@@ -554,17 +665,31 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
           }
         }
       }
+      if constexpr (kTokens) {
+        if (a.vec_tokens) {
+          __syncthreads();
+          T* y = reinterpret_cast<T*>(a.y) + (b * a.V + tb * kTile) * C;
+          const int there = (int)min((long long)kTile, a.V - tb * kTile);
+          for (int r = threadIdx.x >> 5; r < there; r += blockDim.x >> 5)
+            for (int c = threadIdx.x & 31; c < pitch / 16 - 1; c += 32)
+              reinterpret_cast<uint4*>(y + (long long)r * C)[c] = *reinterpret_cast<const uint4*>(rows + r * pitch + c * 16);
+        }
+      }
     } else {
       Cell<T, VV> gv[EPT];
       if constexpr (kTokens) {
         constexpr int kPer = 4 / (int)sizeof(T);                          // channels of a word
+        if (a.vec_tokens) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncthreads();
+        }
 #pragma unroll
         for (int e0 = 0; e0 < EPT; e0 += kW) {
           RowPiece<T, kW> o[VV];
 #pragma unroll
           for (int i = 0; i < VV; ++i) {
             const T* g = reinterpret_cast<const T*>(a.g) + tok + (long long)i * C + e0;
-            if (a.vec_tokens && live && e0 < n) o[i].load(g);
+            if (a.vec_tokens && live && e0 < n) o[i].get(rows + (lv * VV + i) * pitch + (c0 + e0) * (int)sizeof(T));
             else o[i].load(g, live ? n - e0 : 0);
           }
 #pragma unroll
@@ -610,7 +735,14 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
         per_position<VV>(s1, t1);
         per_position<VV>(s2, t2);
 #pragma unroll
-        for (int i = 0; i < VV; ++i) slot[grp * kTile + lv * VV + i] = make_float2(t1[i], t2[i]);
+        for (int i = 0; i < VV; ++i) {
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            t1[i] += __shfl_xor_sync(0xffffffffu, t1[i], LV << k);
+            t2[i] += __shfl_xor_sync(0xffffffffu, t2[i], LV << k);
+          }
+          if ((threadIdx.x & 31) < LV) slot[warp * kTile + lv * VV + i] = make_float2(t1[i], t2[i]);
+        }
       }
       if (a.partial) {
         float v[EPT];
@@ -639,8 +771,9 @@ __global__ void __launch_bounds__(512, kBackward || VV == 2 ? 1 : 2) norm_volume
 #pragma unroll
         for (int i = 0; i < VV; ++i) {
           float s1 = 0.f, s2 = 0.f;
-          for (int k = 0; k < parts; ++k) {
-            const float2 s = slot[k * kTile + lv * VV + i];
+#pragma unroll 4
+          for (int w = 0; w < warps; ++w) {
+            const float2 s = slot[w * kTile + lv * VV + i];
             s1 += s.x;
             s2 += s.y;
           }
@@ -836,6 +969,7 @@ Plan make_plan(const d2c_layer_norm_desc& d, bool backward, bool aligned, int sm
       p.path = Path::volume;
       const int g = p.threads / p.lv;
       p.smem = sizeof(float) * 2 * g * p.ept + sizeof(float2) * 2 * g * p.lv * p.vv;
+      if (d.layout == D2C_NORM_VOLUME_TO_ROWS) p.smem += (size_t)p.lv * p.vv * (C * size + 16);
       const long long tiles = (d.positions + p.lv * p.vv - 1) / (p.lv * p.vv) * d.batch;
       const long long most = (long long)sms * std::min(8, std::max(1, (backward ? 512 : 1024) / p.threads));
       p.blocks = (int)(tiles < most ? tiles : most);
@@ -925,7 +1059,7 @@ int run_typed(const d2c_layer_norm_desc& d, NormArgs a, const Plan& p, bool back
   } else if (p.path == Path::volume) {
     const bool tokens = d.layout == D2C_NORM_VOLUME_TO_ROWS;
     const int w = std::min<int>(32 / (int)sizeof(T), p.ept);
-    a.vec_tokens = tokens && d.channels % w == 0 && aligned_to(backward ? a.g : a.y, w * sizeof(T));
+    a.vec_tokens = tokens && d.channels % w == 0 && aligned_to(backward ? a.g : a.y, 16);
     const int rc = p.ept == 8 ? volume_lv<T, 8>(a, p, tokens, backward, st) : volume_lv<T, 32>(a, p, tokens, backward, st);
     if (rc) return rc;
   } else {

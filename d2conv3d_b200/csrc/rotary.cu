@@ -31,7 +31,7 @@ struct RotaryArgs {
 // V pairs of a thread: channels u0 .. and v0 .. (halves of a section, which V divides), or 2 V neighbouring channels (which may
 // belong to two sections).  The first heads are asked for before the angles are formed.
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) rotary_kernel(RotaryArgs a) {
   constexpr int kHeads = 4;                                      // in flight
   __shared__ double freqs[256];                                  // turns per position of every pair
   const int pairs = a.dim / 2, j = threadIdx.x * V;              // first pair of this thread

@@ -207,4 +207,6 @@ def test_more_elements_than_32_bits_count():
     del x
     v = torch.zeros(65600, 512, 64, device="cuda", dtype=torch.bfloat16)
     v[-1] = torch.randn(512, 64, device="cuda").bfloat16()
-    assert torch.equal(d2c.layer_norm(v, layout="channels_first")[-1:], d2c.layer_norm(v[-1:].clone(), layout="channels_first"))
+    got = d2c.layer_norm(v, layout="channels_first")[-1:]
+    want = layer_norm_oracle(v[-1:], None, None, torch.zeros_like(v[-1:]), 1e-5, 1)["y"]
+    assert_within(got, want[0], rounded(*want, torch.bfloat16), "last clip")
