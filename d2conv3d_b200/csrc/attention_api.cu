@@ -56,15 +56,18 @@ bool tensor_rows(const d2c_attention_desc& d, const int64_t (&s)[3], int tokens,
   return true;
 }
 
-// Parts of the tensor-core kernels' operands; 0 where they do not apply.  fp32 goes by the math mode: hi and lo parts for parity
-// (the gradients' operands fit shared memory up to 64 channels), hi alone, or CUDA cores.  The running maximum is that of the raw
+// Parts of the tensor-core kernels' operands; 0 where they do not apply.  fp32 goes by the math mode: two parts for parity, one, or CUDA
+// cores.  The running maximum is that of the raw
 // scores, so the scale has to be above zero.
 int tensor_parts(const d2c_attention_desc& d, int mode, bool aligned, bool backward) {
   if (!aligned || !(d.scale > 1e-30f)) return 0;
   if (d.dtype == D2C_F32) {
     if (mode == D2C_MATH_FP32) return 0;
     if (mode == D2C_MATH_BF16) return 1;
-    return backward && d.dim > 64 ? 0 : 2;
+    // staging and joining are launches of their own: 2 x 1015 x 179, 4 heads of 32 channels, trains in 84 us on CUDA cores and in 113
+    // in two parts; 2 x 400 x 400, 4 heads of 64, in 118 and 107
+    const double products = (double)d.batch * d.q_heads * d.queries * d.keys * d.dim;
+    return mode == D2C_MATH_AUTO && products < (double)(1 << 26) ? 0 : 2;
   }
   return d.dim % 8 == 0 && tensor_rows(d, d.q_stride, d.queries, d.q_heads) && tensor_rows(d, d.k_stride, d.keys, d.kv_heads) &&
          tensor_rows(d, d.v_stride, d.keys, d.kv_heads) && (!backward || tensor_rows(d, d.g_stride, d.queries, d.q_heads));

@@ -1,5 +1,5 @@
 // Gradients of cross attention on tensor cores: fp16 and bf16 tensors whose head width is a multiple of 8, up to 128 channels; fp32
-// tensors staged in 16 bits (attention_sm100.cu: split_rows), in two parts up to 64 channels, in one up to 128.
+// tensors staged in 16 bits (attention_sm100.cu: split_rows), in one part or two; up to 128 channels.
 //
 // One kernel, two uses.  A block keeps a tile of 128 rows X (X1, X2) and runs over tiles of 128 rows Y (Y1, Y2):
 //   S = X1 Y1^T,  dP = X2 Y2^T,  P = 2^(S scale log2 e - lse),  dS = P (dP - delta)
@@ -12,11 +12,12 @@
 //
 // A tile's products, exponentials and gradients wait for one another: what a SM does at a time is what it has of independent tiles.  Up
 // to 64 channels Y tiles have 64 rows (kY), so that tensor memory (64 + 64 + 64 + 64 columns) and shared memory hold two blocks a SM, of
-// 4 working warps, a thread a row.  Above, and with operands in two parts, Y tiles have 128 rows and the one block has 8 working warps, a
-// thread a row and half of the columns.
+// 4 working warps, a thread a row.  With operands twice as large (128 channels, or two parts) Y tiles have 128 rows and the one block has
+// 8 working warps, a thread a row and half of the columns.  With both, shared memory holds X and one Y1 and one Y2 of 64 rows: the next
+// are loaded when these are done.
 //
 // fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
-// they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, becomes 2^14 .. 2^15) and the sums scaled back.
+// they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, is at most 2^14) and the sums scaled back.
 #include <algorithm>
 #include <type_traits>
 
@@ -39,25 +40,25 @@ struct BwdParams {
   int* status;
 };
 
+constexpr int y_rows(int size) { return size == 128 ? 128 : 64; }    // size: channels (64, 128) times parts
 template <int DP, int kParts>
-constexpr int kYRows = DP * kParts == 64 ? 64 : 128;
+constexpr int kYRows = y_rows(DP * kParts);
 template <int DP, int kParts>
 constexpr int kThreads = kYRows<DP, kParts> == 64 ? 256 : 384;       // working warps; MMA issuer, loader, two idle (see registers_up)
 template <int DP, int kParts>
-constexpr int kStages = DP * kParts == 64 ? 8 : 4;
+constexpr int kStages = DP * kParts == 64 ? 8 : (DP * kParts == 128 ? 4 : 2);
 template <int DP, int kParts>
 constexpr int kYBytes = kYRows<DP, kParts> * DP * 2 * kParts;
 template <int DP, int kParts>
 constexpr int kSmem = 2 * kTileBytes<DP> * kParts + kStages<DP, kParts> * kYBytes<DP, kParts> + 1024;
 
 template <typename T, typename Out, int DP, int kParts, bool kKeys>
-__global__ void __launch_bounds__(kThreads<DP, kParts>, kYRows<DP, kParts> == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads<DP, kParts>, DP * kParts == 64 ? 2 : 1)
 bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2, const __grid_constant__ CUtensorMap my1,
               const __grid_constant__ CUtensorMap my2, const __grid_constant__ BwdParams p) {
   constexpr int kY = kYRows<DP, kParts>, kWork = kY / 16;        // rows of a Y tile, working warps
   constexpr int kSt = kStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kYB = kYBytes<DP, kParts>;
-  constexpr int kMmaWarp = kWork, kLoadWarp = kWork + 1, kCols = kY == 64 ? 256 : 512;
-  static_assert(kY == 128 || DP == 64);
+  constexpr int kMmaWarp = kWork, kLoadWarp = kWork + 1, kCols = kY == 64 && DP == 64 ? 256 : 512;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
   extern __shared__ uint8_t raw[];
@@ -91,8 +92,10 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   if constexpr (kHalf) {
     const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
     const int n_heads = p.B * p.Hkv;
-    const float bound = 2.f * p.D * __uint_as_float(q[2 * n_heads]) * __uint_as_float(q[3 * n_heads]);
-    if (bound > 0.f && bound < INFINITY) e_ds = max(-100, min(100, 14 - ilogbf(bound)));       // 2^e_ds * bound <= 2^15
+    const float most_v = __uint_as_float(q[2 * n_heads]), most_g = __uint_as_float(q[3 * n_heads]);
+    // |dS| <= |dP| + |delta| <= 2 D most_v most_g, taken by exponents: the product itself may be beyond fp32
+    if (most_v > 0.f && most_g > 0.f)
+      e_ds = max(-126, min(126, 14 - (ilogbf(most_v) + ilogbf(most_g) + 2 + ilogbf((float)(4 * p.D - 1)))));
     if constexpr (kParts == 2) {
       e_q = scale_exponent(q[0]);
       e_k = scale_exponent(q[n_heads]);
@@ -125,11 +128,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = tmem_slot, tS = tmem, tD = tmem + kY, tA1 = tmem + 2 * kY, tA2 = tA1 + (kY == 64 ? 64 : 128);
+  const uint32_t tmem = tmem_slot, tS = tmem, tD = tmem + kY, tA1 = tmem + 2 * kY, tA2 = tA1 + DP;
 
   if (warp >= kWork) {
-    if constexpr (kY == 64) registers_down_4();
-    else registers_down();
+    if constexpr (kCols == 256) registers_down_4();                       // (8 warps alone on a SM have registers enough)
+    else if constexpr (kY == 128) registers_down();
     if (warp == kLoadWarp) {
       int i = 0;                                  // Y tiles asked for: Y1 Y2 Y1 Y2 ...
       if (n > 0) {
@@ -198,22 +201,28 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (int i = 0; i < n; ++i) {
           const int y1 = 2 * i, y2 = y1 + 1;
           const bool more = i + 1 < n;
-          if (more && !there(y1 + 2)) return;     // what is there long before P
+          if (kSt > 2 && more && !there(y1 + 2)) return;                  // what is there long before P
           if (!ptx::mbar_wait(p_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
           if constexpr (kKeys) {
             weigh(tA1, tS, slot(y2), i > 0);
             ptx::umma_commit(empty(y2 % kSt));    // before the next S: a short ring waits for this tile's place
           }
-          if (more) {
+          if (kSt > 2 && more) {
             mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
             ptx::umma_commit(s_full);
+            if (!there(y2 + 2)) return;
           }
-          if (more && !there(y2 + 2)) return;
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
           weigh(tA2, tD, slot(y1), i > 0);
           ptx::umma_commit(empty(y1 % kSt));
+          if (kSt == 2 && more) {                 // the next tiles take the places of these
+            if (!there(y1 + 2)) return;
+            mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(y1 + 2), id_s, ksteps);
+            ptx::umma_commit(s_full);
+            if (!there(y2 + 2)) return;
+          }
           if (more) {
             mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(y2 + 2), id_s, ksteps);
             ptx::umma_commit(dp_full);
@@ -226,8 +235,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       drain(done, 0);
     }
   } else {
-    if constexpr (kY == 64) registers_up_4();
-    else registers_up();
+    if constexpr (kCols == 256) registers_up_4();
+    else if constexpr (kY == 128) registers_up();
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, xi = x0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tS + 64 * half + lanes, d_at = tD + 64 * half + lanes;
@@ -411,9 +420,9 @@ template <typename T, typename Out, int DP, int kParts>
 int by_side(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStream_t st) {
   return keys ? launch<T, Out, DP, kParts, true>(m, p, st) : launch<T, Out, DP, kParts, false>(m, p, st);
 }
-template <typename T, typename Out>
+template <typename T, typename Out, int kParts>
 int by_width(const CUtensorMap (&m)[4], const BwdParams& p, bool keys, cudaStream_t st) {
-  return p.width <= 64 ? by_side<T, Out, 64, 1>(m, p, keys, st) : by_side<T, Out, 128, 1>(m, p, keys, st);
+  return p.width <= 64 ? by_side<T, Out, 64, kParts>(m, p, keys, st) : by_side<T, Out, 128, kParts>(m, p, keys, st);
 }
 
 }  // namespace
@@ -426,8 +435,7 @@ int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys
   int rc;
   const bool staged = dtype == D2C_F32;
   if (staged) dtype = parts == 2 ? D2C_F16 : D2C_BF16;
-  const int y_rows = parts == 1 && p.width <= 64 ? 64 : 128;            // kYRows
-  const int q_rows = keys ? y_rows : kRows, k_rows = keys ? kRows : y_rows;
+  const int rows = y_rows((p.width <= 64 ? 64 : 128) * parts), q_rows = keys ? rows : kRows, k_rows = keys ? kRows : rows;
   if ((rc = tile_map(&q, x[0], dtype, p.width, a.Hq, a.Lq, a.B * parts, q_rows))) return rc;
   if ((rc = tile_map(&k, x[1], dtype, p.width, a.Hkv, a.Lk, a.B * parts, k_rows))) return rc;
   if ((rc = tile_map(&v, x[2], dtype, p.width, a.Hkv, a.Lk, a.B * parts, k_rows))) return rc;
@@ -441,8 +449,8 @@ int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys
   p.part = a.part;
   p.a = a;
   if ((rc = status_pointer(&p.status))) return rc;
-  if (staged) return parts == 2 ? by_side<__half, float, 64, 2>(maps, p, keys, st) : by_width<__nv_bfloat16, float>(maps, p, keys, st);
-  return dtype == D2C_BF16 ? by_width<__nv_bfloat16, __nv_bfloat16>(maps, p, keys, st) : by_width<__half, __half>(maps, p, keys, st);
+  if (staged) return parts == 2 ? by_width<__half, float, 2>(maps, p, keys, st) : by_width<__nv_bfloat16, float, 1>(maps, p, keys, st);
+  return dtype == D2C_BF16 ? by_width<__nv_bfloat16, __nv_bfloat16, 1>(maps, p, keys, st) : by_width<__half, __half, 1>(maps, p, keys, st);
 }
 
 }  // namespace attn

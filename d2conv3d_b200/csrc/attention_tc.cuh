@@ -136,7 +136,7 @@ __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t pack
 // Exponent e that brings a largest element to 2^14 .. 2^15 (bits of a float, as largest_sizes writes it; 0: all are zero).
 __device__ __forceinline__ int scale_exponent(uint32_t size) {
   const float f = __uint_as_float(size);
-  return f > 0.f ? max(-100, min(100, 14 - ilogbf(f))) : 0;
+  return f > 0.f ? max(-126, min(126, 14 - ilogbf(f))) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // |e| <= 126
 // Eight neighbouring results of a row, the first `n` of them (16-byte stores where all are there; dst is then 16-byte aligned).

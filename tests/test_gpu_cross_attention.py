@@ -22,10 +22,11 @@ def run(q, k, v, g, lengths=None, scale=None):
     return (o.detach(),) + torch.autograd.grad(o, leaves, g)
 
 
-# fp32 by math mode: (half a step of the probabilities, what the operands' rounding takes from a product).  "auto": hi + lo fp16
+# fp32 by math mode: (half a step of the probabilities, what the operands' rounding takes from a product).  "bf16x3", the mode of split
+# operands, which "auto" takes for large calls: hi + lo fp16
 # parts keep a factor to 2^-22 (half a step of the second part, 2^-11 of at most 2^-11), and lo lo, at most 2^-22, is left out.
 # "bf16": each factor to 2^-9.
-FP32_MODES = {"fp32": (U, 0.0), "auto": (2.0 ** -22, 3 * 2.0 ** -22), "bf16": (2.0 ** -9, 2.0 ** -8 + 2.0 ** -18)}
+FP32_MODES = {"fp32": (U, 0.0), "bf16x3": (2.0 ** -22, 3 * 2.0 ** -22), "bf16": (2.0 ** -9, 2.0 ** -8 + 2.0 ** -18)}
 
 
 def check(q, k, v, g, lengths=None, scale=None):
@@ -150,6 +151,18 @@ def test_many_keys_few_queries_and_the_reverse(dtype):
     check(*make(1, 3000, 40, 2, 1, 64, dtype, 9))
 
 
+def test_large_fp32_calls_take_split_operands():
+    q, k, v, g = make(1, 600, 1000, 2, 1, 64, torch.float32, 21)
+    auto = run(q, k, v, g)
+    for mode, same in (("bf16x3", True), ("fp32", False)):
+        try:
+            d2c.set_math_mode(mode)
+            other = run(q, k, v, g)
+        finally:
+            d2c.set_math_mode("auto")
+        assert all(torch.equal(a, b) for a, b in zip(auto, other)) == same
+
+
 def test_gradient_by_differences():
     torch.manual_seed(0)
     q, k, v, g = make(1, 9, 21, 2, 1, 16, torch.float32, 1)
@@ -179,6 +192,33 @@ def test_empty():
     o = d2c.cross_attention(q[:, :0], k, k)
     assert o.shape == (2, 0, 4, 64) and (torch.autograd.grad(o.sum(), k)[0] == 0).all()
     assert d2c.cross_attention(q[:0], k[:0], k[:0]).shape == (0, 3, 4, 64)
+
+
+@pytest.mark.parametrize("big,small", [(1e30, 1e-30), (3e38, 1.0), (1e-38, 1e-3)])
+def test_fp32_beyond_the_range_of_16_bits(big, small):
+    # operands are scaled by powers of two before they are split: nothing overflows, nothing vanishes
+    q, k, v, g = make(2, 300, 400, 2, 1, 64, torch.float32, 22)
+    d2c.set_math_mode("bf16x3")
+    try:
+        check(q, k, v, g)
+        plain = run(q, k, v, g)
+        big, small = 2.0 ** min(127, round(math.log2(big))), 2.0 ** round(math.log2(small))   # 2^128 is not a float32
+        if big > 2.0 ** 100:
+            v = v / 64
+            plain = (plain[0] / 64, plain[1] / 64, plain[2] / 64, plain[3])
+        o = run(q, k, v * big, g)[0]
+        if big < 2.0 ** -100:
+            # below fp32's normal range: v is scaled to 1 at most, not to 2^14, so that its parts end at 2^-25 of that, and the result
+            # is a multiple of 2^-149 on either side
+            assert (o.double() - plain[0].double() * big).abs().max() <= big * v.abs().max() * 2.0 ** -22 + 2.0 ** -148
+        else:
+            assert torch.equal(o, plain[0] * big)
+        gv = run(q, k, v, g * small)[3]
+        assert torch.equal(gv, plain[3] * small)
+        if 1e-30 < small < 1:
+            assert torch.equal(run(q * small, k / small, v, g)[0], plain[0])
+    finally:
+        d2c.set_math_mode("auto")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
