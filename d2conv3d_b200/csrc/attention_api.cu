@@ -83,7 +83,7 @@ int fewest_shares(int parts, int steps, long long rows, int dim) {
 }
 
 // `slots` blocks at a time on the tensor cores.
-Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, int steps_rows, int slots,
+Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, long long steps_rows, int slots,
                int sms) {
   const bool tensor = parts > 0;
   const int tile = tensor ? 128 : kTile;
@@ -111,7 +111,7 @@ Plan plan_bwd(const d2c_attention_desc& d, int mode, bool keys, bool aligned, in
   const int slots = parts == 1 && d.dim <= 64 ? 2 * sms : sms;
   if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, slots, sms);
   const int tile = parts ? 128 : kTile;
-  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), slots, sms);
+  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, (long long)ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), slots, sms);
 }
 
 size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 4 * d.batch * d.kv_heads, 256); }
@@ -152,8 +152,8 @@ int checked(const d2c_attention_desc* d) {
   if (d->batch < 1 || d->queries < 1 || d->keys < 1 || d->q_heads < 1 || d->kv_heads < 1 || d->dim < 1 || d->dim > 128)
     return D2C_ERR_SHAPE;
   if (d->q_heads % d->kv_heads) return D2C_ERR_GROUPS;
-  // grids and row indexes of the kernels
-  if (q_rows(*d) > 0x7fffffffLL || kv_rows(*d) > 0x7fffffffLL || (long long)d->batch * d->q_heads > 65535) return D2C_ERR_TOO_LARGE;
+  // grids, row indexes and the kernels' 32-bit steps over tokens
+  if (q_rows(*d) > 0x7fffffffLL || kv_rows(*d) > 0x7fffffffLL || d->queries > 1 << 30 || d->keys > 1 << 30) return D2C_ERR_TOO_LARGE;
   return D2C_OK;
 }
 

@@ -343,32 +343,34 @@ template <typename T>
 __global__ void __launch_bounds__(256) bound_kernel(const __grid_constant__ RowsArgs p) {
   constexpr int kU = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.z, H = p.H[i];
-  if ((int)blockIdx.y >= p.B * H) return;
-  const int h = blockIdx.y % H, b = blockIdx.y / H, hk = h / (H / p.a.Hkv);
-  const int len = p.keys[i] ? key_length(p.a, b) : p.L[i], step = gridDim.x * 8;
-  const T* x = reinterpret_cast<const T*>(p.x[i]) + b * p.s[i][0] + h * p.s[i][2];
-  float most = 0.f;
-  for (int r = blockIdx.x * 8 + warp; r < len; r += step * kU) {
-    float v[kU][4];
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[u][e] = r + u * step < len && lane + 32 * e < p.D ? fabsf(to_f32(x[(long long)(r + u * step) * p.s[i][1] + lane + 32 * e])) : 0.f;
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v[u][e] < INFINITY) most = fmaxf(most, v[u][e]);
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
   __shared__ float all[8];
-  if (lane == 0) all[warp] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) most = fmaxf(most, all[w]);
-    if (most > 0.f) atomicMax(p.bounds + ((long long)p.which[i] * p.B + b) * p.a.Hkv + hk, __float_as_uint(most));
+  for (long long head = blockIdx.y; head < (long long)p.B * H; head += gridDim.y) {
+    const int h = (int)(head % H), b = (int)(head / H), hk = h / (H / p.a.Hkv);
+    const int len = p.keys[i] ? key_length(p.a, b) : p.L[i], step = gridDim.x * 8;
+    const T* x = reinterpret_cast<const T*>(p.x[i]) + b * p.s[i][0] + h * p.s[i][2];
+    float most = 0.f;
+    for (int r = blockIdx.x * 8 + warp; r < len; r += step * kU) {
+      float v[kU][4];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[u][e] = r + u * step < len && lane + 32 * e < p.D ? fabsf(to_f32(x[(long long)(r + u * step) * p.s[i][1] + lane + 32 * e])) : 0.f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v[u][e] < INFINITY) most = fmaxf(most, v[u][e]);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    __syncthreads();                                             // the last head's values have been read
+    if (lane == 0) all[warp] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) most = fmaxf(most, all[w]);
+      if (most > 0.f) atomicMax(p.bounds + ((long long)p.which[i] * p.B + b) * p.a.Hkv + hk, __float_as_uint(most));
+    }
   }
 }
 
@@ -468,10 +470,10 @@ int largest_sizes(int dtype, const Args& a, bool values_only, uint32_t* bounds, 
   RowsArgs s = rows_args(a, bounds);
   int n = 0;
   for (int which = values_only ? 2 : 0; which < (a.g ? 4 : 3); ++which) add_rows(s, n++, a, which);
-  const long long heads = (long long)a.B * a.Hq;                 // <= 65535, and not fewer than the key heads
+  const long long heads = (long long)a.B * a.Hq;                 // not fewer than the key heads
   const long long rows = (std::max(a.Lq, a.Lk) + 31) / 32;       // steps of a block
   const unsigned x = (unsigned)std::max<long long>(1, std::min<long long>(rows, (148 * 4 + heads * n - 1) / (heads * n)));
-  const dim3 grid(x, (unsigned)heads, n);
+  const dim3 grid(x, (unsigned)std::min<long long>(heads, 65535), n);
   switch (dtype) {
     case D2C_F32: bound_kernel<float><<<grid, 256, 0, st>>>(s); break;
     case D2C_F16: bound_kernel<__half><<<grid, 256, 0, st>>>(s); break;

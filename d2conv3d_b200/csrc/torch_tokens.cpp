@@ -222,6 +222,7 @@ Tensor rotary(const Tensor& x, const OptTensor& positions_, const std::array<int
       case at::kFloat: d.pos_kind = D2C_POS_F32; break;
       default: TORCH_CHECK(false, "rotary_embedding_3d: positions must be int32, int64 or float32, got ", positions.scalar_type());
     }
+    TORCH_CHECK(!positions.requires_grad(), "rotary_embedding_3d: not differentiable in positions");
     d.pos_batch_stride = positions.dim() == 3 && positions.size(0) > 1 ? x.size(1) * 3 : 0;
   } else {
     int64_t n = 1;

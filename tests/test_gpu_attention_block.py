@@ -1,4 +1,7 @@
 """The token operators as they are used together: norm, projection, rotary positions, attention, projection."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -88,3 +91,50 @@ def test_decoder_with_the_attention_bridge(train):
     y.square().mean().backward()
     for name, p in net.gc.named_parameters():
         assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, name
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_block_under_autocast(dtype):
+    torch.manual_seed(3)
+    m = d2c.CrossAttention3d(48, 80, heads=2, head_dim=64).cuda()
+    x, context = torch.randn(2, 48, 2, 5, 7, device="cuda", requires_grad=True), torch.randn(2, 80, 2, 9, 13, device="cuda")
+    full = m(x, context)
+    with torch.autocast("cuda", dtype):
+        y = m(x, context)
+        y16 = m(x.to(dtype), context.to(dtype))
+    # rounding of tokens, projections, probabilities and outputs: a dozen half steps of 16 bits
+    for got in (y, y16):
+        assert (got - full).abs().max() <= 12 * torch.finfo(dtype).eps / 2 * full.abs().max()
+    y.square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+import d2conv3d_b200 as d2c
+mode = "bf16x3" if "%(dtype)s" == "float32" else "auto"
+d2c.set_math_mode(mode)
+def make(*s):
+    return torch.randn(*s, device="cuda").to(torch.%(dtype)s).requires_grad_()
+x, w, q, k, g = make(2, 64, 90), make(64), make(1, 90, 2, 64), make(1, 200, 2, 64), make(1, 90, 2, 64).detach()
+one, gn = make(1, 1, 2, 64), make(2, 90, 64).detach()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def step():
+    y = d2c.layer_norm(x, w, layout="tokens")
+    r = d2c.rotary_embedding_3d(q, (1, 9, 10), (16, 24, 24))
+    o = d2c.cross_attention(r, k, k)
+    return (y, o, d2c.cross_attention(one.detach(), k.detach(), k.detach())) + torch.autograd.grad((y, o), (x, w, q, k), (gn, g))
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_first_calls_of_a_process_are_captured(dtype):
+    # whatever a first call sets up must not disturb a capture
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED % {"dtype": dtype}], capture_output=True, text=True, timeout=240)
+    assert p.returncode == 0, p.stderr[-2000:]

@@ -294,6 +294,20 @@ def test_offsets_that_pass_32_bits(dtype):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_more_heads_than_a_grid_dimension(dtype):
+    q, k, v, g = make(2, 17, 40, 1, 1, 16, dtype, 14)
+    if dtype == torch.float32:
+        d2c.set_math_mode("bf16x3")
+    try:
+        want = run(q, k, v, g)
+        many = [t.repeat(35000, 1, 1, 1) for t in (q, k, v, g)]
+        for a, b in zip(run(*many), want):
+            assert torch.equal(a[-2:], b) and torch.equal(a[:2], b)
+    finally:
+        d2c.set_math_mode("auto")
+
+
 def test_refusals():
     q, k, v, _ = make(2, 3, 5, 4, 2, 64, torch.float32)
     for args, text in (((q.double(), k.double(), v.double()), "not implemented"), ((q, k.half(), v), "same type"),

@@ -108,6 +108,8 @@ def test_refusals():
         d2c.rotary_embedding_3d(x, torch.zeros(5, 3, device="cuda"), (8, 12, 12))
     with pytest.raises(RuntimeError, match="int32, int64 or float32"):
         d2c.rotary_embedding_3d(x, torch.zeros(4, 3, device="cuda").double(), (8, 12, 12))
+    with pytest.raises(RuntimeError, match="not differentiable in positions"):
+        d2c.rotary_embedding_3d(x, torch.zeros(4, 3, device="cuda", requires_grad=True), (8, 12, 12))
     with pytest.raises(RuntimeError, match="expected positions on"):
         d2c.rotary_embedding_3d(x, torch.zeros(4, 3), (8, 12, 12))
     with pytest.raises(RuntimeError, match="even number of channels"):

@@ -84,7 +84,8 @@ def test_c_abi_checks_sizes_before_anything_is_launched():
     assert attention() == 0
     assert attention(dtype=1) == -2 and attention(kv_heads=3) == -4 and attention(dim=129) == -3 and attention(dim=0) == -3
     assert attention(queries=0) == -3 and attention(keys=0) == -3
-    assert attention(queries=1 << 30, q_heads=4) == -9
+    assert attention(queries=1 << 30, q_heads=4) == -9 and attention(keys=(1 << 30) + 1, kv_heads=1) == -9
+    assert attention(batch=1 << 20, q_heads=8, kv_heads=8) == 0
     assert L.d2c_status_string(-13) != b"unknown status"
 
 
