@@ -74,23 +74,22 @@ int tensor_parts(const d2c_attention_desc& d, int mode, bool aligned, bool backw
 }
 
 // The tensor cores add into their accumulator with truncation: a chain of n accumulating products loses about n * 2^-27 of the
-// result.  With two parts (24 products a tile) a share ends after 8 tiles, 1.5e-6, and the shares are added in fp32 -- unless their
-// results would take more than 2 GB.  (Measured at 1215 x 3240, 64 channels: gradients 5e-6 off with 12 tiles.)
-constexpr int kChainTiles = 8;
-int fewest_shares(int parts, int steps, long long rows, int dim) {
+// result.  With two parts (24 products a tile, 8 of them into the sum of the hi parts where those of lo parts have one of their own) a
+// share ends after 8 tiles, or 3, 0.5e-6, and the shares are added in fp32 -- unless their results would take more than 2 GB.
+int fewest_shares(int parts, bool apart, int steps, long long rows, int dim) {
   if (parts != 2) return 1;
-  return (int)std::min<long long>(ceil_div(steps, kChainTiles), std::max(1LL, (2LL << 30) / (4 * rows * dim)));
+  return (int)std::min<long long>(ceil_div(steps, apart ? 8 : 3), std::max(1LL, (2LL << 30) / (4 * rows * dim)));
 }
 
 // `slots` blocks at a time on the tensor cores.
 Plan make_plan(const d2c_attention_desc& d, int parts, int rows_x, int heads_x, long long rows_out, int per_block, long long steps_rows, int slots,
-               int sms) {
+               int sms, bool apart) {
   const bool tensor = parts > 0;
   const int tile = tensor ? 128 : kTile;
   const int steps = ceil_div(steps_rows, tile);
   return {tensor ? Path::tensor : Path::exact,
           shares((long long)ceil_div(rows_x, tile * per_block) * heads_x * d.batch, steps, tensor ? slots : 2 * sms, tensor ? 3.0 : 1.0,
-                 join_steps(rows_out, d.dim), fewest_shares(parts, steps, rows_out, d.dim)),
+                 join_steps(rows_out, d.dim), fewest_shares(parts, apart, steps, rows_out, d.dim)),
           parts};
 }
 
@@ -103,15 +102,15 @@ Plan plan_fwd(const d2c_attention_desc& d, int mode, bool aligned, int sms) {
   }
   const int parts = tensor_parts(d, mode, aligned, false);
   const bool two_tiles = parts > 0 && !(parts == 2 && d.dim > 64);
-  return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), two_tiles ? 2 : 1, d.keys, sms, sms);
+  return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), two_tiles ? 2 : 1, d.keys, sms, sms, true);
 }
 // A gradient kernel's block has a tile of one side and runs over the other.
 Plan plan_bwd(const d2c_attention_desc& d, int mode, bool keys, bool aligned, int sms) {
   const int parts = tensor_parts(d, mode, aligned, true);
   const int slots = parts == 1 && d.dim <= 64 ? 2 * sms : sms;
-  if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, slots, sms);
+  if (!keys) return make_plan(d, parts, d.queries, d.q_heads, q_rows(d), 1, d.keys, slots, sms, d.dim <= 64);
   const int tile = parts ? 128 : kTile;
-  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, (long long)ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), slots, sms);
+  return make_plan(d, parts, d.keys, d.kv_heads, 2 * kv_rows(d), 1, (long long)ceil_div(d.queries, tile) * tile * (d.q_heads / d.kv_heads), slots, sms, d.dim <= 64);
 }
 
 size_t bound_bytes(const d2c_attention_desc& d) { return align_up(sizeof(uint32_t) * 4 * d.batch * d.kv_heads, 256); }

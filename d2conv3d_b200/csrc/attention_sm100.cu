@@ -84,7 +84,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const uint32_t tS = tmem, tO = tmem + 256;      // S_t at 128 t (P_t over it), O_t at DP t
+  const uint32_t tS = tmem, tO = tmem + 256;      // S_t at 128 t (P_t over it), O_t at DP t (two parts: the lo sums 128 columns further)
 
   if (warp >= 8) {
   registers_down();
@@ -145,7 +145,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             for (int h = 0; h < 2; ++h) {         // the first half of the keys while the second's p is formed
               if (!ptx::mbar_wait(p_ready(t, h), j & 1, abort_flag)) return;
               ptx::tc_fence_after();
-              mma_weigh<DP, kParts>(tO + DP * t, tS + 128 * t + 32 * h, 64, d_v + (sv * kTB >> 4) + 512 * h, id_o, j > 0 || h > 0);
+              mma_weigh<DP, kParts, kParts == 2>(tO + DP * t, tS + 128 * t + 32 * h, 64, d_v + (sv * kTB >> 4) + 512 * h, id_o, j > 0 || h > 0);
             }
             if (more) {
               mma_scores<DP, kParts>(tS + 128 * t, d_q + (t * kTB >> 4), d_k + (sk * kTB >> 4), id_s, ksteps);
@@ -207,14 +207,15 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         const float to = fmaxf(mx, m), f = exp2_fast(m - to);
         m = to;
         l *= f;
-        for (int c0 = 0; c0 < dcols; c0 += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(o_at + c0, o);
-          ptx::tmem_ld_wait();
+        for (int part = 0; part < kParts; ++part)
+          for (int c0 = 0; c0 < dcols; c0 += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32(o_at + 128 * part + c0, o);
+            ptx::tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st_32x32(o_at + c0, o);
-        }
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st_32x32(o_at + 128 * part + c0, o);
+          }
       }
       F2 sum[2] = {0ull, 0ull};
       const F2 c2 = f2(c, c), m2 = f2(-m, -m);
@@ -256,8 +257,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       for (int c0 = 0; c0 < p.D; c0 += 32) {
         uint32_t o[32];
         if (n > 0) {
-          ptx::tmem_ld_32x32(o_at + c0, o);
-          ptx::tmem_ld_wait();
+          load_sums<kParts == 2>(o_at + c0, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;

@@ -59,6 +59,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   constexpr int kY = kYRows<DP, kParts>, kWork = kY / 16;        // rows of a Y tile, working warps
   constexpr int kSt = kStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kYB = kYBytes<DP, kParts>;
   constexpr int kMmaWarp = kWork, kLoadWarp = kWork + 1, kCols = kY == 64 && DP == 64 ? 256 : 512;
+  constexpr bool kApart = kParts == 2 && DP == 64;                        // tensor memory has room for sums of lo parts
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
   extern __shared__ uint8_t raw[];
@@ -186,8 +187,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       auto slot = [&](int i) { return (uint32_t)((i % kSt) * kYB) >> 4; };
       auto there = [&](int i) { return ptx::mbar_wait(full(i % kSt), (i / kSt) & 1, abort_flag); };
       auto weigh = [&](uint32_t acc, uint32_t w, uint32_t y, bool more) {   // each half of the columns has its parts at its own start
-        mma_weigh<DP, kParts, kY>(acc, w, 32, d_yt + y, id_a, more);
-        if constexpr (kY == 128) mma_weigh<DP, kParts, kY>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
+        mma_weigh<DP, kParts, kApart, kY>(acc, w, 32, d_yt + y, id_a, more);
+        if constexpr (kY == 128) mma_weigh<DP, kParts, kApart, kY>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
       };
       auto run = [&]() {
         if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
@@ -369,8 +370,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (; c0 < c_end; c0 += 32) {
           uint32_t r[32];
           if (n > 0) {
-            ptx::tmem_ld_32x32(acc + c0, r);
-            ptx::tmem_ld_wait();
+            load_sums<kApart>(acc + c0, r);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = 0u;

@@ -94,27 +94,46 @@ __device__ __forceinline__ bool elect_one() {
 //
 // D (128 x RY) = X Y^T over the channels, both K-major (descriptors of the first part's first step); ksteps = channels / 16 rounded up
 // (zero-filled above D).
+// The products with a lo part come first: the tensor cores truncate the sum at every product, by the size that it has then.
 template <int DP, int kParts, int RY = kRows>
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint64_t x, uint64_t y, uint32_t idesc, int ksteps) {
 #pragma unroll
-  for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
+  for (int pass = kParts == 2 ? 2 : 0; pass >= 0; --pass) {              // hi lo, lo hi, hi hi
     const uint32_t xp = pass == 1 ? kTileBytes<DP> >> 4 : 0, yp = pass == 2 ? RY * DP * 2 >> 4 : 0;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       const uint32_t in = (k & 3) * 2, h = k >> 2;
       if (k < ksteps)
-        ptx::umma_bf16(d_tmem, x + (xp + in + h * (kHalfBytes >> 4)), y + (yp + in + h * (RY * 128 >> 4)), idesc, pass > 0 || k > 0);
+        ptx::umma_bf16(d_tmem, x + (xp + in + h * (kHalfBytes >> 4)), y + (yp + in + h * (RY * 128 >> 4)), idesc,
+                       (kParts == 2 && pass < 2) || k > 0);
     }
   }
 }
 // D (128 x N) (+)= A Y, A 128 x 64 in tensor memory (32 columns; its lo part `lo` columns further), 64 rows of Y, MN-major, the reduction.
-template <int DP, int kParts, int RY = kRows>
+// kApart: what has a lo part adds up in 128 columns further on, so that the large sum is truncated a third as often.
+template <int DP, int kParts, bool kApart, int RY = kRows>
 __device__ __forceinline__ void mma_weigh(uint32_t d_tmem, uint32_t a_tmem, int lo, uint64_t y, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int pass = 0; pass < (kParts == 2 ? 3 : 1); ++pass) {
     const uint32_t ap = a_tmem + (pass == 1 ? lo : 0), yp = pass == 2 ? RY * DP * 2 >> 4 : 0;
+    const uint32_t d = d_tmem + (kApart && pass > 0 ? 128 : 0);
+    const bool fresh = pass == 0 || (kApart && pass == 1);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) umma_ts(d_tmem, ap + 8 * k, y + (yp + 128 * k), idesc, accumulate || pass > 0 || k > 0);
+    for (int k = 0; k < 4; ++k) umma_ts(d, ap + 8 * k, y + (yp + 128 * k), idesc, accumulate || !fresh || k > 0);
+  }
+}
+// 32 columns of such an accumulator, both parts added.
+template <bool kApart>
+__device__ __forceinline__ void load_sums(uint32_t at, uint32_t (&r)[32]) {
+  ptx::tmem_ld_32x32(at, r);
+  if constexpr (kApart) {
+    uint32_t q[32];
+    ptx::tmem_ld_32x32(at + 128, q);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(q[e]));
+  } else {
+    ptx::tmem_ld_wait();
   }
 }
 
