@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Args a) {
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float shift = m == -INFINITY ? 0.f : m;
   float acc[4] = {}, sum = 0.f;
-#pragma unroll 8
+#pragma unroll (W == 1 ? 4 : 8)
   for (int s = first; s < a.splits; s += W) {
     const float f = exp2f(a.part_lse[s * rows + row] - shift);
     const float* p = a.part + (s * rows + row) * a.D;

@@ -901,7 +901,7 @@ __global__ void __launch_bounds__(512) norm_fold_kernel(const float* __restrict_
   const int c = blockIdx.x * 32 + cx, part = blockIdx.y;
   float s = 0.f;
   if (c < C) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = share; i < blocks; i += 16) s += partial[((long long)i * 2 + part) * C + c];
   }
   sh[share][cx] = s;
