@@ -21,13 +21,23 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // blocks of 102 steps on 148 SMs take 102 steps whole, 4 * 28.5 in 9 shares.)  At least `fewest` of them.
 int shares(long long blocks, int steps, int slots, double start, double join, int fewest) {
   fewest = std::max(1, std::min(fewest, steps));
+  const int most = std::min(steps, fewest + 127);
   int best = fewest;
   double least = 0;
-  for (int s = fewest; s <= std::min(steps, fewest + 127); ++s) {
-    const long long waves = (blocks * s + slots - 1) / slots;
-    const double cost = waves * (ceil_div(steps, s) + start) + (s > 1 ? start + join * s : 0.0);
-    if (s == fewest || cost < least) { best = s; least = cost; }
-    if (s > fewest && waves > 16) break;
+  auto look = [&](long long s) {
+    if (s < fewest || s > most) return;
+    const double cost = (double)((blocks * s + slots - 1) / slots) * (ceil_div(steps, s) + start) + (s > 1 ? start + join * s : 0.0);
+    if (least == 0 || cost < least) {
+      best = (int)s;
+      least = cost;
+    }
+  };
+  look(fewest);
+  look(fewest + 1);
+  for (int waves = 1; waves <= 16; ++waves) {
+    const long long s = (long long)waves * slots / blocks;        // the most that these waves hold
+    look(std::min<long long>(s, most));
+    if (s >= most) break;
   }
   return best;
 }

@@ -475,6 +475,15 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
 
 // ---- joining shares -----------------------------------------------------------------------------------------
 
+// Place of a row of [B, Lq, Hq]; there are fewer than 2^31 of them.
+struct RowAt {
+  int head, query, clip;
+};
+__device__ __forceinline__ RowAt row_at(const Args& a, unsigned row) {
+  const unsigned t = row / (unsigned)a.Hq, b = t / (unsigned)a.Lq;
+  return {(int)(row - t * (unsigned)a.Hq), (int)(t - b * (unsigned)a.Lq), (int)b};
+}
+
 // o = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m).  A block of 8 warps; W of them share a row's parts (1, or 8 where a few rows
 // have many parts: their loads then wait for memory at the same time).  Launched beside the kernel that writes the parts, which it
 // waits for: nothing here is read before that, and nothing through the read-only path.
@@ -512,9 +521,8 @@ __global__ void __launch_bounds__(256) combine_kernel(Args a) {
       for (int e = 0; e < 4; ++e) acc[e] += sh[w][e][lane];
     }
   }
-  const int h = (int)(row % a.Hq);
-  const long long t = row / a.Hq;
-  const int qi = (int)(t % a.Lq), b = (int)(t / a.Lq);
+  const RowAt r = row_at(a, (unsigned)row);
+  const int h = r.head, qi = r.query, b = r.clip;
   const bool any = key_length(a, b) > 0;
   const float inv = any ? 1.f / sum : 0.f;
 #pragma unroll
@@ -528,13 +536,14 @@ __global__ void __launch_bounds__(256) delta_kernel(Args a) {
   const long long rows = (long long)a.B * a.Lq * a.Hq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
-  const int h = (int)(row % a.Hq);
-  const long long t = row / a.Hq;
-  const int qi = (int)(t % a.Lq), b = (int)(t / a.Lq);
+  const RowAt r = row_at(a, (unsigned)row);
+  const int h = r.head, qi = r.query, b = r.clip;
   const T* g = reinterpret_cast<const T*>(a.g) + b * a.gs[0] + (long long)qi * a.gs[1] + h * a.gs[2];
   const T* o = reinterpret_cast<const T*>(a.o_in) + row * a.D;
   float s = 0.f;
-  for (int c = lane; c < a.D; c += 32) s = fmaf(to_f32(g[c]), to_f32(o[c]), s);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane + 32 * e < a.D) s = fmaf(to_f32(g[lane + 32 * e]), to_f32(o[lane + 32 * e]), s);
 #pragma unroll
   for (int k = 16; k >= 1; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + qi] = s;

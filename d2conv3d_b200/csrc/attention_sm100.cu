@@ -439,11 +439,18 @@ void add_rows(RowsArgs& s, int i, const Args& a, int which) {
 
 // The device's status word.  The first call registers it, which a capture in progress on this thread must not mind.
 int status_pointer(int** out) {
+  static std::atomic<int*> known[64];
+  int dev = -1;
+  D2C_CUDA_TRY(cudaGetDevice(&dev));
+  const bool kept = dev >= 0 && dev < 64;
+  if (kept && (*out = known[dev].load(std::memory_order_acquire))) return D2C_OK;
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   D2C_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
   const int rc = status_word_device_ptr(out);
   const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
-  return rc ? rc : check_cuda(back);
+  if (rc) return rc;
+  if (kept) known[dev].store(*out, std::memory_order_release);
+  return check_cuda(back);
 }
 
 // [clips, tokens, heads, D] 16-bit; a dimension of one element has no stride.

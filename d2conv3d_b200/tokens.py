@@ -12,6 +12,7 @@ import torch.nn as nn
 
 from . import _lib
 
+_NO_GRID, _UNIT_STEP = (0, 0, 0), (1.0, 1.0, 1.0)
 _LAYOUTS = {"channels_last": 0, "channels_first": 1, "tokens": 2}
 
 
@@ -42,18 +43,16 @@ def rotary_embedding_3d(x, positions, axis_dims, base=10000.0, interleaved=False
     grid_step  with a grid: cell size on each axis, position = (index + 1/2) * step - 1/2, so that the levels of a pyramid
                share one frame; 1 if None
     Differentiable in x."""
-    axis_dims = tuple(int(n) for n in axis_dims)
     if len(axis_dims) != 3:
         raise ValueError(f"axis_dims must have three entries, got {axis_dims}")
     if torch.is_tensor(positions):
         if grid_step is not None:
             raise ValueError("grid_step goes with a grid, not with positions of its own")
-        return _lib.native().rotary_embedding_3d(x, positions, (0, 0, 0), (1.0, 1.0, 1.0), axis_dims, base, interleaved)
-    grid = tuple(int(n) for n in positions)
-    step = (1.0, 1.0, 1.0) if grid_step is None else tuple(float(s) for s in grid_step)
-    if len(grid) != 3 or len(step) != 3:
+        return _lib.native().rotary_embedding_3d(x, positions, _NO_GRID, _UNIT_STEP, axis_dims, base, interleaved)
+    step = _UNIT_STEP if grid_step is None else grid_step
+    if len(positions) != 3 or len(step) != 3:
         raise ValueError("a grid and its steps have three entries")
-    return _lib.native().rotary_embedding_3d(x, None, grid, step, axis_dims, base, interleaved)
+    return _lib.native().rotary_embedding_3d(x, None, positions, step, axis_dims, base, interleaved)
 
 
 def cross_attention(query, key, value, key_lengths=None, scale=None):

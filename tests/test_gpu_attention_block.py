@@ -1,4 +1,5 @@
 """The token operators as they are used together: norm, projection, rotary positions, attention, projection."""
+import os
 import subprocess
 import sys
 
@@ -9,6 +10,7 @@ import d2conv3d_b200 as d2c
 from d2conv3d_b200.decoder import Decoder, pyramid_shapes
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def plain_block(m, x, context, lengths):
@@ -136,5 +138,5 @@ assert all(torch.equal(a, b) for a, b in zip(got, step()))
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 def test_first_calls_of_a_process_are_captured(dtype):
     # whatever a first call sets up must not disturb a capture
-    p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED % {"dtype": dtype}], capture_output=True, text=True, timeout=240)
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED % {"dtype": dtype}], capture_output=True, text=True, timeout=240, cwd=ROOT)
     assert p.returncode == 0, p.stderr[-2000:]
