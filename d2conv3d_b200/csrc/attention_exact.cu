@@ -344,12 +344,12 @@ __global__ void __launch_bounds__(kThreads) bwd_kv_kernel(Args a) {
 // ---- a few queries ------------------------------------------------------------------------------------------
 
 // R query rows (heads that share keys, times queries) against a share of the keys, which are read once.  LPK lanes hold a key's
-// channels, 16 bytes each; every such group of lanes runs a softmax of its own over every (32 / LPK * 4)-th key, four keys at a
-// time so that eight 16-byte loads are in flight; the groups meet in shared memory.  Bound by HBM where the GPU is filled.
+// channels, 16 bytes each; every such group of lanes runs a softmax of its own over some of the keys, four or eight at a time, so
+// that 8 or 16 16-byte loads are in flight; the groups meet in shuffles and shared memory.  Bound by HBM where the GPU is filled.
 constexpr int kFewThreads = 256;
 template <typename T, int LPK, int R>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {
-  constexpr int V = 16 / (int)sizeof(T), kGroups = kFewThreads / LPK, kU = 4;
+  constexpr int V = 16 / (int)sizeof(T), kGroups = kFewThreads / LPK, kU = sizeof(T) == 2 && R <= 4 && LPK <= 8 ? 8 : 4;
   next_kernel_may_start();
   const int group = a.Hq / a.Hkv, all_rows = group * a.Lq, row_sets = (all_rows + R - 1) / R;
   long long id = blockIdx.x;
@@ -499,14 +499,24 @@ __global__ void __launch_bounds__(256) combine_kernel(Args a) {
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float shift = m == -INFINITY ? 0.f : m;
   float acc[4] = {}, sum = 0.f;
-#pragma unroll (W == 1 ? 4 : 8)
-  for (int s = first; s < a.splits; s += W) {
-    const float f = exp2f(a.part_lse[s * rows + row] - shift);
-    const float* p = a.part + (s * rows + row) * a.D;
-    sum += f;
+  constexpr int kU = W == 1 ? 4 : 8;                             // parts on their way at the same time
+  for (int s0 = first; s0 < a.splits; s0 += kU * W) {
+    float f[kU], v[kU][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < a.D) acc[e] = fmaf(f, p[lane + 32 * e], acc[e]);
+    for (int u = 0; u < kU; ++u) {
+      const long long at = (s0 + u * W) * rows + row;
+      const bool in = s0 + u * W < a.splits;
+      f[u] = in ? a.part_lse[at] : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[u][e] = in && lane + 32 * e < a.D ? a.part[at * a.D + lane + 32 * e] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      f[u] = exp2f(f[u] - shift);
+      sum += f[u];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f[u], v[u][e], acc[e]);
+    }
   }
   if constexpr (W > 1) {
     __shared__ float sh[W][4][32], sums[W];

@@ -64,24 +64,19 @@ __device__ __forceinline__ void params_at(const float* p, float (&f)[VEC]) {
 // VEC neighbouring values as pairs (one instruction for two operations), where there are pairs.
 template <typename T, int VEC>
 __device__ __forceinline__ F2 value_pair(const Vec<T, VEC>& v, int i) {
-  if constexpr (sizeof(T) == 4) {
-    return f2(v.v[2 * i], v.v[2 * i + 1]);
-  } else {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[i];
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-      return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    } else {
-      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
-      return f2(h.x, h.y);
-    }
-  }
+  if constexpr (sizeof(T) == 4) return f2(v.v[2 * i], v.v[2 * i + 1]);
+  else return unpack_word<T>(reinterpret_cast<const uint32_t*>(&v)[i]);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void set_pair(Vec<T, VEC>& v, int i, F2 f) {
   float a, b;
   f2_split(f, a, b);
-  v.v[2 * i] = from_f32<T>(a);
-  v.v[2 * i + 1] = from_f32<T>(b);
+  if constexpr (sizeof(T) == 4) {
+    v.v[2 * i] = a;
+    v.v[2 * i + 1] = b;
+  } else {
+    reinterpret_cast<uint32_t*>(&v)[i] = pack_word<T>(a, b);
+  }
 }
 __device__ __forceinline__ float both_halves(F2 f) {
   float a, b;

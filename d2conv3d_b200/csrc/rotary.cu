@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) rotary_kernel(Rot
       v0 = start + i + (axis[0] < 3 ? a.n[axis[0]] : a.dim - start) / 2;
     }
   }
-  const bool turns = axis[0] < 3;                                // a thread whose first pair stays has none that turns
+  const bool turns = axis[0] < 3, all_turn = axis[V - 1] < 3;    // sections come in order
   for (long long tok = (long long)blockIdx.x * blockDim.y + threadIdx.y; tok < a.tokens; tok += (long long)gridDim.x * blockDim.y) {
     const long long b = tok / a.length;
     const int l = (int)(tok - b * a.length);
@@ -108,12 +108,30 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) rotary_kernel(Rot
         if (turns) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            T& ru = kInterleaved ? p[h].v[2 * e] : p[h].v[e];
-            T& rv = kInterleaved ? p[h].v[2 * e + 1] : q[kInterleaved ? 0 : h].v[e];
-            const float u = to_f32(ru), v = to_f32(rv);
-            if (!kInterleaved || axis[e] < 3) {                  // what stays keeps its bits
-              ru = from_f32<T>(u * c[e] - v * s[e]);
-              rv = from_f32<T>(u * s[e] + v * c[e]);
+            if constexpr (kInterleaved && sizeof(T) == 2) {        // a pair is a word
+              uint32_t& w = reinterpret_cast<uint32_t*>(&p[h])[e];
+              float u, v;
+              f2_split(unpack_word<T>(w), u, v);
+              const uint32_t r = pack_word<T>(u * c[e] - v * s[e], u * s[e] + v * c[e]);
+              if (all_turn || axis[e] < 3) w = r;                  // what stays keeps its bits
+            } else if constexpr (!kInterleaved && sizeof(T) == 2 && V % 2 == 0) {
+              if (e % 2 == 0) {                                    // two pairs are two words
+                uint32_t& wu = reinterpret_cast<uint32_t*>(&p[h])[e / 2];
+                uint32_t& wv = reinterpret_cast<uint32_t*>(&q[h])[e / 2];
+                float u0, u1, v0, v1;
+                f2_split(unpack_word<T>(wu), u0, u1);
+                f2_split(unpack_word<T>(wv), v0, v1);
+                wu = pack_word<T>(u0 * c[e] - v0 * s[e], u1 * c[e + 1] - v1 * s[e + 1]);
+                wv = pack_word<T>(u0 * s[e] + v0 * c[e], u1 * s[e + 1] + v1 * c[e + 1]);
+              }
+            } else {
+              T& ru = kInterleaved ? p[h].v[2 * e] : p[h].v[e];
+              T& rv = kInterleaved ? p[h].v[2 * e + 1] : q[kInterleaved ? 0 : h].v[e];
+              const float u = to_f32(ru), v = to_f32(rv);
+              if (!kInterleaved || all_turn || axis[e] < 3) {
+                ru = from_f32<T>(u * c[e] - v * s[e]);
+                rv = from_f32<T>(u * s[e] + v * c[e]);
+              }
             }
           }
         }

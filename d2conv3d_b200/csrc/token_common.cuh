@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "d2c_common.cuh"
 
 namespace d2c {
@@ -72,6 +74,24 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Two 16-bit values of one word, and back (one conversion for both).
+template <typename T>
+__device__ __forceinline__ F2 unpack_word(uint32_t w) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return f2(h.x, h.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_word(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
