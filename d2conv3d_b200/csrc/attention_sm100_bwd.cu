@@ -16,6 +16,9 @@
 // 8 working warps, a thread a row and half of the columns.  With both, shared memory holds X and one Y1 and one Y2 of 64 rows: the next
 // are loaded when these are done.
 //
+// 2 clips of 3240 queries and up to 12960 keys, 4 heads of 64 in bf16: keys 183 us, queries 152 us, with tiles of 128 x 64 and two blocks a
+// SM; with one block of 128 x 128 tiles 212 and 162.
+//
 // fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
 // they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, is at most 2^14) and the sums scaled back.
 #include <algorithm>
