@@ -20,7 +20,7 @@
 // SM; with one block of 128 x 128 tiles 212 and 162.
 //
 // fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
-// they are rounded (P by 2^14; dS so that 2 D max|grad_o| max|v|, which bounds it, is at most 2^14) and the sums scaled back.
+// they are rounded (P by 2^14; dS so that D max|grad_o| max|v| / 2, which bounds it, is at most 2^15) and the sums scaled back.
 #include <algorithm>
 #include <type_traits>
 
@@ -97,9 +97,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
     const int n_heads = p.B * p.Hkv;
     const float most_v = __uint_as_float(q[2 * n_heads]), most_g = __uint_as_float(q[3 * n_heads]);
-    // |dS| <= |dP| + |delta| <= 2 D most_v most_g, taken by exponents: the product itself may be beyond fp32
+    // dS_j = p_j ((1 - p_j) dP_j - sum of the other p_k dP_k), and the other p_k add up to 1 - p_j: |dS| <= 2 p (1 - p) max |dP| <=
+    // D most_v most_g / 2.  That is brought to 2^15 at most, half of what fp16 holds: with many keys p is 1 / keys, and what a second part
+    // has left of dS must not sink below fp16's smallest.  By exponents: the product itself may be beyond fp32.
     if (most_v > 0.f && most_g > 0.f)
-      e_ds = max(-126, min(126, 14 - (ilogbf(most_v) + ilogbf(most_g) + 2 + ilogbf((float)(4 * p.D - 1)))));
+      e_ds = max(-126, min(126, 15 - (ilogbf(most_v) + ilogbf(most_g) + ilogbf((float)(4 * p.D - 1)))));
     if constexpr (kParts == 2) {
       e_q = scale_exponent(q[0]);
       e_k = scale_exponent(q[n_heads]);

@@ -323,3 +323,25 @@ def test_refusals():
     wide = torch.zeros(1, 2, 1, 136, device="cuda")
     with pytest.raises(RuntimeError, match="1 to 128"):
         d2c.cross_attention(wide, wide, wide)
+
+
+@pytest.mark.parametrize("keys", [32768, 262144])
+def test_fp32_gradients_of_many_keys(keys):
+    # Probabilities of about 1 / keys: the score gradients are far below the bound that their scale is taken from.  Values and gradients
+    # of +-1 give that bound its largest distance.  Scores of std 8 * 2^-5 * 2^-3: p keys is 1 within some per cent.
+    # Tolerance, 2-norm: a chain of at most 72 products whose sums are truncated to 24 bits, each by at most 2^-23 of the result: 2^-16.8;
+    # the second parts of dS: scaled by 2^8 (15 - ilogb(255)), dS has rms 8 * 2^8 / keys, at 2^18 keys 2^-7, and a step of 2^-24 leaves
+    # 2^-25.8 of it: 2^-18.8.  Together 1.1e-5 (a scale that is smaller by 2^3 alone leaves 2^-15.8, 1.8e-5).
+    gen = torch.Generator().manual_seed(7)
+    sign = lambda *s: (torch.randint(0, 2, s, generator=gen) * 2 - 1).float().cuda()  # noqa: E731
+    n, d = max(6, 2 ** 20 // keys), 64
+    q = (torch.randn(1, n, 1, d, generator=gen) / 32).cuda()
+    k = torch.randn(1, keys, 1, d, generator=gen).cuda()
+    v, g = sign(1, keys, 1, d), sign(1, n, 1, d)
+    got = run(q, k, v, g)
+    leaves = [t.double().requires_grad_() for t in (q, k, v)]
+    p = torch.softmax(torch.einsum("bqhd,bkhd->bhqk", leaves[0], leaves[1]) * d ** -0.5, -1)
+    o = torch.einsum("bhqk,bkhd->bqhd", p, leaves[2])
+    want = (o.detach(),) + torch.autograd.grad(o, leaves, g.double())
+    for name, a, e in zip(("o", "grad_q", "grad_k", "grad_v"), got, want):
+        assert float((a.double() - e).norm() / e.norm()) <= 1.1e-5, name
