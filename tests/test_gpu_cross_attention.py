@@ -345,3 +345,12 @@ def test_fp32_gradients_of_many_keys(keys):
     want = (o.detach(),) + torch.autograd.grad(o, leaves, g.double())
     for name, a, e in zip(("o", "grad_q", "grad_k", "grad_v"), got, want):
         assert float((a.double() - e).norm() / e.norm()) <= 1.1e-5, name
+
+
+def test_fp32_gradients_of_many_keys_in_parts():
+    before = d2c.get_math_mode()
+    try:
+        d2c.set_math_mode("bf16x3")        # whatever "auto" takes for so many keys
+        test_fp32_gradients_of_many_keys(262144)
+    finally:
+        d2c.set_math_mode(before)
