@@ -37,6 +37,30 @@ inline Tensor bytes_on(size_t n, const Tensor& t) {
 }
 inline void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// A tensor that a node keeps for its backward.  Saved-tensor hooks decide what comes back: another layout is for the caller to deal with
+// (contiguous(), or fresh strides), another size, type or device is refused here, since the kernels go by the forward's sizes.
+class Saved {
+ public:
+  Saved() = default;
+  Saved(const Tensor& t, bool is_output)
+      : variable_(t, is_output), sizes_(t.sizes().begin(), t.sizes().end()), type_(t.scalar_type()), device_(t.device()) {}
+  Tensor unpack(std::shared_ptr<Node> owner = nullptr) const {
+    Tensor t = variable_.unpack(std::move(owner));
+    if (t.defined())
+      TORCH_CHECK(t.sizes() == at::IntArrayRef(sizes_) && t.scalar_type() == type_ && t.device() == device_ && t.layout() == at::kStrided,
+                  "a saved tensor came back from its hooks as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(),
+                  ": it was saved as ", type_, " ", at::IntArrayRef(sizes_), " on ", device_);
+    return t;
+  }
+  void reset() { variable_.reset_data(); }
+
+ private:
+  SavedVariable variable_;
+  at::DimVector sizes_;
+  at::ScalarType type_ = at::kFloat;
+  at::Device device_ = at::kCUDA;
+};
+
 // Results of a backward node: gradients are computed outside the graph, so a second derivative has to fail loudly.
 inline variable_list once_differentiable(variable_list&& grads) {
   if (!at::GradMode::is_enabled()) return std::move(grads);

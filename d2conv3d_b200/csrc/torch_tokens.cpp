@@ -29,13 +29,13 @@ struct LayerNormNode : public Node {
   bool has_bias, empty;
   at::TensorOptions param_options;
   std::vector<int64_t> shape;
-  SavedVariable x, weight;
+  Saved x, weight;
   Tensor stats;
 
   std::string name() const override { return "D2CLayerNormBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data(); weight.reset_data();
+    x.reset(); weight.reset();
     stats = Tensor();
   }
 
@@ -50,6 +50,7 @@ struct LayerNormNode : public Node {
     {
       at::AutoGradMode no_grad(false);
       c10::cuda::CUDAGuard guard(xv.device());
+      xv = xv.contiguous(); wv = contiguous(wv);
       if (task_should_compute_output(0)) gx = at::empty(shape, xv.options().requires_grad(false));
       if (wv.defined() && task_should_compute_output(1)) gw = at::empty({desc.channels}, param_options);
       if (has_bias && task_should_compute_output(2)) gb = at::empty({desc.channels}, param_options);
@@ -123,8 +124,8 @@ Tensor layer_norm(const Tensor& input, const OptTensor& weight_, const OptTensor
     node->desc = d; node->has_bias = bias.defined(); node->empty = empty;
     node->shape = input.sizes().vec();
     if (p.defined()) node->param_options = p.options().requires_grad(false);
-    node->x = SavedVariable(x, false);
-    if (w.defined()) node->weight = SavedVariable(w, false);
+    node->x = Saved(x, false);
+    if (w.defined()) node->weight = Saved(w, false);
     node->stats = stats;
     torch::autograd::set_history(y, node);
   }
@@ -163,12 +164,12 @@ Tensor rotate(const Tensor& input, Rotary r, bool inverse) {
 
 struct RotaryNode : public Node {
   d2c_rotary_desc desc;
-  SavedVariable positions;
+  Saved positions;
 
   std::string name() const override { return "D2CRotaryEmbedding3dBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    positions.reset_data();
+    positions.reset();
   }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined()) return variable_list(1);
@@ -181,6 +182,7 @@ struct RotaryNode : public Node {
     {
       at::AutoGradMode no_grad(false);
       c10::cuda::CUDAGuard guard(grads[0].device());
+      r.positions = contiguous(r.positions);
       gx = rotate(grads[0], r, true);
     }
     return once_differentiable({gx});
@@ -248,7 +250,7 @@ Tensor rotary(const Tensor& x, const OptTensor& positions_, const std::array<int
     auto node = std::shared_ptr<RotaryNode>(new RotaryNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x));
     node->desc = d;
-    if (r.positions.defined()) node->positions = SavedVariable(r.positions, false);
+    if (r.positions.defined()) node->positions = Saved(r.positions, false);
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -273,13 +275,13 @@ void take_strides(int64_t (&out)[3], const Tensor& t) {
 struct AttentionNode : public Node {
   d2c_attention_desc desc;
   bool empty;
-  SavedVariable q, k, v, lengths, o;
+  Saved q, k, v, lengths, o;
   Tensor lse;
 
   std::string name() const override { return "D2CCrossAttentionBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    q.reset_data(); k.reset_data(); v.reset_data(); lengths.reset_data(); o.reset_data();
+    q.reset(); k.reset(); v.reset(); lengths.reset(); o.reset();
     lse = Tensor();
   }
   variable_list apply(variable_list&& grads) override {
@@ -293,6 +295,8 @@ struct AttentionNode : public Node {
     {
       at::AutoGradMode no_grad(false);
       c10::cuda::CUDAGuard guard(qv.device());
+      // saved-tensor hooks may have laid the tensors out anew: the strides are those of what came back
+      qv = attention_rows(qv); kv = attention_rows(kv); vv = attention_rows(vv); nv = contiguous(nv); ov = ov.contiguous();
       gq = at::empty(qv.sizes(), qv.options().requires_grad(false));
       gk = at::empty(kv.sizes(), kv.options().requires_grad(false));
       gv = at::empty(vv.sizes(), vv.options().requires_grad(false));
@@ -301,7 +305,7 @@ struct AttentionNode : public Node {
       } else {
         const Tensor g = attention_rows(grads[0]);
         d2c_attention_desc d = desc;
-        take_strides(d.g_stride, g);
+        take_strides(d.q_stride, qv); take_strides(d.k_stride, kv); take_strides(d.v_stride, vv); take_strides(d.g_stride, g);
         const size_t n = d2c_attention_bwd_workspace_bytes(&d);
         const Tensor ws = bytes_on(n, qv);
         check(d2c_attention_bwd(&d, ptr(g), ptr(qv), ptr(kv), ptr(vv), ptr(nv), ptr(ov), ptr(lv), ptr(gq), ptr(gk), ptr(gv),
@@ -365,13 +369,13 @@ Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& val
     auto node = std::shared_ptr<AttentionNode>(new AttentionNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(query, key, value));
     node->desc = d; node->empty = empty;
-    node->q = SavedVariable(q, false);
-    node->k = SavedVariable(k, false);
-    node->v = SavedVariable(v, false);
-    if (n.defined()) node->lengths = SavedVariable(n, false);
+    node->q = Saved(q, false);
+    node->k = Saved(k, false);
+    node->v = Saved(v, false);
+    if (n.defined()) node->lengths = Saved(n, false);
     node->lse = lse;
     torch::autograd::set_history(o, node);
-    node->o = SavedVariable(o, true);
+    node->o = Saved(o, true);
   }
   return o;
 }
