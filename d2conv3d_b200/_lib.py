@@ -245,6 +245,16 @@ def profile_read(max_records=65536):
     return [(recs[i].name.decode(), float(recs[i].ms)) for i in range(n.value)]
 
 
+def _came_back(t, saved):
+    """A tensor that a backward goes by, as its saved-tensor hooks returned it: contiguous, and refused if it is another one."""
+    if t is None:
+        return None
+    if (t.shape, t.dtype, t.device) != saved:
+        raise RuntimeError(f"a saved tensor came back from its hooks as {t.dtype} {tuple(t.shape)} on {t.device}: it was saved as "
+                           f"{saved[1]} {tuple(saved[0])} on {saved[2]}")
+    return t.contiguous()
+
+
 class _ActGroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, relu):
@@ -262,12 +272,13 @@ class _ActGroupNorm(torch.autograd.Function):
                                            1 if relu else 0, ptr(stats), n, stream_of(x)), "act_group_norm")
         ctx.save_for_backward(x, weight, stats)
         ctx.cfg = (B, C, spatial, groups, float(eps), 1 if relu else 0, bias is not None)
+        ctx.saved = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, weight, stats)]
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, weight, stats = ctx.saved_tensors
+        x, weight, stats = (_came_back(t, what) for t, what in zip(ctx.saved_tensors, ctx.saved))
         B, C, spatial, groups, eps, relu, has_bias = ctx.cfg
         gy = gy.contiguous()
         L = lib()

@@ -106,7 +106,7 @@ struct DeformNode : public Node {
   d2c_head_desc head;
   int field_mode;
   bool has_bias;
-  SavedVariable x, geo, mask, weight;
+  Saved x, geo, mask, weight;
   Tensor cache_buf;
   d2c_sample_cache cache{};
 
@@ -116,7 +116,7 @@ struct DeformNode : public Node {
   // own nodes do; the pass itself works on its own references.
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data(); geo.reset_data(); mask.reset_data(); weight.reset_data();
+    x.reset(); geo.reset(); mask.reset(); weight.reset();
     cache_buf = Tensor();
     cache = d2c_sample_cache{};
   }
@@ -138,6 +138,7 @@ struct DeformNode : public Node {
       at::AutoGradMode no_grad(false);
       c10::cuda::CUDAGuard guard(xv.device());
       const Tensor gy = grads[0].contiguous();
+      xv = xv.contiguous(); gv = gv.contiguous(); mv = contiguous(mv); wv = wv.contiguous();
       gx = like(xv); ggeo = like(gv); gmask = like(mv); gw = like(wv);
       if (has_bias) gbias = at::empty({wv.size(0)}, wv.options());
       const int op = (kind == Kind::field || kind == Kind::head_field) ? D2C_OP_DYNDIL_BWD : D2C_OP_DEFORM_BWD;
@@ -237,10 +238,10 @@ Tensor run_deform(Kind kind, const d2c_conv_desc& desc, const d2c_head_desc& hea
       node->set_next_edges(torch::autograd::collect_next_edges(input, geo, mask, weight, bias));
     node->kind = kind; node->desc = desc; node->head = head; node->field_mode = field_mode;
     node->has_bias = bias.defined();
-    node->x = SavedVariable(x, false);
-    node->geo = SavedVariable(g, false);
-    if (m.defined()) node->mask = SavedVariable(m, false);
-    node->weight = SavedVariable(w, false);
+    node->x = Saved(x, false);
+    node->geo = Saved(g, false);
+    if (m.defined()) node->mask = Saved(m, false);
+    node->weight = Saved(w, false);
     if (cache.format) {           // nothing kept: the buffer is released here
       node->cache = cache;
       node->cache_buf = cache_buf;
@@ -396,12 +397,12 @@ Tensor deform_conv1d(Tensor input, Tensor offset, const OptTensor& alpha_, Tenso
 struct DepthwiseNode : public Node {
   d2c_conv_desc desc;
   bool has_bias, unbatched;
-  SavedVariable x, weight;
+  Saved x, weight;
 
   std::string name() const override { return "D2CDepthwiseConv3dBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data(); weight.reset_data();
+    x.reset(); weight.reset();
   }
 
   variable_list apply(variable_list&& grads) override {
@@ -415,6 +416,7 @@ struct DepthwiseNode : public Node {
     {
       at::AutoGradMode no_grad(false);
       c10::cuda::CUDAGuard guard(xv.device());
+      xv = xv.contiguous(); wv = wv.contiguous();
       const Tensor gy = (unbatched ? grads[0].unsqueeze(0) : grads[0]).contiguous();
       if (task_should_compute_output(0)) gx = like(xv);
       Tensor ws;
@@ -472,8 +474,8 @@ Tensor depthwise_conv3d(const Tensor& input, const Tensor& weight, const OptTens
     auto node = std::shared_ptr<DepthwiseNode>(new DepthwiseNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(input, weight, bias));
     node->desc = desc; node->has_bias = bias.defined(); node->unbatched = unbatched;
-    node->x = SavedVariable(x, false);
-    node->weight = SavedVariable(w, false);
+    node->x = Saved(x, false);
+    node->weight = Saved(w, false);
     torch::autograd::set_history(y, node);
   }
   return y;

@@ -49,8 +49,37 @@ def attention(dtype, layout):
     return [q, kv], lambda: d2c.cross_attention(q.transpose(1, 2), kv[:, :, 0], kv[:, :, 1], key_lengths=n)
 
 
+def layer(dtype, kind):
+    from d2conv3d_b200.dconv_native import modules
+    cls, kw = {"offsets": (modules.MDConv3d, dict(init="random", fused_head=False)), "head": (modules.MDConv3d, dict(init="random")),
+               "field": (modules.XYZSizeConditionedMDConv3d, dict(init="random", fused_head=False))}[kind]
+    m = cls(64, 64, 3, padding=1, **kw).cuda()
+    x = torch.randn(1, 64, 3, 6, 7, device="cuda", requires_grad=True)
+    return [x] + list(m.parameters()), lambda: m(x)
+
+
+def conv1d(dtype, _):
+    x = torch.randn(2, 8, 33, device="cuda", requires_grad=True)
+    off, w = torch.randn(2, 3, 33, device="cuda", requires_grad=True), torch.randn(6, 8, 3, device="cuda", requires_grad=True)
+    return [x, off, w], lambda: d2c.dconv_native._ops.deform_conv1d(x, off, None, w, None, 1, 1, 1, 1, 1)
+
+
+def depthwise(dtype, _):
+    m = d2c.DepthwiseConv3d(16, 16, 3, padding=1, groups=16).cuda().to(dtype)
+    x = torch.randn(2, 16, 4, 6, 8, device="cuda").to(dtype).requires_grad_()
+    return [x] + list(m.parameters()), lambda: m(x)
+
+
+def act_group_norm(dtype, _):
+    x = torch.randn(2, 16, 4, 6, 8, device="cuda", requires_grad=True)
+    w, b = (torch.randn(16, device="cuda", requires_grad=True) for _ in range(2))
+    return [x, w, b], lambda: d2c._lib.act_group_norm(x, w, b, 1)
+
+
 CASES = [(norm, "channels_last"), (norm, "channels_first"), (norm, "tokens"), (rotary, ""), (attention, "many"), (attention, "few")]
 IDS = ["norm_rows", "norm_volume", "norm_tokens", "rotary", "attention", "attention_few"]
+CONVOLUTIONS = [(layer, "offsets"), (layer, "head"), (layer, "field"), (conv1d, ""), (depthwise, ""), (act_group_norm, "")]
+CONVOLUTION_IDS = ["offsets", "head", "field", "conv1d", "depthwise", "act_group_norm"]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
@@ -77,4 +106,31 @@ def test_another_tensor_is_refused(case, change):
     with saved_tensors_hooks(kept, back):
         y = call()
     with pytest.raises(RuntimeError, match="saved tensor came back"):
+        torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("case", CONVOLUTIONS, ids=CONVOLUTION_IDS)
+def test_convolutions_take_the_layout_that_comes_back(case):
+    torch.manual_seed(0)
+    leaves, call = case[0](torch.float32, case[1])
+    with torch.no_grad():
+        g = torch.randn_like(call())
+    want = torch.autograd.grad(call(), leaves, g)
+    for name, hooks in HOOKS.items():
+        with hooks():
+            y = call()
+        for a, b in zip(torch.autograd.grad(y, leaves, g), want):
+            # the gradients of a deformable layer's input are sums by atomics: fp32 sums of some hundred terms in another order
+            assert (a - b).abs().max() <= 1e-5 * b.abs().max(), name
+
+
+@pytest.mark.parametrize("case", CONVOLUTIONS, ids=CONVOLUTION_IDS)
+@pytest.mark.parametrize("change", ["size", "type", "device"])
+def test_convolutions_refuse_another_tensor(case, change):
+    torch.manual_seed(0)
+    leaves, call = case[0](torch.float32, case[1])
+    back = {"size": lambda t: t[:1], "type": lambda t: t.double(), "device": lambda t: t.cpu()}[change]
+    with saved_tensors_hooks(kept, lambda t: back(t) if t.numel() != t[:1].numel() or change != "size" else t.flatten()):
+        y = call()
+    with pytest.raises(RuntimeError, match="came back"):
         torch.autograd.grad(y, leaves, torch.ones_like(y))
