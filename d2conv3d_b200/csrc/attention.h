@@ -14,6 +14,7 @@ struct Args {
   void *o, *gq, *gk, *gv;
   float* lse;                            // [B, Hq, Lq]: log2 of the sum of exp2(scores in log2 units); -inf without keys
   float* delta;                          // [B, Hq, Lq]: sum_d grad_o * o
+  int* g_exp;                            // [B, Hq, Lq]: grad_o 2^g_exp has its largest element in 2^14 .. 2^15; NULL where operands are bf16
   const void* lengths;
   int lengths_i64;
   int B, Lq, Lk, Hq, Hkv, D;
@@ -32,6 +33,12 @@ __device__ __forceinline__ int key_length(const Args& a, int b) {
   return (int)(n < 0 ? 0 : (n > a.Lk ? a.Lk : n));
 }
 
+// Exponent e that brings a largest element to 2^14 .. 2^15 (bits of a float, as largest_sizes writes it; 0: all are zero).
+__device__ __forceinline__ int scale_exponent(uint32_t size) {
+  const float f = __uint_as_float(size);
+  return f > 0.f ? max(-126, min(126, 14 - ilogbf(f))) : 0;
+}
+
 // Share [begin, end) of n items, of `splits`.
 __device__ __forceinline__ void share(int n, int splits, int s, int& begin, int& end) {
   begin = (int)((long long)n * s / splits);
@@ -45,7 +52,7 @@ int few_fwd(int dtype, const Args& a, cudaStream_t st);          // needs 16-byt
 int exact_bwd_q(int dtype, const Args& a, cudaStream_t st);
 int exact_bwd_kv(int dtype, const Args& a, cudaStream_t st);
 int combine(int dtype, const Args& a, cudaStream_t st);          // partial outputs -> o, lse
-int delta_rows(int dtype, const Args& a, cudaStream_t st);
+int delta_rows(int dtype, const Args& a, cudaStream_t st);       // delta, g_exp
 int sum_parts(int dtype, const float* part, int splits, long long n, void* out0, void* out1, cudaStream_t st);   // out1: NULL, or a second sum
 
 // ---- tensor cores: operands with positive strides and 16-byte rows, scale > 0

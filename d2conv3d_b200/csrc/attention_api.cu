@@ -143,6 +143,9 @@ size_t fwd_workspace(const d2c_attention_desc& d, int mode, int sms) {
 }
 
 size_t delta_bytes(const d2c_attention_desc& d) { return align_up(sizeof(float) * q_rows(d), 256); }
+// Rows' exponents, where operands are fp16.
+bool scaled_rows(const d2c_attention_desc& d, int parts) { return parts == 2 || (parts && d.dtype == D2C_F16); }
+size_t exponent_bytes(const d2c_attention_desc& d, int parts) { return scaled_rows(d, parts) ? align_up(sizeof(int) * q_rows(d), 256) : 0; }
 size_t staged_bytes(const d2c_attention_desc& d, int parts) {
   if (d.dtype != D2C_F32 || !parts) return 0;
   return 2 * split_bytes(d.batch, d.queries, d.q_heads, d.dim, parts) + 2 * split_bytes(d.batch, d.keys, d.kv_heads, d.dim, parts);
@@ -151,7 +154,7 @@ size_t bwd_bytes(const d2c_attention_desc& d, const Plan& pq, const Plan& pk) {
   size_t part = 0;                    // one gradient kernel's shares at a time
   if (pq.splits > 1) part = std::max<size_t>(part, sizeof(float) * pq.splits * q_rows(d) * d.dim);
   if (pk.splits > 1) part = std::max<size_t>(part, sizeof(float) * 2 * pk.splits * kv_rows(d) * d.dim);
-  return delta_bytes(d) + bound_bytes(d) + staged_bytes(d, pq.parts) + align_up(part, 256);
+  return delta_bytes(d) + exponent_bytes(d, pq.parts) + bound_bytes(d) + staged_bytes(d, pq.parts) + align_up(part, 256);
 }
 size_t bwd_workspace(const d2c_attention_desc& d, int mode, int sms) {
   size_t n = 0;
@@ -227,18 +230,22 @@ int run_bwd(const d2c_attention_desc& d, Args a, int mode, void* workspace, int 
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.delta = reinterpret_cast<float*>(ws);
   ws += delta_bytes(d);
+  if (scaled_rows(d, pk.parts)) {
+    a.g_exp = reinterpret_cast<int*>(ws);
+    ws += exponent_bytes(d, pk.parts);
+  }
   uint32_t* bounds = reinterpret_cast<uint32_t*>(ws);
   ws += bound_bytes(d);
   Operand x[4];
   own_operands(a, x);
   int rc;
-  if (tensor && (d.dtype == D2C_F16 || pk.parts == 2) && (rc = largest_sizes(d.dtype, a, d.dtype == D2C_F16, bounds, st))) return rc;
+  if ((rc = delta_rows(d.dtype, a, st))) return rc;
+  if (scaled_rows(d, pk.parts) && (rc = largest_sizes(d.dtype, a, d.dtype == D2C_F16, bounds, st))) return rc;
   if (tensor && d.dtype == D2C_F32) {
     if ((rc = split_rows(a, pk.parts, bounds, ws, x, st))) return rc;
     ws += staged_bytes(d, pk.parts);
   }
   a.part = reinterpret_cast<float*>(ws);
-  if ((rc = delta_rows(d.dtype, a, st))) return rc;
   a.splits = pk.splits;
   if ((rc = tensor ? tc_bwd(d.dtype, a, x, pk.parts, true, bounds, st) : exact_bwd_kv(d.dtype, a, st))) return rc;
   if (a.splits > 1) {

@@ -551,13 +551,26 @@ __global__ void __launch_bounds__(256) delta_kernel(Args a) {
   const int h = r.head, qi = r.query, b = r.clip;
   const T* g = reinterpret_cast<const T*>(a.g) + b * a.gs[0] + (long long)qi * a.gs[1] + h * a.gs[2];
   const T* o = reinterpret_cast<const T*>(a.o_in) + row * a.D;
-  float s = 0.f;
+  float s = 0.f, most = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < a.D) s = fmaf(to_f32(g[lane + 32 * e]), to_f32(o[lane + 32 * e]), s);
+  for (int e = 0; e < 4; ++e) {
+    if (lane + 32 * e < a.D) {
+      const float f = to_f32(g[lane + 32 * e]);
+      s = fmaf(f, to_f32(o[lane + 32 * e]), s);
+      if (fabsf(f) < INFINITY) most = fmaxf(most, fabsf(f));     // as largest_sizes takes them
+    }
+  }
 #pragma unroll
-  for (int k = 16; k >= 1; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-  if (lane == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + qi] = s;
+  for (int k = 16; k >= 1; k >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, k);
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
+  }
+  if (lane == 0) {
+    const long long at = ((long long)b * a.Hq + h) * a.Lq + qi;
+    a.delta[at] = s;
+    // a row of zeros: the largest exponent, so that no other row is measured by it
+    if (a.g_exp) a.g_exp[at] = most > 0.f ? scale_exponent(__float_as_uint(most)) : 126;
+  }
 }
 
 // out[y] = sum of `splits` parts of n values each, part[y]'s one behind the other; y = blockIdx.y.  Launched beside the kernel that

@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(256) bound_kernel(const __grid_constant__ Rows
   }
 }
 
-// x fp32 with any strides -> [parts][B, L, H, width]: fp16 hi and lo of x 2^e, or bf16; zeros from D on.  A thread writes 8 channels.
+// x fp32 with any strides -> [parts][B, L, H, width]: fp16 hi and lo of x 2^e (e of the clip and key head, grad_o: of the row), or bf16;
+// zeros from D on.  A thread writes 8 channels.
 __global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__ RowsArgs a) {
   const int t = blockIdx.y, L = a.L[t], H = a.H[t], per = a.width / 8;
   const long long n = (long long)a.B * L * H * per;
@@ -402,7 +403,8 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__
     }
     uint32_t hi[4], lo[4];
     if (a.parts == 2) {
-      const float up = pow2(scale_exponent(a.bounds[((long long)a.which[t] * a.B + b) * a.a.Hkv + h / (H / a.a.Hkv)]));
+      const float up = pow2(a.which[t] == 3 ? a.a.g_exp[((long long)b * H + h) * L + l]
+                                            : scale_exponent(a.bounds[((long long)a.which[t] * a.B + b) * a.a.Hkv + h / (H / a.a.Hkv)]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x0 = f[2 * e] * up, x1 = f[2 * e + 1] * up;
@@ -493,7 +495,8 @@ int largest_sizes(int dtype, const Args& a, bool values_only, uint32_t* bounds, 
   return D2C_OK;
 }
 
-// Stages fp32 q, k, v and, if it is there, grad_o; o[0..3] become the staged operands.  Two parts: largest_sizes before.
+// Stages fp32 q, k, v and, if it is there, grad_o; o[0..3] become the staged operands.  Two parts: largest_sizes, and delta_rows for
+// grad_o, before.
 int split_rows(const Args& a, int parts, uint32_t* bounds, void* workspace, Operand (&o)[4], cudaStream_t st) {
   RowsArgs s = rows_args(a, bounds);
   s.parts = parts;

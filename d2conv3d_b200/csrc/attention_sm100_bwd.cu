@@ -19,8 +19,16 @@
 // 2 clips of 3240 queries and up to 12960 keys, 4 heads of 64 in bf16: keys 183 us, queries 152 us, with tiles of 128 x 64 and two blocks a
 // SM; with one block of 128 x 128 tiles 212 and 162.
 //
-// fp16: a probability is of the order of 1 / keys, and score gradients are smaller still; both are scaled by powers of two before
-// they are rounded (P by 2^14; dS so that D max|grad_o| max|v| / 2, which bounds it, is at most 2^15) and the sums scaled back.
+// fp16 operands: a probability is of the order of 1 / keys, score gradients are smaller still, and both go with what a loss makes of its
+// queries, which may differ by any power of two.  So a row of X has a power of two of its own, 2^lift, that follows the largest of its
+// P_xy g_y so far, or a tile's sum of them (g_y: the size of that query's grad_o against the largest; 1 in the queries' kernel, where the
+// row is the query): a tile that brings far more takes the row's sums back by the difference, as a running softmax does.  Under that
+// scale |dS| <= 2^15, since |dP - delta| <= 2 D max|g_y| max|v|; dS typically lies 2^7 below that, and the second part ends at 2^-24.  fp32
+// tensors are staged with every query's grad_o at its own exponent: P g_y takes P's place and is scaled alike.  P itself, for fp16
+// tensors, is scaled by 2^14.  Whatever the sizes of grad_o and the number of keys (3240 .. 1000000), fp32 gradients are 0.6e-6 ..
+// 1.9e-6 (2-norm) from 64 bits; one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  It
+// costs 6 % of these kernels in two parts of 64 channels and 12 % of the fp16 keys' kernel of 64 (208 us with one scale, 233 with
+// the rows').
 #include <algorithm>
 #include <type_traits>
 
@@ -37,11 +45,17 @@ struct BwdParams {
   int splits, blocks_x;          // tiles of X per head
   const float *lse, *delta;
   const uint32_t* bounds;        // fp16: see largest_sizes
+  const int* g_exp;              // fp16: see Args
   void *g1, *g2;                 // keys: grad_v, grad_k; queries: g2 = grad_q
   float* part;                   // queries [splits][B, Lq, Hq][D]; keys [grad_k, grad_v][splits][B, Lk, Hkv][D]
   Args a;                        // lengths
   int* status;
 };
+
+// P of a row adds up to 1 over its keys, so that dS_j = p_j ((1 - p_j) dP_j - sum of the other p_k dP_k) is at most max|dP| / 2, a quarter of
+// what 2^e_one brings to 1: 2^17 keep it within 2^15.  With one part that does for the queries' kernel: 11 bits of dS down to p =
+// 2^-24 where dP is 2^7 below its bound.
+constexpr int kFixedLift = 17;
 
 constexpr int y_rows(int size) { return size == 128 ? 128 : 64; }    // size: channels (64, 128) times parts
 template <int DP, int kParts>
@@ -55,6 +69,19 @@ constexpr int kYBytes = kYRows<DP, kParts> * DP * 2 * kParts;
 template <int DP, int kParts>
 constexpr int kSmem = 2 * kTileBytes<DP> * kParts + kStages<DP, kParts> * kYBytes<DP, kParts> + 1024;
 
+__device__ __forceinline__ void lift_row(uint32_t (&s)[2][32], int lift) {
+  const F2 mul = f2(pow2(lift), pow2(lift));
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float x, y;
+      f2_split(mul2(f2(__uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1])), mul), x, y);
+      s[k][e] = __float_as_uint(x);
+      s[k][e + 1] = __float_as_uint(y);
+    }
+}
+
 template <typename T, typename Out, int DP, int kParts, bool kKeys>
 __global__ void __launch_bounds__(kThreads<DP, kParts>, DP * kParts == 64 ? 2 : 1)
 bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2, const __grid_constant__ CUtensorMap my1,
@@ -64,10 +91,13 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   constexpr int kMmaWarp = kWork, kLoadWarp = kWork + 1, kCols = kY == 64 && DP == 64 ? 256 : 512;
   constexpr bool kApart = kParts == 2 && DP == 64;                        // tensor memory has room for sums of lo parts
   constexpr bool kHalf = std::is_same_v<T, __half>;
-  constexpr float kUp = kHalf ? 14.f : 0.f;       // P is scaled by 2^kUp
+  constexpr int kUp = kHalf && kKeys && kParts == 1 ? 14 : 0;             // P is scaled by 2^kUp
+  constexpr bool kLift = kHalf && (kKeys || kParts == 2);                 // a row's scale follows what it meets; else it is 2^kFixedLift
+  constexpr bool kShared = kLift && kY == 128;    // a row's columns belong to two threads
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kSt + 8];
-  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][2][kY];     // lse - kUp, delta of the queries of a Y tile
+  __shared__ uint64_t bars[2 * kSt + 12];
+  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][kHalf && kParts == 1 ? 3 : 2][kY];   // of a Y tile's queries: lse, delta, g_y
+  __shared__ float row_top[kShared ? 2 : 1][kShared ? 2 : 1][kShared ? kRows : 1];    // by turns: what either half of the columns has
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -77,6 +107,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   auto empty = [&](int s) { return bar0 + 8 * (kSt + s); };
   const uint32_t x_full = bar0 + 16 * kSt, tail = x_full + 8, done = x_full + 16, s_full = x_full + 24, dp_full = x_full + 32,
                  p_ready = x_full + 40, ds_ready = x_full + 48;
+  auto pair = [&](int w) { return x_full + 56 + 8 * w; };                 // the two warps of 32 rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   long long id = blockIdx.x;
@@ -91,26 +122,19 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   share(kKeys ? qtiles * group : (len + kY - 1) / kY, p.splits, split, i0, i1);
   if (kKeys && x0 >= len) i1 = i0;                // keys that are not there
   const int n = i1 - i0;
-  // powers of two: of the operands (two parts), and of dS
-  int e_q = 0, e_k = 0, e_v = 0, e_g = 0, e_ds = 0;
+  // powers of two: of the operands (two parts; e_v and e_g bound them in one part too), and of dP - delta, which they bring to 1 at most
+  int e_q = 0, e_k = 0, e_v = 0, e_g = 0, e_one = 0;
   if constexpr (kHalf) {
     const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
     const int n_heads = p.B * p.Hkv;
-    const float most_v = __uint_as_float(q[2 * n_heads]), most_g = __uint_as_float(q[3 * n_heads]);
-    // dS_j = p_j ((1 - p_j) dP_j - sum of the other p_k dP_k), and the other p_k add up to 1 - p_j: |dS| <= 2 p (1 - p) max |dP| <=
-    // D most_v most_g / 2.  That is brought to 2^15 at most, half of what fp16 holds: with many keys p is 1 / keys, and what a second part
-    // has left of dS must not sink below fp16's smallest.  By exponents: the product itself may be beyond fp32.
-    if (most_v > 0.f && most_g > 0.f)
-      e_ds = max(-126, min(126, 15 - (ilogbf(most_v) + ilogbf(most_g) + ilogbf((float)(4 * p.D - 1)))));
+    e_v = scale_exponent(q[2 * n_heads]);
+    e_g = scale_exponent(q[3 * n_heads]);         // not above any row's
+    e_one = -31 - (32 - __clz(p.D - 1));          // |g 2^e_g| < 2^15, |v 2^e_v| < 2^15, D products, and delta is no larger
     if constexpr (kParts == 2) {
       e_q = scale_exponent(q[0]);
       e_k = scale_exponent(q[n_heads]);
-      e_v = scale_exponent(q[2 * n_heads]);
-      e_g = scale_exponent(q[3 * n_heads]);
     }
   }
-  // dS 2^e_ds = P (dP dp_mul - delta d_mul), with P scaled by 2^kUp and dP by its operands
-  const float d_mul = exp2f((float)e_ds - kUp), dp_mul = exp2f((float)(e_ds - e_v - e_g) - kUp);
   // tile i of Y: head, first row
   auto y_head = [&](int i) { return kKeys ? head * group + i / qtiles : hk; };
   auto y_row = [&](int i) { return (kKeys ? i % qtiles : i) * kY; };
@@ -124,6 +148,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     ptx::mbar_init(dp_full, 1);
     ptx::mbar_init(p_ready, kWork);
     ptx::mbar_init(ds_ready, kWork);
+    for (int w = 0; w < 4; ++w) ptx::mbar_init(pair(w), 2);
     abort_word = 0;
     ptx::fence_mbar_init();
   }
@@ -150,16 +175,37 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         for (; i < 2 * n; ++i) {
           const int s = i % kSt, y = i0 + (i >> 1), h = y_head(y), r0 = y_row(y);
           const bool second = i & 1;
+          // the queries' values are asked for before the wait
+          float row_lse[kKeys ? kY / 32 : 1], row_delta[kKeys ? kY / 32 : 1];
+          int row_exp[kKeys && kHalf ? kY / 32 : 1];
+          if constexpr (kKeys) {
+            if (!second) {
+              const long long at = ((long long)b * p.Hq + h) * p.Lq;
+#pragma unroll
+              for (int e = 0; e < kY / 32; ++e) {
+                const int r = min(r0 + lane + 32 * e, p.Lq - 1);
+                row_lse[e] = p.lse[at + r];
+                row_delta[e] = p.delta[at + r];
+                if constexpr (kHalf) row_exp[e] = p.g_exp[at + r];
+              }
+            }
+          }
           if (!warp_wait(empty(s), ((i / kSt) & 1) ^ 1, abort_flag)) break;
           if constexpr (kKeys) {
             if (!second) {
-              const long long at = ((long long)b * p.Hq + h) * p.Lq + r0;
 #pragma unroll
               for (int e = 0; e < kY / 32; ++e) {
                 const int r = lane + 32 * e;
                 const bool live = r0 + r < p.Lq;  // queries that are not there: P = 0
-                rows_of_y[s >> 1][0][r] = live ? p.lse[at + r] - kUp : INFINITY;
-                rows_of_y[s >> 1][1][r] = live ? p.delta[at + r] * d_mul : 0.f;
+                float l = row_lse[e] - (float)kUp, d = row_delta[e];
+                if constexpr (kHalf) {
+                  const int ge = row_exp[e];
+                  d = d * pow2(e_v) * pow2(kParts == 2 ? ge : e_g) * pow2(e_one);
+                  if constexpr (kParts == 2) l += (float)(ge - e_g);      // P g_y
+                  else rows_of_y[s >> 1][2][r] = live && e_g - ge >= -126 ? pow2(e_g - ge) : 0.f;
+                }
+                rows_of_y[s >> 1][0][r] = live ? l : INFINITY;
+                rows_of_y[s >> 1][1][r] = live ? d : 0.f;
               }
               __syncwarp();
             }
@@ -247,16 +293,74 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tS + 64 * half + lanes, d_at = tD + 64 * half + lanes;
     float lse = INFINITY, delta = 0.f;            // queries: this row's
+    int e_row = e_g;                              // exponent of grad_o
     if (!kKeys && xi < p.Lq) {
       const long long at = ((long long)b * p.Hq + head) * p.Lq + xi;
-      lse = p.lse[at] - kUp;
-      delta = p.delta[at] * d_mul;
+      lse = p.lse[at];
+      if constexpr (kHalf) e_row = p.g_exp[at];
+      delta = p.delta[at];
+      if constexpr (kHalf) delta = delta * pow2(e_v) * pow2(e_row) * pow2(e_one);
     }
+    float dp_mul = !kHalf ? 1.f : pow2(min(126, e_one + (kParts == 2 ? 0 : e_row + e_v)));   // (126: a row of zeros)
+    if constexpr (kHalf && !kLift) {
+      dp_mul *= pow2(kFixedLift);
+      delta *= pow2(kFixedLift);
+    }
+    int lift = kHalf && !kLift ? kFixedLift : 0;  // of this row: P 2^lift
     const bool row_in = kKeys ? xi < len : true, x_ragged = kKeys && x0 + kRows > len;
     constexpr bool kZeroEach = kKeys && kParts == 2;   // keys that are not there value by value: at the end, both parts spill
     float c = p.c;
     if constexpr (kParts == 2) c = ldexpf(c, -e_q - e_k);
     const F2 c2 = f2(c, c);
+    // a sum's columns that this thread takes back: all of its row, or half of them
+    auto take_back = [&](uint32_t acc, float f) {
+      constexpr int kOwn = kShared ? DP / 2 : DP;
+      acc += lanes + (kShared ? half * kOwn : 0);
+#pragma unroll 1
+      for (int c0 = 0; c0 < (kApart ? 2 : 1) * kOwn; c0 += 32) {
+        const uint32_t at = acc + (c0 < kOwn ? c0 : 128 + c0 - kOwn);
+        uint32_t r[32];
+        ptx::tmem_ld_32x32(at, r);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+        tmem_st_32x32(at, r);
+      }
+      tmem_st_wait();
+    };
+    // The row's `lift` goes by the exponent of tile i's largest value or sum: what this thread has of the row, and what the row has.  It is
+    // brought to 2^kTop, and may grow to 2^15 afterwards (above 2^35 it is not finite).
+    constexpr int kTop = kKeys && kParts == 2 ? 9 : 11;
+    bool lower = false;                           // the warp's sums are to be taken back, by `fall`
+    float fall = 1.f, own_top = 0.f;
+    auto post = [&](int i, float top) {
+      own_top = top;
+      if constexpr (kShared) {
+        row_top[i & 1][half][row] = top;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(pair(warp & 3));
+      }
+    };
+    auto follow = [&](int i) {
+      float top = own_top;
+      if constexpr (kShared) {
+        if (!warp_wait(pair(warp & 3), i & 1, abort_flag)) return false;
+        top = fmaxf(top, row_top[i & 1][half ^ 1][row]);
+      }
+      const int to = kTop - __float2int_rd(fminf(fmaxf(top, -89.f), 35.f));
+      lower = false;
+      fall = 1.f;
+      if (i == 0) {
+        lift = to;
+      } else if (__any_sync(0xffffffffu, lift - to >= 15 - kTop)) {
+        lower = true;
+        if (lift - to >= 15 - kTop) {
+          fall = pow2(to - lift);
+          lift = to;
+        }
+      }
+      return true;
+    };
     bool ok = true;
     for (int i = 0; ok && i < n; ++i) {
       if (!warp_wait(s_full, i & 1, abort_flag)) { ok = false; break; }
@@ -284,11 +388,59 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           for (int u = 0; u < 4; u += 2) {
             float x, y;
             f2_split(fma2(f2(__uint_as_float(s[k][e + u]), __uint_as_float(s[k][e + u + 1])), c2, lv[u / 2]), x, y);
-            const bool out = kZeroEach && !row_in;
-            s[k][e + u] = out ? 0u : __float_as_uint(exp2_fast(x));
-            s[k][e + u + 1] = out ? 0u : __float_as_uint(exp2_fast(y));
+            if constexpr (kKeys && kParts == 2) {
+              s[k][e + u] = row_in ? __float_as_uint(x) : 0xff800000u;    // keys that are not there
+              s[k][e + u + 1] = row_in ? __float_as_uint(y) : 0xff800000u;
+            } else {
+              s[k][e + u] = __float_as_uint(exp2_fast(x));
+              s[k][e + u + 1] = __float_as_uint(exp2_fast(y));
+            }
           }
         }
+      if constexpr (kKeys && kParts == 2) {
+        // P waits for its scale: from the largest exponent, which the other warp has before the exponentials are formed
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 64; e += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            top4[u] = fmaxf(fmaxf(top4[u], __uint_as_float(s[e >> 5][(e & 31) + u])), __uint_as_float(s[e >> 5][(e & 31) + 4 + u]));
+        post(i, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
+#pragma unroll
+        for (int e = 0; e < 64; ++e) s[e >> 5][e & 31] = __float_as_uint(exp2_fast(__uint_as_float(s[e >> 5][e & 31])));
+        if (!follow(i)) { ok = false; break; }
+        if (lower) take_back(tA1, fall);
+        lift_row(s, lift);
+      } else if constexpr (kLift) {
+        // only dS waits for it: from the sum, which is at least the largest.  (64 maxima, of half the additions' rate, took a fifth of the
+        // queries' kernel.)
+        if (ragged) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (64 * half + e >= valid) s[e >> 5][e & 31] = 0u;
+        }
+        F2 sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          const uint32_t* v = &s[e >> 5][e & 31];
+          const F2 a = f2(__uint_as_float(v[0]), __uint_as_float(v[1])), b = f2(__uint_as_float(v[2]), __uint_as_float(v[3]));
+          F2 &sa = sum[e / 2 & 2], &sb = sum[(e / 2 & 2) + 1];
+          if constexpr (kKeys) {
+            const float4 g4 = *reinterpret_cast<const float4*>(ly + 2 * kY + e);
+            sa = fma2(a, f2(g4.x, g4.y), sa);
+            sb = fma2(b, f2(g4.z, g4.w), sb);
+          } else {
+            sa = add2(sa, a);
+            sb = add2(sb, b);
+          }
+        }
+        float x, y;
+        f2_split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
+        post(i, row_in ? (float)((int)(__float_as_uint(x + y) >> 23) - 127) : -INFINITY);
+        if constexpr (!kKeys) {
+          if (!follow(i)) { ok = false; break; }
+        }
+      }
       if constexpr (kKeys) {
         uint32_t w[32], rest[32];
 #pragma unroll
@@ -307,9 +459,21 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_ready);
+        if constexpr (kLift && kParts == 1) {
+          if (!follow(i)) { ok = false; break; }
+          lift_row(s, lift);
+        }
       }
       if (!warp_wait(dp_full, i & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
+      float dm = dp_mul, dd = delta;
+      if constexpr (kLift) {
+        if constexpr (!kKeys) {
+          dm *= pow2(lift);
+          dd *= pow2(lift);
+        }
+        if (lower) take_back(tA2, fall);
+      }
       uint32_t w[32], rest[kParts == 2 ? 32 : 1];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -318,7 +482,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          float4 d4 = make_float4(delta, delta, delta, delta);
+          float4 d4 = make_float4(dd, dd, dd, dd);
           if constexpr (kKeys) d4 = *reinterpret_cast<const float4*>(ly + kY + 32 * k + e);
           const F2 dv[2] = {f2(-d4.x, -d4.y), f2(-d4.z, -d4.w)};
           float v[4];
@@ -326,7 +490,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           for (int u = 0; u < 4; u += 2) {
             const F2 dp = f2(__uint_as_float(d[e + u]), __uint_as_float(d[e + u + 1]));
             const F2 t = mul2(f2(__uint_as_float(s[k][e + u]), __uint_as_float(s[k][e + u + 1])),
-                              kHalf ? fma2(dp, f2(dp_mul, dp_mul), dv[u / 2]) : add2(dp, dv[u / 2]));
+                              kHalf ? fma2(dp, f2(dm, dm), dv[u / 2]) : add2(dp, dv[u / 2]));
             f2_split(t, v[u], v[u + 1]);
           }
           if constexpr (kZeroEach) {
@@ -367,8 +531,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       const int there = kKeys ? p.Lk : p.Lq;
       const long long rows = (long long)p.B * there * heads, out = ((long long)b * there + xi) * heads + head;
       auto write = [&](bool first, int c0, int c_end) {
-        // grad_v: P 2^kUp and grad_o; dS and the other factor
-        const float mul = first ? exp2f(-kUp - (float)e_g) : p.scale * exp2f((float)-e_ds) * exp2f((float)-(kKeys ? e_q : e_k));
+        // what the sums were scaled by: P (by kUp, or lift) and grad_o; P, dP - delta and the other factor
+        const int up = first ? (kParts == 2 ? lift + e_g : kUp) : kUp + lift + e_row + e_v + e_one + (kKeys ? e_q : e_k);
+        // (three factors: together they may be beyond a float's exponents)
+        const int down = max(-378, min(378, -up));
+        const float m1 = pow2(down / 3), m2 = pow2((down + 1) / 3), m3 = pow2(down - down / 3 - (down + 1) / 3);
         const uint32_t acc = (first ? tA1 : tA2) + lanes;
         Out* dst = reinterpret_cast<Out*>(first ? p.g1 : p.g2) + out * p.D;
         float* part = p.splits > 1 ? p.part + (((long long)(first ? p.splits : 0) + split) * rows + out) * p.D : nullptr;
@@ -386,7 +553,10 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             if (c0 + e >= c_end) break;
             float f[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(r[e + u]) * mul;
+            for (int u = 0; u < 8; ++u) {
+              f[u] = __uint_as_float(r[e + u]) * (first ? 1.f : p.scale);
+              if constexpr (kHalf) f[u] = f[u] * m1 * m2 * m3;
+            }
             if (part) store8(part + c0 + e, f, p.D - c0 - e, p.D % 4 == 0);
             else store8(dst + c0 + e, f, p.D - c0 - e, p.D * sizeof(Out) % 16 == 0);
           }
@@ -449,7 +619,7 @@ int tc_bwd(int dtype, const Args& a, const Operand (&x)[4], int parts, bool keys
   p.c = a.scale * kLog2e; p.scale = a.scale;
   p.splits = a.splits;
   p.blocks_x = ((keys ? a.Lk : a.Lq) + kRows - 1) / kRows;
-  p.lse = a.lse; p.delta = a.delta; p.bounds = bounds;
+  p.lse = a.lse; p.delta = a.delta; p.bounds = bounds; p.g_exp = a.g_exp;
   p.g1 = a.gv; p.g2 = keys ? a.gk : a.gq;
   p.part = a.part;
   p.a = a;

@@ -22,8 +22,9 @@ template <int DP>
 constexpr int kTileBytes = kHalfBytes * (DP / 64);
 
 // fp32 tensors are staged (split_rows) in `kParts` = 2 operand tiles behind one another: fp16, hi = fp16(x 2^e) and lo = fp16(x 2^e - hi),
-// whose products hi hi + lo hi + hi lo keep 22 bits of each factor, with 2^e from the largest element of the clip and key head, so that
-// neither type's range matters; or in one, bf16.  The parts are the outer half of a tensor map's clips.
+// whose products hi hi + lo hi + hi lo keep 22 bits of each factor, with 2^e from the largest element of the clip and key head (grad_o: of
+// the query's row, whose sizes differ by what a loss makes of them): an element keeps its 22 bits down to 2^-18 of that largest one, and
+// is off by 2^-40 of it below.  Or in one part, bf16.  The parts are the outer half of a tensor map's clips.
 //
 // One box of 64 channels x 1 head x 128 (R) tokens x 1 clip; what lies outside the tensor arrives as zeros.  x is 0 or 64.
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, int clip, uint32_t bar) {
@@ -151,11 +152,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t packed) {
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&packed));
   return pack2<__half>(lo - h.x, hi - h.y);
-}
-// Exponent e that brings a largest element to 2^14 .. 2^15 (bits of a float, as largest_sizes writes it; 0: all are zero).
-__device__ __forceinline__ int scale_exponent(uint32_t size) {
-  const float f = __uint_as_float(size);
-  return f > 0.f ? max(-126, min(126, 14 - ilogbf(f))) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // |e| <= 126
 // Eight neighbouring results of a row, the first `n` of them (16-byte stores where all are there; dst is then 16-byte aligned).
