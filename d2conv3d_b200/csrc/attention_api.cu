@@ -76,10 +76,6 @@ int tensor_parts(const d2c_attention_desc& d, int mode, bool aligned, bool backw
     if (mode == D2C_MATH_BF16) return 1;
     // staging and joining are launches of their own: 2 x 1015 x 179, 4 heads of 32 channels, trains in 84 us on CUDA cores and in 113
     // in two parts; 2 x 400 x 400, 4 heads of 64, in 118 and 107
-    // With many keys a score gradient is small beside the bound that its fp16 parts are scaled by, and the second part loses bits: normal
-    // values, 64 channels, are 1.5e-6 (2-norm) from 64 bits at 32768 keys, 1e-5 at 262144 and 4e-5 at 1000000, where CUDA cores, at
-    // several times the time, stay with fp32
-    if (mode == D2C_MATH_AUTO && backward && d.keys > 1 << 16) return 0;
     const double products = (double)d.batch * d.q_heads * d.queries * d.keys * d.dim;
     return mode == D2C_MATH_AUTO && products < (double)(1 << 26) ? 0 : 2;
   }

@@ -139,3 +139,13 @@ def test_queries_without_a_gradient(dtype):
     check(q, k, v, g, names=("grad_k", "grad_v"))
     none = gradients(q, k, v, torch.zeros_like(g))
     assert all((t == 0).all() for t in none)
+
+
+@pytest.mark.parametrize("keys", [65536, 65537, 200000])
+def test_the_default_mode_takes_parts_for_any_number_of_keys(keys):
+    """No edge at some number of keys: the calls just above one were four times slower."""
+    q, k, v, g = make(130, keys, 64, torch.float32, 5)
+    want = gradients(q, k, v, g)
+    d2c.set_math_mode("auto")
+    assert all(torch.equal(a, b) for a, b in zip(gradients(q, k, v, g), want))
+    check(q, k, v, g)
