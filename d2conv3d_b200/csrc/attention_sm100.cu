@@ -5,7 +5,8 @@
 // four warps a tile (a thread a row) form p = 2^(s scale log2 e - m) with the running maximum and sum, and write it over S as the
 // 16-bit A operand of O_t += P_t V, whose accumulator stays in tensor memory too.  While one tile's warps work on their scores the
 // tensor cores work for the other tile.  The maximum that p refers to is raised, and O rescaled, only when the row's maximum has
-// outgrown it by 2^8: p is then at most 256, which both types hold, and most tiles skip the pass over O.
+// outgrown it by 2^8: p is then at most 256, which both types hold, and most tiles skip the pass over O.  fp16 p are scaled by 2^7 besides:
+// what lies 2^-32 below a row's largest is still there (many keys alike, 17 nats below one: 6 % of what they add were lost at 2^-25).
 // 51360 queries, 12960 keys, 4 heads of 128 in bf16: 1.10 ms (1240 TFLOP/s) in a few calls, 1.25 ms (1090) in a long run, where the power
 // cap holds; 2 clips of 3240 queries and up to 12960 keys, 4 heads of 64: 136 us.  The chain of a tile (scores, exponentials, product)
 // bounds it: two tiles in flight keep the special-function pipe 61 .. 65 % and the tensor pipe 26 .. 58 % busy.
@@ -44,6 +45,7 @@ template <typename T, typename Out, int DP, int kParts>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
               const __grid_constant__ TcParams p) {
+  constexpr float kUp = std::is_same_v<T, __half> ? 7.f : 0.f;   // p is scaled by 2^kUp
   constexpr int kStages = kFwdStages<DP, kParts>, kTB = kTileBytes<DP> * kParts, kQ = kQTiles<DP, kParts>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kStages + 9];
@@ -177,7 +179,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       c = ldexpf(c, -scale_exponent(q[0]) - scale_exponent(q[n_heads]));
       o_mul = pow2(-scale_exponent(q[2 * n_heads]));
     }
-    float m = 0.f, l = 0.f;
+    float m = 0.f, l = 0.f;                       // p = 2^(s c - m)
     bool ok = t < nt;
     for (int j = 0; ok && j < n; ++j) {
       if (!warp_wait(s_full(t), j & 1, abort_flag)) { ok = false; break; }
@@ -205,9 +207,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx *= c;
       if (j == 0) {
-        m = mx == -INFINITY ? 0.f : mx;
-      } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-        const float to = fmaxf(mx, m), f = exp2_fast(m - to);
+        m = mx == -INFINITY ? 0.f : mx - kUp;
+      } else if (__any_sync(0xffffffffu, mx > m + (kUp + 8.f))) {
+        const float to = fmaxf(mx - kUp, m), f = exp2_fast(m - to);
         m = to;
         l *= f;
         for (int part = 0; part < kParts; ++part)

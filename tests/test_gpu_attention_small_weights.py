@@ -1,0 +1,42 @@
+"""Cross attention where most of a row's weights are far below its largest: they are small, but there are many of them."""
+import pytest
+import torch
+
+import d2conv3d_b200 as d2c
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def in_parts():
+    before = d2c.get_math_mode()
+    d2c.set_math_mode("bf16x3")            # float32: whatever the size of the call
+    yield
+    d2c.set_math_mode(before)
+
+
+@pytest.mark.parametrize("gap", [8.0, 11.0, 14.0, 17.0])
+@pytest.mark.parametrize("keys,d", [(1000, 64), (12960, 64), (12960, 128), (51360, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_one_key_above_many_alike(dtype, keys, d, gap):
+    """One key scores `gap` nats above all others, which are alike; values 1 for them and 0 for it, so that the result is the share that
+    the others have: keys e^-gap / (1 + keys e^-gap), 4e-5 and more.  A weight is off by half a step of fp16's smallest numbers, 2^-25,
+    against a largest one of 2^7 at least: 2^-32 e^gap of itself; the rest is roundings of a few 2^-23 (float32: two parts; the scores, 1e-6 of
+    gap at most; a chain of truncated sums, 72 2^-23) and half a step of the result, and of P (float16)."""
+    q = torch.ones(1, 300, 1, d, device="cuda", dtype=dtype)
+    k = torch.zeros(1, keys, 1, d, device="cuda", dtype=dtype)
+    v = torch.ones(1, keys, 1, d, device="cuda", dtype=dtype)
+    for at in (0, 200, keys - 1):                                        # in the first tile, a later one, the last one
+        kk, vv = k.clone(), v.clone()
+        kk[0, at] = gap / d ** 0.5                                       # scale * q . k = d^-1/2 * d * gap d^-1/2
+        vv[0, at] = 0
+        s = float(kk[0, at, 0, 0].double()) * d ** 0.5
+        share = (keys - 1) * torch.exp(torch.tensor(-s, dtype=torch.float64))
+        want = float(share / (1 + share))
+        half = torch.finfo(dtype).eps / 2
+        rounding = 2.0 ** -16.8 + 2.0 ** -20 * gap if dtype == torch.float32 else 2 * half + 2.0 ** -16.8
+        bound = want * (2.0 ** -32 * torch.exp(torch.tensor(s)).item() + rounding) + torch.finfo(dtype).smallest_normal * half * 2
+        with torch.no_grad():
+            o = d2c.cross_attention(q, kk, vv)
+        off = float((o.double() - want).abs().max())
+        assert off <= bound, f"key {at}: off by {off / want:.2e}, allowed {bound / want:.2e}"
