@@ -179,7 +179,7 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       c = ldexpf(c, -scale_exponent(q[0]) - scale_exponent(q[n_heads]));
       o_mul = pow2(-scale_exponent(q[2 * n_heads]));
     }
-    float m = 0.f, l = 0.f;                       // p = 2^(s c - m)
+    float m = -INFINITY, l = 0.f;                 // p = 2^(s c - m), 0 as long as all scores are -inf
     bool ok = t < nt;
     for (int j = 0; ok && j < n; ++j) {
       if (!warp_wait(s_full(t), j & 1, abort_flag)) { ok = false; break; }
@@ -207,9 +207,9 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx *= c;
       if (j == 0) {
-        m = mx == -INFINITY ? 0.f : mx - kUp;
+        m = mx - kUp;
       } else if (__any_sync(0xffffffffu, mx > m + (kUp + 8.f))) {
-        const float to = fmaxf(mx - kUp, m), f = exp2_fast(m - to);
+        const float to = fmaxf(mx - kUp, m), f = m == -INFINITY ? 0.f : exp2_fast(m - to);
         m = to;
         l *= f;
         for (int part = 0; part < kParts; ++part)
@@ -223,7 +223,8 @@ fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
           }
       }
       F2 sum[2] = {0ull, 0ull};
-      const F2 c2 = f2(c, c), m2 = f2(-m, -m);
+      const float shift = m == -INFINITY ? 0.f : m;
+      const F2 c2 = f2(c, c), m2 = f2(-shift, -shift);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t w[32], rest[32];

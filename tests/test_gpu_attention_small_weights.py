@@ -40,3 +40,39 @@ def test_one_key_above_many_alike(dtype, keys, d, gap):
             o = d2c.cross_attention(q, kk, vv)
         off = float((o.double() - want).abs().max())
         assert off <= bound, f"key {at}: off by {off / want:.2e}, allowed {bound / want:.2e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("keys,lq", [(300, 140), (3000, 20), (300, 1)])
+def test_a_first_tile_that_scores_minus_infinity(dtype, keys, lq):
+    """Keys whose scores are all -inf weigh nothing, wherever they are, and what follows may lie far below zero."""
+    torch.manual_seed(0)
+    q = torch.rand(1, lq, 2, 64, device="cuda").to(dtype) + 1
+    k, v = (torch.randn(1, keys, 2, 64, device="cuda").to(dtype) for _ in range(2))
+    k[..., 1] = -200                       # scores of about -37 nats, 2^-54: beyond what fp16 holds
+    k[:, :150, :, 0] = -float("inf")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = d2c.cross_attention(*leaves)
+    rest = d2c.cross_attention(q, k[:, 150:], v[:, 150:])
+    want = torch.softmax(torch.einsum("bihd,bjhd->bhij", q.double(), k[:, 150:].double()) / 8, -1)
+    want = torch.einsum("bhij,bjhd->bihd", want, v[:, 150:].double())
+    # P and the result are rounded by half a step each; P against values whose signs are not alike
+    bound = torch.finfo(dtype).eps * 2 * v.abs().max().double()
+    assert (o.double() - want).abs().max() <= bound and (rest.double() - want).abs().max() <= bound
+
+
+def test_rows_without_weights_beside_rows_that_grow():
+    """Products beyond the type's range are -inf for the queries that meet them so, through two tiles, while the other queries' scores
+    grow from tile to tile."""
+    torch.manual_seed(1)
+    dtype = torch.bfloat16
+    q = torch.rand(1, 140, 1, 64, device="cuda").to(dtype) + 1
+    k, v = (torch.randn(1, 600, 1, 64, device="cuda").to(dtype) for _ in range(2))
+    q[:, ::2, :, 0], q[:, 1::2, :, 0] = 1e20, 1e-20
+    k[:, :300, :, 0], k[:, 300:, :, 0] = -1e20, 0
+    k[..., 1] = torch.linspace(-200, 0, 600, device="cuda").to(dtype).view(1, -1, 1)
+    with torch.no_grad():
+        o = d2c.cross_attention(q, k, v)
+    want = torch.softmax(torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) / 8, -1)
+    want = torch.einsum("bhij,bjhd->bihd", want, v.double())
+    assert (o.double() - want).abs().max() <= torch.finfo(dtype).eps * 2 * v.abs().max().double()
