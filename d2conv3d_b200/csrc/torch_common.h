@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <optional>
 
 #include "d2conv3d.h"
@@ -36,6 +37,12 @@ inline Tensor bytes_on(size_t n, const Tensor& t) {
   return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)) : Tensor();
 }
 inline void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// The operators have no forward-mode derivative, and they pass the dispatcher by, which would say so: a tangent must not get lost.
+inline void refuse_tangents(const char* op, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), op, ": forward-mode derivatives are not implemented");
+}
 
 // A tensor that a node keeps for its backward.  Saved-tensor hooks decide what comes back: another layout is for the caller to deal with
 // (contiguous(), or fresh strides), another size, type or device is refused here, since the kernels go by the forward's sizes.

@@ -71,6 +71,7 @@ struct LayerNormNode : public Node {
 
 Tensor layer_norm(const Tensor& input, const OptTensor& weight_, const OptTensor& bias_, double eps, int64_t layout) {
   const Tensor weight = get(weight_), bias = get(bias_);
+  refuse_tangents("layer_norm", {&input, &weight, &bias});
   D2C_REQUIRE(input.is_cuda(), "input.device().is_cuda()");
   same_device("layer_norm", input, weight, "weight");
   same_device("layer_norm", input, bias, "bias");
@@ -192,6 +193,7 @@ struct RotaryNode : public Node {
 Tensor rotary(const Tensor& x, const OptTensor& positions_, const std::array<int64_t, 3>& grid, const std::array<double, 3>& step,
               const std::array<int64_t, 3>& axis_dims, double base, bool interleaved) {
   const Tensor positions = get(positions_);
+  refuse_tangents("rotary_embedding_3d", {&x, &positions});
   D2C_REQUIRE(x.is_cuda(), "x.device().is_cuda()");
   D2C_REQUIRE(x.dim() == 4, "x.ndimension() == 4");
   Rotary r{};
@@ -318,6 +320,7 @@ struct AttentionNode : public Node {
 
 Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& value, const OptTensor& lengths_, double scale) {
   const Tensor lengths = get(lengths_);
+  refuse_tangents("cross_attention", {&query, &key, &value});
   D2C_REQUIRE(query.is_cuda(), "query.device().is_cuda()");
   D2C_REQUIRE(query.dim() == 4, "query.ndimension() == 4");
   D2C_REQUIRE(key.dim() == 4, "key.ndimension() == 4");
