@@ -253,6 +253,7 @@ Tensor run_deform(Kind kind, const d2c_conv_desc& desc, const d2c_head_desc& hea
 
 // SANITY_CHECK_DCONV_INPUTS / _GROUPS, csrc/ops/dconv_gpu_common.h:17-51
 void sanity_check(const Tensor& input, const Tensor& offset, const Tensor& alpha, const Tensor& weight, const Tensor& bias) {
+  refuse_tangents("deform_conv3d", {&input, &offset, &alpha, &weight, &bias});
   D2C_REQUIRE(input.dim() == 5, "input.ndimension() == ((3) + 2)");
   D2C_REQUIRE(offset.dim() == 5, "offset.ndimension() == ((3) + 2)");
   D2C_REQUIRE(!alpha.defined() || alpha.dim() == 5, "alpha.ndimension() == ((3) + 2)");
@@ -333,6 +334,7 @@ Tensor deform_conv3d_head(const Tensor& input, const Tensor& raw, const Tensor& 
                           const Triple& padding, const Triple& dilation, int64_t groups, int64_t offset_groups,
                           const OptTensor& cache_buf) {
   const Tensor bias = get(bias_);
+  refuse_tangents("deform_conv3d", {&input, &raw, &weight, &bias});
   D2C_REQUIRE(input.dim() == 5, "input.ndimension() == 5");
   D2C_REQUIRE(input.is_cuda(), "input.device().is_cuda()");
   D2C_REQUIRE(raw.dim() == 5, "deformation.ndimension() == 5");
@@ -358,6 +360,7 @@ Tensor deform_conv1d(Tensor input, Tensor offset, const OptTensor& alpha_, Tenso
                      int64_t stride, int64_t padding, int64_t dilation, int64_t groups, int64_t offset_groups, bool upcast) {
   Tensor alpha = get(alpha_), bias = get(bias_);
   if (upcast) upcast_if_any_half({&input, &offset, &alpha, &weight, &bias});
+  refuse_tangents("deform_conv1d", {&input, &offset, &alpha, &weight, &bias});
   D2C_REQUIRE(input.dim() == 3, "input.ndimension() == 3");
   D2C_REQUIRE(input.is_cuda(), "input.device().is_cuda()");
   D2C_REQUIRE(offset.dim() == 3, "offset.ndimension() == 3");
@@ -438,6 +441,7 @@ struct DepthwiseNode : public Node {
 Tensor depthwise_conv3d(const Tensor& input, const Tensor& weight, const OptTensor& bias_, const Triple& stride,
                         const Triple& padding, const Triple& dilation) {
   const Tensor bias = get(bias_);
+  refuse_tangents("depthwise_separable_conv3d", {&input, &weight, &bias});
   TORCH_CHECK(input.is_cuda() && weight.is_cuda(), "depthwise_separable_conv3d expects CUDA tensors");
   TORCH_CHECK(input.device() == weight.device() && (!bias.defined() || bias.device() == input.device()),
               "expects input and weight tensors to be on the same device.");

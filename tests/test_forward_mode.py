@@ -31,3 +31,24 @@ def test_a_primal_passes_the_check():
         x = forward_ad.unpack_dual(duals(1, 0, 1, 4, 2, 8)[0]).primal
         with pytest.raises(RuntimeError, match="is_cuda"):
             d2c.layer_norm(x)
+
+
+def test_convolutions():
+    with forward_ad.dual_level():
+        x, w, off = torch.randn(1, 8, 3, 5, 5), torch.randn(8, 8, 3, 3, 3), torch.zeros(1, 81, 3, 5, 5)
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        native = d2c._lib.native()
+        three = (1, 1, 1)
+        for i in range(3):
+            t = [x, off, w]
+            t[i] = dual(t[i])
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                native.deform_conv3d(t[0], t[1], None, t[2], None, three, three, three, 1, 1, False)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                native.deform_conv3d_head(t[0], t[1], t[2], None, -1, -1, 0, 0, three, three, three, 1, 1, None)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            native.dyn_dilated_conv3d(x, dual(torch.ones(1, 1, 3, 5, 5)), None, w, None, 0, three, three, three, 1, 1, False)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            native.deform_conv1d(dual(torch.randn(1, 8, 9)), torch.zeros(1, 3, 9), None, torch.randn(8, 8, 3), None, 1, 1, 1, 1, 1, False)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            native.depthwise_conv3d(dual(x), torch.randn(8, 1, 3, 3, 3), None, three, three, three)
