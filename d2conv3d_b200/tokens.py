@@ -35,7 +35,8 @@ def rotary_embedding_3d(x, positions, axis_dims, base=10000.0, interleaved=False
 
     x          [B, L, H, D] with any strides; the result is contiguous
     positions  (T, H, W): the tokens are this volume's voxels in row-major order; or a tensor [L, 3] / [B, L, 3] of
-               (time, height, width), int32, int64 or float32, anywhere up to 2^53 (angles are formed in 64 bits)
+               (time, height, width), int32, int64 or float32.  Angles are formed in 64 bits: a position p costs up to
+               p * 2^-50 radians, which float32's own rounding (2^-23) hides up to p = 2^27
     axis_dims  channels that time, height and width turn: even, in this order from the first channel on; channels behind
                their sum stay as they are
     base       pair i of an axis with n channels turns by position * base^(-2 i / n)
