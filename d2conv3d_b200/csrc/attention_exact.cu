@@ -8,7 +8,7 @@
 // The backward is two kernels, one with a tile of queries that runs over the keys, one with a tile of keys that runs over the
 // queries of all heads that share them: each gradient has one writer, so that there are no atomics and every call gives the
 // same bits, for 7 products a score instead of 5.  Bound by the FMA pipe: a thread forms 4 x 4 scores from 16-byte
-// shared-memory reads.  1215 x 3240, 4 heads of 64 in fp32: 165 us forward, 225 (queries) and 333 us (keys), 24, 19 and 17 TFLOP/s.
+// shared-memory reads.  1215 x 3240, 4 heads of 64 in fp32: 165 us forward, 225 (queries) and 333 us (keys), 24, 27 and 24 TFLOP/s.
 #include "attention.h"
 
 #include <algorithm>

@@ -450,7 +450,9 @@ int d2c_attention_check(const d2c_attention_desc* desc);
  * outside 0 .. keys are taken as the nearer of the two).  No keys: o = 0.  lse: NULL, or [batch, q_heads, queries] floats for
  * the backward.  Keys and values behind a clip's length are not used, whatever they hold.  dim <= 128, queries and keys <= 2^30.
  * 16-bit tensors with 16-byte rows run on tensor cores; fp32 tensors follow the math mode: AUTO (large calls) and BF16X3 in two 16-bit
- * parts scaled by powers of two (22 bits of a factor), BF16 in one, FP32 on CUDA cores.  The workspace depends on the mode. */
+ * parts scaled by powers of two (22 bits of a factor down to 2^-18 of the largest element of its clip and key head -- grad_o: of its
+ * row --, 2^-40 of that one below; what an element that is not finite meets is NaN), BF16 in one, FP32 on CUDA cores.  The workspace
+ * depends on the mode. */
 size_t d2c_attention_fwd_workspace_bytes(const d2c_attention_desc* desc);
 int d2c_attention_fwd(const d2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* key_lengths,
                       void* o, void* lse, void* workspace, size_t workspace_bytes, d2c_stream_t stream);
