@@ -25,8 +25,8 @@
 // row is the query): a tile that brings far more takes the row's sums back by the difference, as a running softmax does.  Under that
 // scale |dS| <= 2^15, since |dP - delta| <= 2 D max|g_y| max|v|; dS typically lies 2^7 below that, and the second part ends at 2^-24.  fp32
 // tensors are staged with every query's grad_o at its own exponent: P g_y takes P's place and is scaled alike.  P itself, for fp16
-// tensors, is scaled by 2^14.  Whatever the sizes of grad_o and the number of keys (3240 .. 1000000), fp32 gradients are 0.6e-6 ..
-// 1.9e-6 (2-norm) from 64 bits; one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  It
+// tensors, is scaled by 2^14.  Whatever the sizes of grad_o in fp32's normal range and the number of keys (3240 .. 1000000), fp32
+// gradients are 0.6e-6 .. 1.9e-6 (2-norm) from 64 bits; one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  It
 // costs 6 % of these kernels in two parts of 64 channels and 12 % of the fp16 keys' kernel of 64 (208 us with one scale, 233 with
 // the rows').
 #include <algorithm>
