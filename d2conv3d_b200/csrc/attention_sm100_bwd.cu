@@ -19,16 +19,19 @@
 // 2 clips of 3240 queries and up to 12960 keys, 4 heads of 64 in bf16: keys 183 us, queries 152 us, with tiles of 128 x 64 and two blocks a
 // SM; with one block of 128 x 128 tiles 212 and 162.
 //
-// fp16 operands: a probability is of the order of 1 / keys, score gradients are smaller still, and both go with what a loss makes of its
-// queries, which may differ by any power of two.  So a row of X has a power of two of its own, 2^lift, that follows the largest of its
-// P_xy g_y so far, or a tile's sum of them (g_y: the size of that query's grad_o against the largest; 1 in the queries' kernel, where the
-// row is the query): a tile that brings far more takes the row's sums back by the difference, as a running softmax does.  Under that
-// scale |dS| <= 2^15, since |dP - delta| <= 2 D max|g_y| max|v|; dS typically lies 2^7 below that, and the second part ends at 2^-24.  fp32
-// tensors are staged with every query's grad_o at its own exponent: P g_y takes P's place and is scaled alike.  P itself, for fp16
-// tensors, is scaled by 2^14.  Whatever the sizes of grad_o in fp32's normal range and the number of keys (3240 .. 1000000), fp32
-// gradients are 0.6e-6 .. 1.9e-6 (2-norm) from 64 bits; one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  It
-// costs 6 % of these kernels in two parts of 64 channels and 12 % of the fp16 keys' kernel of 64 (208 us with one scale, 233 with
-// the rows').
+// fp16 operands: a probability is of the order of 1 / keys, score gradients are smaller still, and both go with the sizes of grad_o and v,
+// which may differ by any power of two from query to query and from key to key.  fp32 tensors are staged with every query's grad_o at its
+// own exponent; in the keys' kernel P g_y takes P's place (g_y: the size of that query's grad_o against the largest), and has, row by row,
+// a power of two of its own that follows the largest that the row has met: a tile that brings far more takes the row's sums back by the
+// difference, as a running softmax does.  (P of fp16 tensors, and of the queries' kernel, is at most 1 and scaled by a constant.)  dS is
+// scaled by what |dP - delta| <= 2 D max|g_y| max|v| allows, less what dS usually lies below that.  How large it was is added up beside its
+// rounding, and if a row of the block was beyond fp16, or so small that its last bits were lost, the block runs over its tiles again, each row
+// with a scale of its own.  Ordinary tensors never need that; one value 2^10 times the others that nobody looks at does, and then costs
+// twice the time instead of 1e-4 of every query's gradient.
+// fp32 gradients are 0.6e-6 .. 1.9e-6 (2-norm) from 64 bits whatever the sizes of grad_o in fp32's normal range and the number of keys
+// (3240 .. 1000000); one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  Against that
+// (2 x 3240 x 12960, 4 heads, keys + queries): two parts of 64 channels 595 + 413 us for 547 + 378; fp16 of 64 channels 216 + 190 for 208 +
+// 167, of 128 channels 324 + 265 for 380 + 257 (a tile's values of the queries are asked for before its place is free).
 #include <algorithm>
 #include <type_traits>
 
@@ -51,11 +54,6 @@ struct BwdParams {
   Args a;                        // lengths
   int* status;
 };
-
-// P of a row adds up to 1 over its keys, so that dS_j = p_j ((1 - p_j) dP_j - sum of the other p_k dP_k) is at most max|dP| / 2, a quarter of
-// what 2^e_one brings to 1: 2^17 keep it within 2^15.  With one part that does for the queries' kernel: 11 bits of dS down to p =
-// 2^-24 where dP is 2^7 below its bound.
-constexpr int kFixedLift = 17;
 
 constexpr int y_rows(int size) { return size == 128 ? 128 : 64; }    // size: channels (64, 128) times parts
 template <int DP, int kParts>
@@ -92,15 +90,15 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   constexpr bool kApart = kParts == 2 && DP == 64;                        // tensor memory has room for sums of lo parts
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr int kUp = kHalf && kKeys && kParts == 1 ? 14 : 0;             // P is scaled by 2^kUp
-  constexpr bool kLift = kHalf && (kKeys || kParts == 2);                 // a row's scale follows what it meets; else it is 2^kFixedLift
-  constexpr bool kShared = kLift && kY == 128;    // a row's columns belong to two threads
+  constexpr bool kLift = kKeys && kParts == 2;    // a row's scale of P follows what it meets
+  constexpr bool kShared = kHalf && kY == 128;    // a row's columns belong to two threads
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kSt + 12];
-  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][kHalf && kParts == 1 ? 3 : 2][kY];   // of a Y tile's queries: lse, delta, g_y
-  __shared__ float row_top[kShared ? 2 : 1][kShared ? 2 : 1][kShared ? kRows : 1];    // by turns: what either half of the columns has
+  __shared__ __align__(16) float rows_of_y[kKeys ? kSt / 2 : 1][2][kY];   // of a Y tile's queries: lse, delta
+  __shared__ float row_top[kShared ? 2 : 1][kShared ? 2 : 1][kShared ? kRows : 1];    // by turns: what either half of a row's columns has
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
-  volatile int* abort_flag = &abort_word;
+  __shared__ int abort_word, again_word;
+  volatile int *abort_flag = &abort_word, *again = &again_word;
   const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t sx = base, ring = base + 2 * kTB, bar0 = ptx::smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8 * s; };
@@ -108,6 +106,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   const uint32_t x_full = bar0 + 16 * kSt, tail = x_full + 8, done = x_full + 16, s_full = x_full + 24, dp_full = x_full + 32,
                  p_ready = x_full + 40, ds_ready = x_full + 48;
   auto pair = [&](int w) { return x_full + 56 + 8 * w; };                 // the two warps of 32 rows
+  const uint32_t verdict = x_full + 88;           // whether the tiles are run over again (fp16)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   long long id = blockIdx.x;
@@ -122,14 +121,19 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
   share(kKeys ? qtiles * group : (len + kY - 1) / kY, p.splits, split, i0, i1);
   if (kKeys && x0 >= len) i1 = i0;                // keys that are not there
   const int n = i1 - i0;
-  // powers of two: of the operands (two parts; e_v and e_g bound them in one part too), and of dP - delta, which they bring to 1 at most
-  int e_q = 0, e_k = 0, e_v = 0, e_g = 0, e_one = 0;
+  // powers of two: of the operands (two parts; e_v and e_g bound them in one part too), and of dP - delta
+  int e_q = 0, e_k = 0, e_v = 0, e_g = 0, e_one = 0, e_first = 0;
+  bool nothing = false;                           // grad_o or v are zero: so is dS
   if constexpr (kHalf) {
     const uint32_t* q = p.bounds + (long long)b * p.Hkv + hk;
     const int n_heads = p.B * p.Hkv;
     e_v = scale_exponent(q[2 * n_heads]);
     e_g = scale_exponent(q[3 * n_heads]);         // not above any row's
-    e_one = -31 - (32 - __clz(p.D - 1));          // |g 2^e_g| < 2^15, |v 2^e_v| < 2^15, D products, and delta is no larger
+    nothing = q[2 * n_heads] == 0u || q[3 * n_heads] == 0u;
+    // |g 2^e_g| < 2^15, |v 2^e_v| < 2^15, D products, and delta is no larger: 1 at most, and then what dS is scaled by
+    e_one = -31 - (32 - __clz(p.D - 1));
+    e_first = kLift ? 5 : max(22, 32 - __clz(max(len, 2) - 1) + 3);
+    e_one += e_first - kUp;
     if constexpr (kParts == 2) {
       e_q = scale_exponent(q[0]);
       e_k = scale_exponent(q[n_heads]);
@@ -149,7 +153,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     ptx::mbar_init(p_ready, kWork);
     ptx::mbar_init(ds_ready, kWork);
     for (int w = 0; w < 4; ++w) ptx::mbar_init(pair(w), 2);
-    abort_word = 0;
+    ptx::mbar_init(verdict, kWork);
+    abort_word = again_word = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -172,12 +177,16 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           tma_tile<DP, kParts>(sx, &mx1, head, x0, b, p.B, x_full);
           tma_tile<DP, kParts>(sx + kTB, &mx2, head, x0, b, p.B, x_full);
         }
-        for (; i < 2 * n; ++i) {
-          const int s = i % kSt, y = i0 + (i >> 1), h = y_head(y), r0 = y_row(y);
+        for (int pass = 0; ; ++i) {
+          if (i == 2 * n * (pass + 1)) {
+            if (!kHalf || pass || !warp_wait(verdict, 0, abort_flag) || !*again) break;
+            pass = 1;
+          }
+          const int s = i % kSt, y = i0 + (i >> 1) - pass * n, h = y_head(y), r0 = y_row(y);
           const bool second = i & 1;
           // the queries' values are asked for before the wait
           float row_lse[kKeys ? kY / 32 : 1], row_delta[kKeys ? kY / 32 : 1];
-          int row_exp[kKeys && kHalf ? kY / 32 : 1];
+          int row_exp[kKeys && kParts == 2 ? kY / 32 : 1];
           if constexpr (kKeys) {
             if (!second) {
               const long long at = ((long long)b * p.Hq + h) * p.Lq;
@@ -186,7 +195,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
                 const int r = min(r0 + lane + 32 * e, p.Lq - 1);
                 row_lse[e] = p.lse[at + r];
                 row_delta[e] = p.delta[at + r];
-                if constexpr (kHalf) row_exp[e] = p.g_exp[at + r];
+                if constexpr (kParts == 2) row_exp[e] = p.g_exp[at + r];
               }
             }
           }
@@ -198,12 +207,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
                 const int r = lane + 32 * e;
                 const bool live = r0 + r < p.Lq;  // queries that are not there: P = 0
                 float l = row_lse[e] - (float)kUp, d = row_delta[e];
-                if constexpr (kHalf) {
-                  const int ge = row_exp[e];
-                  d = d * pow2(e_v) * pow2(kParts == 2 ? ge : e_g) * pow2(e_one);
-                  if constexpr (kParts == 2) l += (float)(ge - e_g);      // P g_y
-                  else rows_of_y[s >> 1][2][r] = live && e_g - ge >= -126 ? pow2(e_g - ge) : 0.f;
-                }
+                if constexpr (kHalf) d = d * pow2(e_v) * pow2(kParts == 2 ? row_exp[e] : e_g) * pow2(e_one);
+                if constexpr (kParts == 2) l += (float)(row_exp[e] - e_g);        // P g_y
                 rows_of_y[s >> 1][0][r] = live ? l : INFINITY;
                 rows_of_y[s >> 1][1][r] = live ? d : 0.f;
               }
@@ -217,8 +222,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             ptx::mbar_arrive_expect_tx(bar, kYB);
             tma_tile<DP, kParts, kY>(dst, second ? &my2 : &my1, h, r0, b, p.B, bar);
           }
-          if (patch) {                            // the last tile: once per block
-            drain(tail, 0);
+          if (patch) {                            // the last tile: once a pass
+            drain(tail, pass);
             clear_rows<DP, kParts, kY>(dst, len - r0);
             ptx::fence_proxy_async_smem();
             __syncwarp();
@@ -241,23 +246,23 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         mma_weigh<DP, kParts, kApart, kY>(acc, w, 32, d_yt + y, id_a, more);
         if constexpr (kY == 128) mma_weigh<DP, kParts, kApart, kY>(acc, w + 64, 32, d_yt + y + 512, id_a, true);
       };
-      auto run = [&]() {
-        if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(0)) return;
+      auto run = [&](int first) {                 // tiles [first, first + n) of the ring's count
+        if (!ptx::mbar_wait(x_full, 0, abort_flag) || !there(2 * first)) return;
         ptx::tc_fence_after();
-        mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(0), id_s, ksteps);
+        mma_scores<DP, kParts, kY>(tS, d_x, d_y + slot(2 * first), id_s, ksteps);
         ptx::umma_commit(s_full);
-        if (!there(1)) return;
-        mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(1), id_s, ksteps);
+        if (!there(2 * first + 1)) return;
+        mma_scores<DP, kParts, kY>(tD, d_x + (kTB >> 4), d_y + slot(2 * first + 1), id_s, ksteps);
         ptx::umma_commit(dp_full);
-        if (!kKeys) ptx::umma_commit(empty(1));
-        for (int i = 0; i < n; ++i) {
+        if (!kKeys) ptx::umma_commit(empty((2 * first + 1) % kSt));
+        for (int i = first; i < first + n; ++i) {
           const int y1 = 2 * i, y2 = y1 + 1;
-          const bool more = i + 1 < n;
+          const bool more = i + 1 < first + n;
           if (kSt > 2 && more && !there(y1 + 2)) return;                  // what is there long before P
           if (!ptx::mbar_wait(p_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
           if constexpr (kKeys) {
-            weigh(tA1, tS, slot(y2), i > 0);
+            weigh(tA1, tS, slot(y2), i > first);
             ptx::umma_commit(empty(y2 % kSt));    // before the next S: a short ring waits for this tile's place
           }
           if (kSt > 2 && more) {
@@ -267,7 +272,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           if (!ptx::mbar_wait(ds_ready, i & 1, abort_flag)) return;
           ptx::tc_fence_after();
-          weigh(tA2, tD, slot(y1), i > 0);
+          weigh(tA2, tD, slot(y1), i > first);
           ptx::umma_commit(empty(y1 % kSt));
           if (kSt == 2 && more) {                 // the next tiles take the places of these
             if (!there(y1 + 2)) return;
@@ -282,9 +287,16 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
         }
       };
-      run();
+      run(0);
       ptx::umma_commit(done);
-      drain(done, 0);
+      if (kHalf && ptx::mbar_wait(verdict, 0, abort_flag) && *again) {
+        drain(done, 0);
+        run(n);
+        ptx::umma_commit(done);
+        drain(done, 1);
+      } else {
+        drain(done, 0);
+      }
     }
   } else {
     if constexpr (kCols == 256) registers_up_4();
@@ -301,12 +313,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       delta = p.delta[at];
       if constexpr (kHalf) delta = delta * pow2(e_v) * pow2(e_row) * pow2(e_one);
     }
-    float dp_mul = !kHalf ? 1.f : pow2(min(126, e_one + (kParts == 2 ? 0 : e_row + e_v)));   // (126: a row of zeros)
-    if constexpr (kHalf && !kLift) {
-      dp_mul *= pow2(kFixedLift);
-      delta *= pow2(kFixedLift);
-    }
-    int lift = kHalf && !kLift ? kFixedLift : 0;  // of this row: P 2^lift
+    const float dp_mul = !kHalf ? 1.f : pow2(min(126, e_one + (kParts == 2 ? 0 : e_row + e_v)));   // (126: a row of zeros)
+    int lift = 0, scale = 0;                      // of this row: P 2^lift (kLift); dS 2^scale besides the constant one, kLift: 2^(lift + scale)
     const bool row_in = kKeys ? xi < len : true, x_ragged = kKeys && x0 + kRows > len;
     constexpr bool kZeroEach = kKeys && kParts == 2;   // keys that are not there value by value: at the end, both parts spill
     float c = p.c;
@@ -328,42 +336,31 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       }
       tmem_st_wait();
     };
-    // The row's `lift` goes by the exponent of tile i's largest value or sum: what this thread has of the row, and what the row has.  It is
-    // brought to 2^kTop, and may grow to 2^15 afterwards (above 2^35 it is not finite).
-    constexpr int kTop = kKeys && kParts == 2 ? 9 : 11;
-    bool lower = false;                           // the warp's sums are to be taken back, by `fall`
-    float fall = 1.f, own_top = 0.f;
-    auto post = [&](int i, float top) {
-      own_top = top;
+    // What the other half of a row's columns has of a value that this half posts.
+    int turn = 0;
+    auto post = [&](float x) {
       if constexpr (kShared) {
-        row_top[i & 1][half][row] = top;
+        row_top[turn & 1][half][row] = x;
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(pair(warp & 3));
       }
     };
-    auto follow = [&](int i) {
-      float top = own_top;
+    auto other = [&](float mine, float& x) {
+      x = mine;
       if constexpr (kShared) {
-        if (!warp_wait(pair(warp & 3), i & 1, abort_flag)) return false;
-        top = fmaxf(top, row_top[i & 1][half ^ 1][row]);
-      }
-      const int to = kTop - __float2int_rd(fminf(fmaxf(top, -89.f), 35.f));
-      lower = false;
-      fall = 1.f;
-      if (i == 0) {
-        lift = to;
-      } else if (__any_sync(0xffffffffu, lift - to >= 15 - kTop)) {
-        lower = true;
-        if (lift - to >= 15 - kTop) {
-          fall = pow2(to - lift);
-          lift = to;
-        }
+        if (!warp_wait(pair(warp & 3), turn & 1, abort_flag)) return false;
+        x = row_top[turn & 1][half ^ 1][row];
+        ++turn;
       }
       return true;
     };
+    float most = 0.f, most_free = 0.f;            // largest sum of a tile's |dS|, as it is scaled; without 2^lift
     bool ok = true;
+    int pass = 0;
+   run_tiles:
     for (int i = 0; ok && i < n; ++i) {
-      if (!warp_wait(s_full, i & 1, abort_flag)) { ok = false; break; }
+      const int at = pass * n + i;
+      if (!warp_wait(s_full, at & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
       uint32_t s[2][32];
 #pragma unroll
@@ -376,7 +373,7 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       }
       const int valid = kKeys ? kY : len - y_row(i0 + i);   // columns from there on are masked
       const bool ragged = valid < kY;
-      const float* ly = kKeys ? &rows_of_y[(2 * i % kSt) >> 1][0][64 * half] : nullptr;
+      const float* ly = kKeys ? &rows_of_y[(2 * at % kSt) >> 1][0][64 * half] : nullptr;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -397,49 +394,34 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
             }
           }
         }
-      if constexpr (kKeys && kParts == 2) {
-        // P waits for its scale: from the largest exponent, which the other warp has before the exponentials are formed
-        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      bool lower = false;                         // the warp's sums are taken back, by `fall`
+      float fall = 1.f;
+      if constexpr (kLift) {
+        // P waits for its scale: from the largest exponent, which the other warp has before the exponentials are formed.  It is brought to
+        // 2^9 .. 2^10, and may grow to 2^15 afterwards (above 2^35 it is not finite).
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, theirs;
 #pragma unroll
         for (int e = 0; e < 64; e += 8)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             top4[u] = fmaxf(fmaxf(top4[u], __uint_as_float(s[e >> 5][(e & 31) + u])), __uint_as_float(s[e >> 5][(e & 31) + 4 + u]));
-        post(i, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
+        const float largest = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        post(largest);
 #pragma unroll
         for (int e = 0; e < 64; ++e) s[e >> 5][e & 31] = __float_as_uint(exp2_fast(__uint_as_float(s[e >> 5][e & 31])));
-        if (!follow(i)) { ok = false; break; }
-        if (lower) take_back(tA1, fall);
-        lift_row(s, lift);
-      } else if constexpr (kLift) {
-        // only dS waits for it: from the sum, which is at least the largest.  (64 maxima, of half the additions' rate, took a fifth of the
-        // queries' kernel.)
-        if (ragged) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (64 * half + e >= valid) s[e >> 5][e & 31] = 0u;
-        }
-        F2 sum[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          const uint32_t* v = &s[e >> 5][e & 31];
-          const F2 a = f2(__uint_as_float(v[0]), __uint_as_float(v[1])), b = f2(__uint_as_float(v[2]), __uint_as_float(v[3]));
-          F2 &sa = sum[e / 2 & 2], &sb = sum[(e / 2 & 2) + 1];
-          if constexpr (kKeys) {
-            const float4 g4 = *reinterpret_cast<const float4*>(ly + 2 * kY + e);
-            sa = fma2(a, f2(g4.x, g4.y), sa);
-            sb = fma2(b, f2(g4.z, g4.w), sb);
-          } else {
-            sa = add2(sa, a);
-            sb = add2(sb, b);
+        if (!other(largest, theirs)) { ok = false; break; }
+        const int to = 9 - __float2int_rd(fminf(fmaxf(fmaxf(largest, theirs), -89.f), 35.f));
+        if (i == 0) {
+          lift = to;
+        } else if (__any_sync(0xffffffffu, lift - to >= 6)) {
+          lower = true;
+          if (lift - to >= 6) {
+            fall = pow2(to - lift);
+            lift = to;
           }
+          take_back(tA1, fall);
         }
-        float x, y;
-        f2_split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
-        post(i, row_in ? (float)((int)(__float_as_uint(x + y) >> 23) - 127) : -INFINITY);
-        if constexpr (!kKeys) {
-          if (!follow(i)) { ok = false; break; }
-        }
+        lift_row(s, lift);
       }
       if constexpr (kKeys) {
         uint32_t w[32], rest[32];
@@ -459,21 +441,23 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_ready);
-        if constexpr (kLift && kParts == 1) {
-          if (!follow(i)) { ok = false; break; }
-          lift_row(s, lift);
+        if constexpr (kHalf) {                    // the second pass has the row's own scale: with kLift, whatever P's is
+          if (pass) lift_row(s, kLift ? max(-126, scale - lift) : scale);
         }
       }
-      if (!warp_wait(dp_full, i & 1, abort_flag)) { ok = false; break; }
+      if (!warp_wait(dp_full, at & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
       float dm = dp_mul, dd = delta;
-      if constexpr (kLift) {
-        if constexpr (!kKeys) {
-          dm *= pow2(lift);
-          dd *= pow2(lift);
-        }
-        if (lower) take_back(tA2, fall);
+      if constexpr (kHalf && !kKeys) {
+        dm *= pow2(scale);
+        dd *= pow2(scale);
       }
+      if constexpr (kLift) {
+        if (lower && !pass) take_back(tA2, fall);
+      }
+      __half2 sizes[4];                           // sums of |dS| as they are rounded
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sizes[u] = __float2half2_rn(0.f);
       uint32_t w[32], rest[kParts == 2 ? 32 : 1];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -505,6 +489,13 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
           }
           w[16 * k + e / 2] = pack2<T>(v[0], v[1]);
           w[16 * k + e / 2 + 1] = pack2<T>(v[2], v[3]);
+          if constexpr (kHalf) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              __half2& a = sizes[u + (e & 4) / 2];
+              a = __hadd2(a, __habs2(*reinterpret_cast<const __half2*>(&w[16 * k + e / 2 + u])));
+            }
+          }
           if constexpr (kParts == 2) {
             rest[16 * k + e / 2] = pack2_rest(v[0], v[1], w[16 * k + e / 2]);
             rest[16 * k + e / 2 + 1] = pack2_rest(v[2], v[3], w[16 * k + e / 2 + 1]);
@@ -521,18 +512,55 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ds_ready);
+      if constexpr (kHalf) {
+        const float2 x = __half22float2(__hadd2(__hadd2(sizes[0], sizes[1]), __hadd2(sizes[2], sizes[3])));
+        most = fmaxf(most, x.x + x.y);
+        if constexpr (kLift) most_free = fmaxf(most_free, (x.x + x.y) * pow2(-lift));
+      }
     }
     if (ok && n > 0) {
-      ok = warp_wait(done, 0, abort_flag);
+      ok = warp_wait(done, pass, abort_flag);
       ptx::tc_fence_after();
+    }
+    if constexpr (kHalf) {
+      if (ok && n > 0 && !pass) {
+        float theirs;
+        post(most);
+        ok = other(most, theirs);
+        most = fmaxf(most, theirs);
+        if constexpr (kLift) {
+          post(most_free);
+          ok = ok && other(most_free, theirs);
+          most_free = fmaxf(most_free, theirs) * pow2(lift);     // as it would be with the last lift
+        } else {
+          most_free = most;
+        }
+        // What rounding to fp16's smallest step, 2^-24, takes from such a sum: nothing that 22 bits have left, in two parts from 2^0 on, or
+        // 11 bits, in one part from 2^-5 on; nor what a fp16 result shows (|q| or |k| times the scale up to 2^4).  A sum of zero is taken
+        // for 2^-25 where it may be less.
+        const int up = kUp + e_row + e_v + e_one, size = most_free > 0.f ? ilogbf(most_free) : -25;
+        const bool none = nothing || (!kKeys && (e_row == 126 || xi >= p.Lq)), over = most >= 32768.f;
+        const bool under = !none && size < (kParts == 2 ? 0 : -5) && (kParts == 2 || 3 + (31 - __clz(n * kY)) / 2 >= up);
+        const bool off = row_in && (over || under);
+        scale = lift + (over ? (kLift ? 0 : 15) - e_first : (under ? min(100, 11 - size) : 0));
+        if (__any_sync(0xffffffffu, off) && lane == 0) *again = 1;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(verdict);
+        ok = ok && warp_wait(verdict, 0, abort_flag);
+        if (ok && *again) {
+          pass = 1;
+          goto run_tiles;
+        }
+        scale = 0;
+      }
     }
     if (ok) {
       // keys: grad_v and grad_k, by four warps each or one after the other; queries: all channels, or half of them
       const int there = kKeys ? p.Lk : p.Lq;
       const long long rows = (long long)p.B * there * heads, out = ((long long)b * there + xi) * heads + head;
       auto write = [&](bool first, int c0, int c_end) {
-        // what the sums were scaled by: P (by kUp, or lift) and grad_o; P, dP - delta and the other factor
-        const int up = first ? (kParts == 2 ? lift + e_g : kUp) : kUp + lift + e_row + e_v + e_one + (kKeys ? e_q : e_k);
+        // what the sums were scaled by: P and grad_o; dS and the other factor
+        const int up = first ? (kParts == 2 ? lift + e_g : kUp) : kUp + (kLift && pass ? scale : lift + scale) + e_row + e_v + e_one + (kKeys ? e_q : e_k);
         // (three factors: together they may be beyond a float's exponents)
         const int down = max(-378, min(378, -up));
         const float m1 = pow2(down / 3), m2 = pow2((down + 1) / 3), m3 = pow2(down - down / 3 - (down + 1) / 3);

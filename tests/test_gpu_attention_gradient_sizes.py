@@ -130,6 +130,18 @@ def test_probabilities_that_grow_along_the_keys(dtype, d):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("d,at", [(64, 100), (64, 3000), (128, 100)])
+def test_a_large_value_that_nobody_looks_at(dtype, d, at):
+    """A key 36 nats below the others whose value is 2^14 times theirs: it adds nothing to any score gradient."""
+    q, k, v, g = make(300, 3240, d, dtype, 6)
+    q[..., 0] = 6
+    k[..., 0] = 0
+    k[:, at, :, 0] = -6 * d ** 0.5
+    v[:, at] *= 2.0 ** 14
+    check(q, k, v, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_queries_without_a_gradient(dtype):
     """Masked queries: zero gradients give zero rows and change nothing else."""
     q, k, v, g = make(300, 500, 64, dtype, 4)
