@@ -26,12 +26,12 @@
 // difference, as a running softmax does.  (P of fp16 tensors, and of the queries' kernel, is at most 1 and scaled by a constant.)  dS is
 // scaled by what |dP - delta| <= 2 D max|g_y| max|v| allows, less what dS usually lies below that.  How large it was is added up beside its
 // rounding, and if a row of the block was beyond fp16, or so small that its last bits were lost, the block runs over its tiles again, each row
-// with a scale of its own.  Ordinary tensors never need that; one value 2^10 times the others that nobody looks at does, and then costs
+// with a scale of its own.  Ordinary tensors hardly ever need that; one value 2^10 times the others that nobody looks at does, and then costs
 // twice the time instead of 1e-4 of every query's gradient.
 // fp32 gradients are 0.6e-6 .. 1.9e-6 (2-norm) from 64 bits whatever the sizes of grad_o in fp32's normal range and the number of keys
 // (3240 .. 1000000); one scale for all rows lost the queries 2^-20 below the largest altogether, and 4e-5 at 1000000 keys.  Against that
-// (2 x 3240 x 12960, 4 heads, keys + queries): two parts of 64 channels 595 + 413 us for 547 + 378; fp16 of 64 channels 216 + 190 for 208 +
-// 167, of 128 channels 324 + 265 for 380 + 257 (a tile's values of the queries are asked for before its place is free).
+// (2 x 3240 x 12960, 4 heads, keys + queries): two parts of 64 channels 586 + 416 us for 547 + 378; fp16 of 64 channels 217 + 192 for 208 +
+// 167, of 128 channels 325 + 265 for 380 + 257 (a tile's values of the queries are asked for before its place is free).
 #include <algorithm>
 #include <type_traits>
 
@@ -132,7 +132,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     nothing = q[2 * n_heads] == 0u || q[3 * n_heads] == 0u;
     // |g 2^e_g| < 2^15, |v 2^e_v| < 2^15, D products, and delta is no larger: 1 at most, and then what dS is scaled by
     e_one = -31 - (32 - __clz(p.D - 1));
-    e_first = kLift ? 5 : max(22, 32 - __clz(max(len, 2) - 1) + 3);
+    const int bits = 32 - __clz(max(len, 2) - 1); // p is of the order of 2^-bits, dP - delta of 2^-7
+    e_first = kLift ? 5 : (kParts == 2 ? max(22, bits + 3) : max(17, bits));
     e_one += e_first - kUp;
     if constexpr (kParts == 2) {
       e_q = scale_exponent(q[0]);
@@ -357,7 +358,8 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
     float most = 0.f, most_free = 0.f;            // largest sum of a tile's |dS|, as it is scaled; without 2^lift
     bool ok = true;
     int pass = 0;
-   run_tiles:
+    for (bool run = true; run;) {                 // once, or twice: the body keeps its indentation
+    run = false;
     for (int i = 0; ok && i < n; ++i) {
       const int at = pass * n + i;
       if (!warp_wait(s_full, at & 1, abort_flag)) { ok = false; break; }
@@ -547,12 +549,11 @@ bwd_tc_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ C
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(verdict);
         ok = ok && warp_wait(verdict, 0, abort_flag);
-        if (ok && *again) {
-          pass = 1;
-          goto run_tiles;
-        }
-        scale = 0;
+        run = ok && *again;
+        if (run) pass = 1;
+        else scale = 0;
       }
+    }
     }
     if (ok) {
       // keys: grad_v and grad_k, by four warps each or one after the other; queries: all channels, or half of them

@@ -7,7 +7,7 @@ from d2conv3d_b200 import build
 
 # bytes a thread loads back at most.  What spills: the forward with two parts of 128 channels (scores, weights and their rests at a time);
 # layer norm of 32 channels a thread one at a time (rows) or in pairs of positions (volumes); otherwise a handful of set-up values
-MOST = {"fwd_tc_kernel": (8, 456), "bwd_tc_kernel": (16, 150), "few_kernel": (36, 0), "fwd_kernel": (9, 0), "bwd_q_kernel": (9, 88),
+MOST = {"fwd_tc_kernel": (8, 456), "bwd_tc_kernel": (16, 160), "few_kernel": (36, 0), "fwd_kernel": (9, 0), "bwd_q_kernel": (9, 88),
         "bwd_kv_kernel": (9, 24), "combine_kernel": (6, 0), "norm_rows_fwd_kernel": (36, 0), "norm_rows_bwd_kernel": (36, 392),
         "norm_volume_kernel": (120, 252), "rotary_kernel": (18, 60)}
 
